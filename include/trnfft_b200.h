@@ -323,6 +323,86 @@ TRNFFT_API int trnfft_exec_r2c(trnfft_plan_t plan, const float* in, float* out_r
 TRNFFT_API int trnfft_exec_c2r(trnfft_plan_t plan, const float* in_re, const float* in_im, float* out,
                     int64_t batch, void* work, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Sequence and normalisation operators of models over frames (no counterpart
+ * in the reference).  Their operands are real, in the element types below;
+ * states, statistics and the gradients of per-channel parameters are float32.
+ * Pointers are aligned to their element type; 16-byte aligned operands whose
+ * rows are multiples of 16 bytes move in wide accesses. */
+typedef enum { TRNFFT_F32 = 0, TRNFFT_BF16 = 1, TRNFFT_F16 = 2 } trnfft_dtype;
+typedef enum { TRNFFT_ACT_NONE = 0, TRNFFT_ACT_RELU = 1, TRNFFT_ACT_SILU = 2, TRNFFT_ACT_GELU = 3 } trnfft_activation;
+
+/* Shape of a decayed linear attention: q (batch, tokens, heads, key_width),
+ * k (batch, tokens, kv_heads, key_width), v (batch, tokens, kv_heads,
+ * value_width), with strides of batch, token and head in elements and
+ * innermost stride 1.  Query head h reads key and value head
+ * h / (heads / kv_heads).  Outputs and gradients are contiguous; o_stride are
+ * the strides of d_o in the backward call (unused in the forward call).
+ * Widths up to 128.  With cu_seqlens (num_seqs + 1 int32 or int64 values on
+ * the device, ascending), batch is 1 and sequence i is the rows
+ * [cu_seqlens[i], cu_seqlens[i+1]); rows of no sequence get zeros. */
+typedef struct {
+  int64_t batch, tokens, heads, kv_heads, key_width, value_width;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];
+  const void* cu_seqlens;
+  int64_t num_seqs;
+  int32_t cu_is64;
+  int32_t dtype;
+  float scale;
+} trnfft_decay_shape;
+
+/* Bytes of the work area (16-byte aligned) of the forward or backward call; -1 for a bad shape. */
+TRNFFT_API int64_t trnfft_decay_attention_work_bytes(const trnfft_decay_shape* shape, int backward);
+
+/* S_t = exp(log_decay[head]) S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t, from
+ * S = initial (sequences, heads, key_width, value_width) or zero;
+ * final_state (same shape, may be null) receives the last S. */
+TRNFFT_API int trnfft_decay_attention(const trnfft_decay_shape* shape, const void* q, const void* k, const void* v,
+                                      const float* log_decay, const float* initial, void* o, float* final_state,
+                                      void* work, int device, void* stream);
+
+/* Gradients of the above from those of o and (may be null) of the final
+ * state; any of dq, dk, dv and d_initial may be null. */
+TRNFFT_API int trnfft_decay_attention_backward(const trnfft_decay_shape* shape, const void* q, const void* k,
+                                               const void* v, const float* log_decay, const float* initial,
+                                               const void* d_o, const float* d_final, void* dq, void* dk, void* dv,
+                                               float* d_initial, void* work, int device, void* stream);
+
+/* One new token of each of `batch` streams: q (batch, heads, key_width),
+ * k and v (batch, kv_heads, width) with strides of batch and head; states
+ * (batch, heads, key_width, value_width), each stream's contiguous; o
+ * (batch, heads, value_width) contiguous.  new_state may be state itself. */
+typedef struct {
+  int64_t batch, heads, kv_heads, key_width, value_width;
+  int64_t q_stride[2], k_stride[2], v_stride[2];
+  int64_t state_stride, new_state_stride;
+  int32_t dtype;
+  float scale;
+} trnfft_decay_step_shape;
+
+TRNFFT_API int trnfft_decay_attention_step(const trnfft_decay_step_shape* shape, const void* q, const void* k,
+                                           const void* v, const float* log_decay, const float* state, float* new_state,
+                                           void* o, int device, void* stream);
+
+/* Bytes of the work area (16-byte aligned) of the two calls below; -1 for bad sizes. */
+TRNFFT_API int64_t trnfft_group_norm_work_bytes(int64_t batch, int64_t spots, int64_t channels, int64_t groups,
+                                                int dtype, int backward);
+
+/* Group normalisation with an activation over channels-last x (batch, spots,
+ * channels), contiguous: y = act((x - mean) rstd weight + bias), with mean and
+ * rstd = 1 / sqrt(var + eps) over the spots and the channels of a group of one
+ * sample.  weight and bias (channels) may be null; mean and rstd (batch,
+ * groups), which the backward call reads, may both be null.  y may be x. */
+TRNFFT_API int trnfft_group_norm(const void* x, const float* weight, const float* bias, void* y, float* mean,
+                                 float* rstd, int64_t batch, int64_t spots, int64_t channels, int64_t groups, float eps,
+                                 int activation, int dtype, void* work, int device, void* stream);
+
+/* Its gradients; each of dx, dw and db may be null. */
+TRNFFT_API int trnfft_group_norm_backward(const void* x, const void* dy, const float* weight, const float* bias,
+                                          const float* mean, const float* rstd, void* dx, float* dw, float* db,
+                                          int64_t batch, int64_t spots, int64_t channels, int64_t groups,
+                                          int activation, int dtype, void* work, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

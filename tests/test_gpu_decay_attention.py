@@ -1,0 +1,422 @@
+"""Decayed linear attention (whole sequences, gradients, single tokens) against the recurrence in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+import trnfft_b200 as trnfft
+from tests.layer_refs import decay_bound, decay_ref
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def rates(h, kind="mixed"):
+    """log_decay of h heads: memories from 2 tokens to a thousand, or the ends of the range."""
+    if kind == "mixed":
+        return torch.log1p(-1.0 / torch.logspace(0.3, 3.0, h, dtype=torch.float64)).float().cuda()
+    ends = {"none": 0.0, "all": -math.inf, "strong": -60.0}
+    return torch.full((h,), ends[kind]).cuda()
+
+
+def inputs(b, t, h, hk, dk, dv, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*s, scale=1.0):
+        return (torch.randn(*s, device="cuda", generator=g) * scale).to(dtype)
+
+    return normal(b, t, h, dk), normal(b, t, hk, dk, scale=dk ** -0.5), normal(b, t, hk, dv), normal(b, t, h, dv)
+
+
+def check(got, want, total, dtype, terms, what, fp32_out=False):
+    off = (got.double() - want).abs()
+    lim = decay_bound(dtype, terms, total, want, fp32_out)
+    assert got.shape == want.shape, what
+    assert bool((off <= lim).all()), f"{what}: {float((off / lim).max()):.3g} times the bound"
+    norm = float(want.norm())
+    if norm:  # far tighter than the worst case: roundings do not line up
+        rel = {torch.float32: 1e-5, torch.bfloat16: 5e-3, torch.float16: 1e-3}[torch.float32 if fp32_out else dtype]
+        assert float((got.detach().double() - want).norm()) <= rel * norm, what
+
+
+def terms_of(t, dk, dv):
+    return 2 * max(dk, dv) + 128 + t // 32
+
+
+SIZES = [  # batch, time, heads, kv heads, dk, dv
+    (1, 1, 1, 1, 1, 1),
+    (2, 2, 2, 1, 5, 3),
+    (1, 31, 3, 3, 16, 48),
+    (2, 63, 2, 2, 32, 32),
+    (1, 64, 4, 2, 64, 64),
+    (2, 65, 2, 1, 40, 72),
+    (1, 127, 2, 2, 128, 128),
+    (1, 129, 3, 1, 128, 64),
+    (1, 300, 2, 2, 64, 128),
+    (3, 257, 2, 2, 33, 127),
+    (1, 1500, 2, 1, 64, 64),
+    (1, 700, 2, 2, 96, 100),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("carried", [False, True])
+def test_prompt(size, dtype, carried):
+    b, t, h, hk, dk, dv = size
+    q, k, v, _ = inputs(*size, dtype)
+    g = rates(h)
+    first = torch.randn(b, h, dk, dv, device="cuda") if carried else None
+    o, s = trnfft.decay_attention(q, k, v, g, initial_state=first, return_state=True)
+    want, ws = decay_ref(q, k, v, g, dk ** -0.5, first)
+    total, ts = decay_ref(q, k, v, g, dk ** -0.5, first, absolute=True)
+    check(o, want, total, dtype, terms_of(t, dk, dv), "o")
+    check(s, ws, ts, dtype, terms_of(t, dk, dv), "state", fp32_out=True)
+    assert torch.equal(o, trnfft.decay_attention(q, k, v, g, initial_state=first)), "the state is wanted or not"
+
+
+@pytest.mark.parametrize("kind", ["none", "all", "strong"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ends_of_the_decay(kind, dtype):
+    size = (1, 200, 2, 2, 64, 64)
+    q, k, v, do = inputs(*size, dtype)
+    g = rates(2, kind)
+    first = torch.randn(1, 2, 64, 64, device="cuda")
+    o, s = trnfft.decay_attention(q, k, v, g, scale=0.5, initial_state=first, return_state=True)
+    want, ws = decay_ref(q, k, v, g, 0.5, first)
+    total, ts = decay_ref(q, k, v, g, 0.5, first, absolute=True)
+    check(o, want, total, dtype, 400, "o")
+    check(s, ws, ts, dtype, 400, "state", fp32_out=True)
+    q.requires_grad_()
+    (dq,) = torch.autograd.grad(trnfft.decay_attention(q, k, v, g), q, do)
+    assert bool(torch.isfinite(dq).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("carried", [False, True])
+def test_gradients(size, dtype, carried):
+    b, t, h, hk, dk, dv = size
+    q, k, v, do = inputs(*size, dtype, seed=1)
+    g, scale = rates(h), 0.3
+    first = torch.randn(b, h, dk, dv, device="cuda") if carried else None
+    dlast = torch.randn(b, h, dk, dv, device="cuda") if carried else None
+    leaves = [x.requires_grad_() for x in ([q, k, v, first] if carried else [q, k, v])]
+    o, s = trnfft.decay_attention(q, k, v, g, scale=scale, initial_state=first, return_state=True)
+    got = torch.autograd.grad((o, s) if carried else o, leaves, (do, dlast) if carried else do)
+
+    def ref(absolute):
+        f = (lambda x: x.detach().double().abs()) if absolute else (lambda x: x.detach().double())
+        xs = [f(x).requires_grad_() for x in leaves]
+        o, s = decay_ref(*xs[:3], g, scale, xs[3] if carried else None)
+        return torch.autograd.grad((o, s) if carried else o, xs, (f(do), f(dlast)) if carried else f(do))
+
+    for name, x, w, tot in zip(("dq", "dk", "dv", "dinitial"), got, ref(False), ref(True)):
+        check(x, w, tot, dtype, terms_of(t, dk, dv) * (h // hk), name, fp32_out=name == "dinitial")
+
+
+def test_gradients_against_differences():
+    """o is linear in each operand, so central differences of any width are exact but for rounding."""
+    q, k, v, do = inputs(1, 90, 2, 1, 16, 24, torch.float32, seed=2)
+    first = torch.randn(1, 2, 16, 24, device="cuda")
+    g = rates(2)
+    leaves = [q, k, v, first]
+    for x in leaves:
+        x.requires_grad_()
+    o = trnfft.decay_attention(q, k, v, g, initial_state=first)
+    grads = torch.autograd.grad(o, leaves, do)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    for i, (x, dx) in enumerate(zip(leaves, grads)):
+        d = torch.randn(x.shape, device="cuda", generator=gen)
+        with torch.no_grad():
+            ends = [trnfft.decay_attention(*(y + e * d if j == i else y for j, y in enumerate(leaves[:3])), g,
+                                           initial_state=first + e * d if i == 3 else first) for e in (1.0, -1.0)]
+        want = ((ends[0].double() - ends[1].double()) / 2 * do.double()).sum()
+        size = float(do.double().norm() * ends[0].double().norm())
+        assert abs(float((dx.double() * d.double()).sum() - want)) < 1e-5 * size
+
+
+def test_gradients_of_some_inputs_and_of_the_state_alone():
+    q, k, v, do = inputs(2, 70, 4, 2, 32, 40, torch.bfloat16)
+    g = rates(4)
+    for x in (q, k, v):
+        x.requires_grad_()
+    o, s = trnfft.decay_attention(q, k, v, g, return_state=True)
+    full = torch.autograd.grad(o, (q, k, v), do, retain_graph=True)
+    for i, x in enumerate((q, k, v)):
+        args = [y if j == i else y.detach() for j, y in enumerate((q, k, v))]
+        (one,) = torch.autograd.grad(trnfft.decay_attention(*args, g), x, do)
+        assert torch.equal(one, full[i])
+    first = torch.zeros(2, 4, 32, 40, device="cuda", requires_grad=True)
+    (di,) = torch.autograd.grad(trnfft.decay_attention(q.detach(), k.detach(), v.detach(), g, initial_state=first), first, do)
+    assert float(di.abs().max()) > 0
+    ds = torch.randn_like(s)
+    dq, dk, dv = torch.autograd.grad(s, (q, k, v), ds)
+    kd, vd = (x.detach().double().requires_grad_() for x in (k, v))
+    _, sd = decay_ref(q.detach(), kd, vd, g, 1.0)
+    wk, wv = torch.autograd.grad(sd, (kd, vd), ds.double())
+    assert float(dq.abs().max()) == 0
+    assert float((dk.double() - wk).norm() / wk.norm()) < 5e-3 and float((dv.double() - wv).norm() / wv.norm()) < 5e-3
+    # a gradient that is one value broadcast
+    o = trnfft.decay_attention(q, k, v, g)
+    a = torch.autograd.grad(o.sum(), q, retain_graph=True)[0]
+    assert torch.equal(a, torch.autograd.grad(o, q, torch.ones_like(o))[0])
+    with pytest.raises(RuntimeError):  # differentiable once only
+        o = trnfft.decay_attention(q, k, v, g)
+        d1 = torch.autograd.grad(o.sum(), q, create_graph=True)[0]
+        torch.autograd.grad(d1.sum(), k)
+
+
+LENGTHS = [
+    ([5], 0, 0),
+    ([0], 0, 0),
+    ([1, 0, 64, 63, 65, 0, 300, 2], 0, 3),
+    ([128, 128, 1], 4, 0),
+    ([700, 1, 90], 7, 9),
+    ([0, 0, 0], 3, 2),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,before,behind", LENGTHS)
+def test_packed(lengths, before, behind, dtype):
+    h, hk, dk, dv = 4, 2, 48, 64
+    total = before + sum(lengths) + behind
+    q, k, v, do = inputs(1, total, h, hk, dk, dv, dtype, seed=3)
+    g, n = rates(h), len(lengths)
+    cu = torch.tensor([before, *lengths]).cumsum(0).cuda()
+    first, dlast = (torch.randn(n, h, dk, dv, device="cuda") for _ in range(2))
+    leaves = [x.requires_grad_() for x in (q, k, v, first)]
+    for c in (cu, cu.int()):
+        o, s = trnfft.decay_attention(q, k, v, g, initial_state=first, cu_seqlens=c, return_state=True)
+    got = torch.autograd.grad((o, s), leaves, (do, dlast))
+    outside = torch.ones(total, dtype=torch.bool, device="cuda")
+    for i, (x, y) in enumerate(zip(cu.tolist(), cu.tolist()[1:])):
+        outside[x:y] = False
+        xs = [z.detach()[:, x:y].double().requires_grad_() for z in (q, k, v)] + [first.detach()[i:i + 1].double().requires_grad_()]
+        wo, ws = decay_ref(*xs[:3], g, dk ** -0.5, xs[3])
+        ab = [z.detach().abs().requires_grad_() for z in xs]
+        to, ts = decay_ref(*ab[:3], g, dk ** -0.5, ab[3])
+        terms = terms_of(y - x, dk, dv)
+        check(o[:, x:y], wo.detach(), to.detach(), dtype, terms, f"o of {i}")
+        check(s[i:i + 1], ws.detach(), ts.detach(), dtype, terms, f"state of {i}", fp32_out=True)
+        if x == y:
+            assert torch.equal(got[3][i], dlast[i])
+            continue
+        wg = torch.autograd.grad((wo, ws), xs, (do[:, x:y].double(), dlast[i:i + 1].double()))
+        tg = torch.autograd.grad((to, ts), ab, (do[:, x:y].double().abs(), dlast[i:i + 1].double().abs()))
+        for name, z, w, t in zip(("dq", "dk", "dv"), got, wg, tg):
+            check(z[:, x:y], w, t, dtype, 2 * terms, f"{name} of {i}")
+        check(got[3][i:i + 1], wg[3], tg[3], dtype, terms, f"dinitial of {i}", fp32_out=True)
+    for z in (o.detach(), *got[:3]):
+        assert float(z[:, outside].abs().sum()) == 0, "rows of no sequence are zero"
+
+
+def test_packed_of_no_sequence():
+    q, k, v, _ = inputs(1, 9, 2, 2, 16, 16, torch.float32)
+    cu = torch.tensor([4], dtype=torch.int32, device="cuda")
+    o, s = trnfft.decay_attention(q, k, v, rates(2), cu_seqlens=cu, return_state=True)
+    assert s.shape == (0, 2, 16, 16) and float(o.abs().sum()) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layouts_and_alignment(dtype):
+    """Any order of the dimensions, gaps, broadcast heads and addresses off the 16-byte grid."""
+    b, t, h, hk, dk, dv = 2, 130, 4, 2, 64, 64
+    q, k, v, do = inputs(b, t, h, hk, dk, dv, dtype, seed=4)
+    g = rates(h)
+    want = trnfft.decay_attention(q, k, v, g)
+    heads_first = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    assert torch.equal(trnfft.decay_attention(*heads_first, g), want)
+    joined = torch.cat([q, k, v], 2)
+    assert torch.equal(trnfft.decay_attention(joined[:, :, :h], joined[:, :, h:h + hk], joined[:, :, h + hk:], g), want)
+    shifted = []
+    for x in (q, k, v):
+        y = torch.empty(x.numel() + 1, dtype=dtype, device="cuda")[1:].view(x.shape)
+        shifted.append(y.copy_(x))
+    assert torch.equal(trnfft.decay_attention(*shifted, g), want)
+    gaps = [torch.nn.functional.pad(x, (1, 2))[..., 1:-2] for x in (q, k, v)]
+    assert torch.equal(trnfft.decay_attention(*gaps, g), want)
+    inner = [x.transpose(-1, -2).contiguous().transpose(-1, -2) for x in (q, k, v)]
+    assert torch.equal(trnfft.decay_attention(*inner, g), want)
+    k1, v1 = k[:, :, :1].expand(-1, -1, hk, -1), v[:, :1].expand(-1, t, -1, -1)
+    assert torch.equal(trnfft.decay_attention(q, k1, v1, g), trnfft.decay_attention(q, k1.contiguous(), v1.contiguous(), g))
+    q.requires_grad_()
+    o = trnfft.decay_attention(q, k, v, g)
+    do2 = do.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(torch.autograd.grad(o, q, do2, retain_graph=True)[0], torch.autograd.grad(o, q, do)[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_continued_sequences_and_single_tokens(dtype):
+    """A sequence in one call, in two, and token by token."""
+    b, t, h, hk, dk, dv = 2, 150, 4, 2, 40, 56
+    q, k, v, _ = inputs(b, t, h, hk, dk, dv, dtype, seed=6)
+    g = rates(h)
+    want, ws = decay_ref(q, k, v, g, dk ** -0.5)
+    total, ts = decay_ref(q, k, v, g, dk ** -0.5, absolute=True)
+    o1, s = trnfft.decay_attention(q[:, :77], k[:, :77], v[:, :77], g, return_state=True)
+    o2, s = trnfft.decay_attention(q[:, 77:], k[:, 77:], v[:, 77:], g, initial_state=s, return_state=True)
+    terms = 2 * terms_of(t, dk, dv)
+    check(torch.cat([o1, o2], 1), want, total, dtype, terms, "two calls")
+    check(s, ws, ts, dtype, terms, "state of two calls", fp32_out=True)
+    pool = torch.randn(b, 3, h, dk, dv, device="cuda")
+    state = pool[:, 1].zero_()
+    others = pool[:, ::2].clone()
+    rows = []
+    for i in range(t):
+        o, got = trnfft.decay_attention_step(q[:, i], k[:, i], v[:, i], g, state)
+        assert got is state
+        rows.append(o)
+    check(torch.stack(rows, 1), want, total, dtype, terms + t, "token by token")
+    check(state, ws, ts, dtype, terms + t, "state token by token", fp32_out=True)
+    assert torch.equal(pool[:, ::2], others)
+
+
+@pytest.mark.parametrize("size", [(1, 1, 1, 1, 1), (3, 4, 2, 5, 7), (2, 2, 1, 64, 64), (5, 8, 4, 40, 72), (70, 2, 2, 128, 128),
+                                  (2, 3, 3, 127, 33), (300, 4, 1, 32, 96), (1, 2, 2, 128, 4)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_step(size, dtype):
+    b, h, hk, dk, dv = size
+    q, k, v, _ = (x[:, 0] for x in inputs(b, 1, h, hk, dk, dv, dtype, seed=7))
+    g = rates(h)
+    state = torch.randn(b, h, dk, dv, device="cuda")
+    want, ws = decay_ref(q[:, None], k[:, None], v[:, None], g, 0.7, state)
+    total, ts = decay_ref(q[:, None], k[:, None], v[:, None], g, 0.7, state, absolute=True)
+    kept, new = state.clone(), torch.full_like(state, float("nan"))
+    o, got = trnfft.decay_attention_step(q, k, v, g, state, scale=0.7, new_state=new)
+    assert got is new and torch.equal(state, kept)
+    check(o, want[:, 0], total[:, 0], dtype, dk + 8, "o")
+    check(new, ws, ts, dtype, 4, "state", fp32_out=True)
+    o2, _ = trnfft.decay_attention_step(q, k, v, g, state, scale=0.7)
+    assert torch.equal(o, o2) and torch.equal(state, new)
+    wide = torch.empty(b, 2 * h * dk * dv + 1, device="cuda")[:, 1:1 + h * dk * dv].view(b, h, dk, dv)  # off the 16-byte grid
+    wide.copy_(kept)
+    o3, _ = trnfft.decay_attention_step(q, k, v, g, wide, scale=0.7)
+    assert float((o3.double() - o.double()).abs().max()) <= float(decay_bound(dtype, dk + 8, total[:, 0], want[:, 0]).max())
+    check(wide, ws, ts, dtype, 4, "state", fp32_out=True)
+
+
+def test_step_refuses_overlap():
+    s = torch.zeros(3, 2, 8, 8, device="cuda")
+    q = torch.zeros(2, 2, 8, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        trnfft.decay_attention_step(q, q, q, torch.zeros(2).cuda(), s[:2], new_state=s[1:])
+    kept = torch.ones(2, 2, 8, 8, device="cuda", requires_grad=True) * 1.0
+    loss = (kept * kept).sum()
+    with torch.no_grad():
+        trnfft.decay_attention_step(q, q, q, torch.zeros(2).cuda(), kept)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+
+
+def test_empty_calls():
+    q, k, v, _ = inputs(2, 0, 2, 2, 8, 8, torch.float32)
+    first = torch.randn(2, 2, 8, 8, device="cuda", requires_grad=True)
+    o, s = trnfft.decay_attention(q, k, v, rates(2), initial_state=first, return_state=True)
+    assert o.shape == (2, 0, 2, 8) and torch.equal(s, first)
+    (d,) = torch.autograd.grad(s, first, torch.ones_like(s))
+    assert torch.equal(d, torch.ones_like(s))
+    _, s = trnfft.decay_attention(q, k, v, rates(2), return_state=True)
+    assert float(s.abs().sum()) == 0
+    q, k, v, _ = inputs(0, 5, 2, 2, 8, 8, torch.float32)
+    o, s = trnfft.decay_attention(q, k, v, rates(2), return_state=True)
+    assert o.shape == (0, 5, 2, 8) and s.shape == (0, 2, 8, 8)
+    o, s = trnfft.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], rates(2), s)
+    assert o.shape == (0, 2, 8)
+
+
+def test_other_values_stay_in_their_rows():
+    """NaN and infinity at one token reach that token and later ones of its head and sequence, nothing else."""
+    q, k, v, _ = inputs(2, 200, 2, 2, 64, 64, torch.bfloat16)
+    g = rates(2)
+    want = trnfft.decay_attention(q, k, v, g)
+    for bad in (float("nan"), float("inf")):
+        v2 = v.clone()
+        v2[1, 100, 0] = bad
+        o = trnfft.decay_attention(q, k, v2, g)
+        assert torch.equal(o[0], want[0]) and torch.equal(o[1, :, 1], want[1, :, 1])
+        assert not bool(torch.isfinite(o[1, 100, 0]).any())
+        packed = trnfft.decay_attention(*(x.reshape(1, 400, 2, 64) for x in (q, k, v2)), g,
+                                        cu_seqlens=torch.tensor([0, 150, 290, 310, 400], device="cuda"))
+        assert bool(torch.isfinite(packed[0, :290]).all()) and bool(torch.isfinite(packed[0, 310:]).all())
+
+
+def test_cpu_tensors_and_devices():
+    q, k, v, _ = inputs(1, 20, 2, 2, 16, 16, torch.float32)
+    g = rates(2)
+    want, ws = trnfft.decay_attention(q, k, v, g, return_state=True)
+    o, s = trnfft.decay_attention(q.cpu(), k.cpu(), v.cpu(), g.cpu(), return_state=True)
+    assert not o.is_cuda and not s.is_cuda and torch.equal(o, want.cpu()) and torch.equal(s, ws.cpu())
+    state = ws.cpu()
+    o, got = trnfft.decay_attention_step(q[:, 0].cpu(), k[:, 0].cpu(), v[:, 0].cpu(), g.cpu(), state)
+    o2, s2 = trnfft.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, ws)
+    assert got is state and torch.equal(o, o2.cpu()) and torch.equal(state, s2.cpu())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_streams_and_graphs(dtype):
+    """A captured training step, replayed on new values, beside eager ones on another stream."""
+    size = (2, 400, 4, 2, 64, 64)
+    q, k, v, do = inputs(*size, dtype, seed=8)
+    g = rates(4)
+    for x in (q, k, v):
+        x.requires_grad_()
+
+    def step():
+        o, s = trnfft.decay_attention(q, k, v, g, return_state=True)
+        return (o.detach(), s.detach(), *torch.autograd.grad(o, (q, k, v), do))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step()
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(kept, eager))
+    with torch.no_grad():
+        for x, y in zip((q, k, v, do), inputs(*size, dtype, seed=9)):
+            x.copy_(y)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(kept, step()))
+
+
+def test_two_graphs_do_not_share_workspaces():
+    g = rates(2)
+    sets = [inputs(1, 3000, 2, 2, 64, 64, torch.float32, seed=s)[:3] for s in (1, 2)]
+    want = [trnfft.decay_attention(*x, g, return_state=True) for x in sets]
+    graphs, got = [], []
+    for x in sets:
+        trnfft.decay_attention(*x, g)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(trnfft.decay_attention(*x, g, return_state=True))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, x in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                x.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_offsets_past_32_bits():
+    """Strides that lead more than 2^31 elements away."""
+    t, far = 70, (1 << 31) + 64
+    q, k, v, _ = inputs(2, t, 1, 1, 64, 64, torch.bfloat16, seed=10)
+    want = trnfft.decay_attention(q, k, v, rates(1))
+    pool = torch.empty(far + t * 64, dtype=torch.bfloat16, device="cuda")
+    views = []
+    y = torch.as_strided(pool, q.shape, (far, 64, 64, 1))
+    y.copy_(q)
+    views.append(y)
+    assert torch.equal(trnfft.decay_attention(y, k, v, rates(1)), want)
+    y.copy_(v)
+    assert torch.equal(trnfft.decay_attention(q, k, y, rates(1)), want)

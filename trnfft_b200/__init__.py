@@ -10,6 +10,8 @@ hand-written CUDA kernels through the C ABI in include/trnfft_b200.h::
 
 __version__ = "0.1.0"
 
+from ._attention import decay_attention, decay_attention_step
+from ._norm import group_norm
 from .api import (
     fft,
     fft2,
@@ -41,7 +43,7 @@ def set_ozaki_product_precision_verified(verified: bool) -> None:
 __all__ = [
     "fft", "ifft", "rfft", "hfft", "ihfft", "irfft", "fft2", "fftn", "ifftn", "rfft2", "irfft2",
     "rfftn", "irfftn", "stft", "istft",
-    "ComplexTensor", "complex_matmul",
+    "ComplexTensor", "complex_matmul", "decay_attention", "decay_attention_step", "group_norm",
     "create_plan", "clear_plan_cache", "FFTPlan", "set_small_n_algorithm", "get_small_n_algorithm",
     "HAS_NKI", "set_backend", "get_backend",
     "set_precision", "set_ozaki_product_precision_verified", "get_precision",

@@ -33,6 +33,24 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 
+
+class DecayShape(ctypes.Structure):
+    """trnfft_decay_shape"""
+
+    _fields_ = [(n, _I64) for n in ("batch", "tokens", "heads", "kv_heads", "key_width", "value_width")] + [
+        (n, _I64 * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + [
+        ("cu_seqlens", _P), ("num_seqs", _I64), ("cu_is64", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float)]
+
+
+class DecayStepShape(ctypes.Structure):
+    """trnfft_decay_step_shape"""
+
+    _fields_ = [(n, _I64) for n in ("batch", "heads", "kv_heads", "key_width", "value_width")] + [
+        (n, _I64 * 2) for n in ("q_stride", "k_stride", "v_stride")] + [
+        ("state_stride", _I64), ("new_state_stride", _I64), ("dtype", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/trnfft_b200.h declares
 SIGNATURES = {
     "trnfft_abi_version": (_INT, []),
@@ -68,6 +86,13 @@ SIGNATURES = {
     "trnfft_exec_istft": (_INT, [_P, _P, _P, _I64, _I64, _I64, _P, _INT, _INT, _INT, _I64, _P, _P]),
     "trnfft_complex_mask_apply": (_INT, [_P, _P, _I64, _P, _P, _P, _P, _I64, _INT, _P]),
     "trnfft_exec_c2r": (_INT, [_P, _P, _P, _P, _I64, _P, _P]),
+    "trnfft_decay_attention_work_bytes": (_I64, [ctypes.POINTER(DecayShape), _INT]),
+    "trnfft_decay_attention": (_INT, [ctypes.POINTER(DecayShape)] + [_P] * 8 + [_INT, _P]),
+    "trnfft_decay_attention_backward": (_INT, [ctypes.POINTER(DecayShape)] + [_P] * 12 + [_INT, _P]),
+    "trnfft_decay_attention_step": (_INT, [ctypes.POINTER(DecayStepShape)] + [_P] * 7 + [_INT, _P]),
+    "trnfft_group_norm_work_bytes": (_I64, [_I64] * 4 + [_INT, _INT]),
+    "trnfft_group_norm": (_INT, [_P] * 6 + [_I64] * 4 + [ctypes.c_float, _INT, _INT, _P, _INT, _P]),
+    "trnfft_group_norm_backward": (_INT, [_P] * 9 + [_I64] * 4 + [_INT, _INT, _P, _INT, _P]),
 }
 
 
@@ -109,12 +134,20 @@ def call(name: str, *args) -> None:
     lib = load()
     rc = getattr(lib, name)(*args)
     if rc != SUCCESS:
-        msg = lib.trnfft_last_error().decode(errors="replace")
-        if rc == UNSUPPORTED:
-            raise NotImplementedError(f"{name}: {msg}")
-        if rc == INVALID_VALUE:
-            raise ValueError(f"{name}: {msg}")
-        raise TrnfftError(name, rc, msg)
+        _raise(name, rc, lib.trnfft_last_error().decode(errors="replace"))
+
+
+def _raise(name: str, rc: int, msg: str) -> None:
+    if rc == UNSUPPORTED:
+        raise NotImplementedError(f"{name}: {msg}")
+    if rc == INVALID_VALUE:
+        raise ValueError(f"{name}: {msg}")
+    raise TrnfftError(name, rc, msg)
+
+
+def raise_last(name: str) -> None:
+    """Raise for a size query that returned -1 (its sizes are not supported)."""
+    _raise(name, UNSUPPORTED, load().trnfft_last_error().decode(errors="replace"))
 
 
 def device_status(device_index: int, clear: bool = True) -> int:

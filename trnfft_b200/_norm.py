@@ -1,0 +1,98 @@
+"""Group normalisation with an activation over channels-last features (trnfft_group_norm)."""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._attention import DTYPES, _addr
+from ._device import place_layer
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _work(n, s, c, groups, dtype, backward, device):
+    size = _lib.load().trnfft_group_norm_work_bytes(n, s, c, groups, dtype, backward)
+    if size < 0:
+        _lib.raise_last("trnfft_group_norm_work_bytes")
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def _forward(x, groups, weight, bias, eps, act, keep):
+    n, c = x.shape[0], x.shape[-1]
+    s = x.numel() // (n * c) if n else 0
+    y = torch.empty_like(x)
+    stats = torch.empty(2, n, groups, dtype=torch.float32, device=x.device) if keep else None
+    dt = DTYPES[x.dtype]
+    work = _work(n, s, c, groups, dt, 0, x.device)
+    at = stats.data_ptr() if keep else None
+    _lib.call("trnfft_group_norm", x.data_ptr(), _addr(weight), _addr(bias), y.data_ptr(), at,
+              at + 4 * n * groups if keep else None, n, s, c, groups, eps, act, dt, _addr(work), x.device.index,
+              torch.cuda.current_stream(x.device).cuda_stream)
+    return y, stats
+
+
+class _GroupNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        w = None if weight is None else weight.float()
+        b = None if bias is None else bias.float()
+        y, stats = _forward(x, groups, w, b, eps, act, True)
+        ctx.save_for_backward(x, w, b, stats)
+        ctx.groups, ctx.act = groups, act
+        ctx.types = (weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, b, stats = ctx.saved_tensors
+        groups, need = ctx.groups, ctx.needs_input_grad
+        n, c = x.shape[0], x.shape[-1]
+        s = x.numel() // (n * c) if n else 0
+        dy = dy.contiguous()
+        dx = torch.empty_like(x) if need[0] else None
+        dw, db = (torch.empty(c, dtype=torch.float32, device=x.device) if f else None for f in need[1:3])
+        dt = DTYPES[x.dtype]
+        work = _work(n, s, c, groups, dt, 1, x.device)
+        at = stats.data_ptr()
+        _lib.call("trnfft_group_norm_backward", x.data_ptr(), dy.data_ptr(), _addr(w), _addr(b), at, at + 4 * n * groups,
+                  _addr(dx), _addr(dw), _addr(db), n, s, c, groups, ctx.act, dt, _addr(work), x.device.index,
+                  torch.cuda.current_stream(x.device).cuda_stream)
+        dw, db = (g if g is None else g.to(t) for g, t in zip((dw, db), ctx.types))
+        return dx, dw, db, None, None, None
+
+
+def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, activation: str | None = None) -> torch.Tensor:
+    """act(group_norm(x)) over channels-last features, in one operator.
+
+    x is (batch, ..., channels), float32, bfloat16 or float16.  The channels fall into
+    num_groups groups; each group of each sample is normalised by its mean and variance
+    over all positions (statistics in float32), then scaled by weight and shifted by bias
+    (channels each, optional) and put through the activation: None, "relu", "silu" or
+    "gelu" (the exact one, with erf).  Differentiable once in x, weight and bias.
+    """
+    if x.dim() < 2:
+        raise ValueError(f"group_norm: x must be (batch, ..., channels), got {tuple(x.shape)}")
+    if x.dtype not in DTYPES:
+        raise ValueError(f"group_norm: x must be float32, bfloat16 or float16, got {x.dtype}")
+    c, num_groups = x.shape[-1], int(num_groups)
+    if c < 1 or num_groups < 1 or c % num_groups:
+        raise ValueError(f"group_norm: {c} channels do not fall into {num_groups} groups")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"group_norm: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
+    if not eps >= 0:
+        raise ValueError(f"group_norm: eps must not be negative, got {eps}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.shape != (c,) or p.dtype not in DTYPES):
+            raise ValueError(f"group_norm: {name} must hold {c} values in float32, bfloat16 or float16, got {p.dtype} "
+                             f"{tuple(p.shape)}")
+    (x, weight, bias), restore = place_layer("group_norm", x, weight, bias)
+    x = x.contiguous()
+    weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(p is not None and p.requires_grad for p in (x, weight, bias)):
+        return restore(_GroupNormFn.apply(x, weight, bias, num_groups, eps, act))
+    w, b = (None if p is None else p.float() for p in (weight, bias))
+    return restore(_forward(x, num_groups, w, b, eps, act, False)[0])

@@ -1,0 +1,79 @@
+// Internal interface of the decayed linear attention kernels (decay_attn.cu,
+// decay_step.cu) and their C-ABI layer (capi_layers.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace tfb {
+
+enum ElemType { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+// One "role": the operator
+//   o_t = a sum_{s<=t} g^{t-s} (q_t . k_s) v_s + r g^{t+1-back} q_t C
+//   C'  = g^n C + c sum_s g^{n-1-s+back} k_s v_s^T
+// over the n tokens of every sequence and every head, in time order
+// (back = 0) or from the last token to the first (back = 1).  The forward
+// pass is one role; the backward pass is three (see decay_attn.cu).
+struct DecayRole {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;                     // null: only the state is wanted
+  long long qs[3], ks[3], vs[3], os[3];  // strides of batch, token, head (elements; innermost 1)
+  int qdiv, kdiv, vdiv;        // head h reads head h / div
+  int wk, wv;                  // widths: of q and k, of v and o
+  int back;
+  float a, r, c;
+  int o_f32;                   // o is float32 whatever the element type
+  const float* first;          // carried-in state or null; element (k, v) of (sequence, head) at
+  long long first_sk, first_sv;  //   (seq*heads + head)*wk*wv + k*first_sk + v*first_sv
+  float* last;                 // final state (wk x wv, row-major) or null
+  float* seg;                  // states of the segments, (unit, head, wk, wv)
+};
+
+constexpr int kMaxRoles = 3;
+
+struct DecayArgs {
+  DecayRole role[kMaxRoles];
+  int roles;
+  int heads;
+  const float* log_decay;
+  // dense: nseq sequences of `tokens` rows, sequence = batch row.  packed
+  // (cu != null): sequence i is rows [cu[i], cu[i+1]) of batch row 0.
+  long long tokens;
+  int nseq;
+  const void* cu;
+  int cu64;
+  // work units: a unit is one segment (seg_len tokens, a multiple of the
+  // chunk) of one sequence; dense: seq = unit / segs.  packed: found from cu;
+  // `units` bounds their number, and unit index `units` zeroes the rows of o
+  // that belong to no sequence.
+  int seg_len;
+  int segs;
+  int units;
+};
+
+cudaError_t launch_decay_attention(ElemType t, const DecayArgs& a, cudaStream_t st);
+
+// out[row][hk][w] = sum over g < group of in[row][hk*group + g][w], float32 in, element type out.
+cudaError_t launch_sum_heads(ElemType t, const float* in, void* out, long long rows, int kv_heads, int group, int width,
+                             cudaStream_t st);
+
+struct DecayStepArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  long long qs[2], ks[2], vs[2];  // strides of batch, head
+  void* o;                        // (batch, heads, dv) contiguous
+  const float* state;
+  float* next;
+  long long state_s, next_s;      // batch strides; (head, dk, dv) contiguous
+  const float* log_decay;
+  int batch, heads, group, dk, dv;
+  float scale;
+};
+
+cudaError_t launch_decay_step(ElemType t, const DecayStepArgs& a, cudaStream_t st);
+
+}  // namespace tfb

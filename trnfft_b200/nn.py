@@ -4,7 +4,9 @@
 GEMM (``trnfft_b200.nki.dispatch.complex_linear``).  ``ComplexConv1d``,
 ``ComplexBatchNorm1d`` and ``ComplexModReLU`` are kept for API compatibility
 (same parameters and values as trnfft/nn.py:52-129); they are off the FFT hot
-path and written as plain torch compositions.
+path and written as plain torch compositions.  ``GroupNorm``,
+``ComplexGroupNorm`` and ``ComplexDecayAttention`` have no counterpart there;
+they run the library's group norm and decayed linear attention kernels.
 """
 
 from __future__ import annotations
@@ -14,6 +16,8 @@ import math
 import torch
 import torch.nn as nn
 
+from ._attention import decay_attention, decay_attention_step
+from ._norm import group_norm
 from .complex import ComplexTensor
 
 
@@ -111,3 +115,79 @@ class ComplexModReLU(nn.Module):
         r = x.abs()
         gain = torch.relu(r + self.bias) / r.clamp_min(1e-8)
         return ComplexTensor(x.real * gain, x.imag * gain)
+
+
+class GroupNorm(nn.Module):
+    """Group normalisation of channels-last features, with an activation (``trnfft_b200.group_norm``).
+
+    Unlike batch statistics it needs no other sample and no running average, so a stream of
+    single frames gets the values that training saw."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True,
+                 activation: str | None = None):
+        super().__init__()
+        self.num_groups, self.eps, self.activation = num_groups, eps, activation
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+
+
+class ComplexGroupNorm(nn.Module):
+    """Group normalisation of the real and the imaginary plane, each with its own statistics and
+    parameters as in ``ComplexBatchNorm1d``, over channels-last features (batch, ..., channels)."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, activation: str | None = None):
+        super().__init__()
+        self.gn_re = GroupNorm(num_groups, num_channels, eps, activation=activation)
+        self.gn_im = GroupNorm(num_groups, num_channels, eps, activation=activation)
+
+    def forward(self, x: ComplexTensor) -> ComplexTensor:
+        return ComplexTensor(self.gn_re(x.real), self.gn_im(x.imag))
+
+
+class ComplexDecayAttention(nn.Module):
+    """Mixing along time for complex features (batch, frames, features): decayed linear attention
+    between ``ComplexLinear`` projections, each head's output normalised for itself.
+
+    A head of complex width w is a real head of width 2w over [re, im], so scores are
+    Re(q conj(k)).  ``forward`` runs whole sequences; ``step`` one frame (batch, features) of each
+    stream on the state that ``forward(..., return_state=True)`` or ``initial_state`` gives, in
+    place.  Head h forgets over 2^(3 + 6h/(heads-1)) frames."""
+
+    def __init__(self, features: int, heads: int, head_width: int):
+        super().__init__()
+        self.heads, self.head_width = heads, head_width
+        self.q = ComplexLinear(features, heads * head_width, bias=False)
+        self.k = ComplexLinear(features, heads * head_width, bias=False)
+        self.v = ComplexLinear(features, heads * head_width, bias=False)
+        self.norm = GroupNorm(heads, 2 * heads * head_width)
+        self.out = ComplexLinear(heads * head_width, features)
+        memory = 2.0 ** (3.0 + 6.0 * torch.arange(heads, dtype=torch.float64) / max(1, heads - 1))
+        self.register_buffer("log_decay", torch.log1p(-1.0 / memory).float())
+
+    def _heads(self, x: ComplexTensor) -> torch.Tensor:
+        planes = [p.unflatten(-1, (self.heads, self.head_width)) for p in (x.real, x.imag)]
+        return torch.cat(planes, dim=-1)
+
+    def _project(self, o: torch.Tensor) -> ComplexTensor:
+        o = self.norm(o.reshape(-1, 2 * self.heads * self.head_width)).view(o.shape)
+        re, im = (p.flatten(-2) for p in o.split(self.head_width, dim=-1))
+        return self.out(ComplexTensor(re, im))
+
+    def initial_state(self, batch: int, device=None) -> torch.Tensor:
+        w = 2 * self.head_width
+        return torch.zeros(batch, self.heads, w, w, device=self.log_decay.device if device is None else device)
+
+    def forward(self, x: ComplexTensor, state: torch.Tensor | None = None, return_state: bool = False):
+        q, k, v = (self._heads(p(x)) for p in (self.q, self.k, self.v))
+        o, last = decay_attention(q, k, v, self.log_decay, initial_state=state, return_state=True)
+        y = self._project(o)
+        return (y, last) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x: ComplexTensor, state: torch.Tensor) -> ComplexTensor:
+        q, k, v = (self._heads(p(x)) for p in (self.q, self.k, self.v))
+        o, _ = decay_attention_step(q, k, v, self.log_decay, state)
+        return self._project(o)
