@@ -81,8 +81,24 @@ def test_no_cpu_fallback():
 
 
 def shape(**kw):
-    s = dict(batch=2, tokens=3, heads=4, kv_heads=2, key_width=8, value_width=6, dtype=0, scale=1.0)
-    return _lib.DecayShape(**{**s, **kw})
+    s = {**dict(batch=2, tokens=3, heads=4, kv_heads=2, key_width=8, value_width=6, cu_seqlens=0, num_seqs=0, dtype=0), **kw}
+    return _lib.DECAY_SHAPE.pack(*(s[x] for x in ("batch", "tokens", "heads", "kv_heads", "key_width", "value_width")),
+                                 *[1] * 12, s["cu_seqlens"], s["num_seqs"], 0, s["dtype"], 1.0)
+
+
+def test_packed_shapes_have_c_layout():
+    class Decay(ctypes.Structure):
+        _fields_ = [(str(i), ctypes.c_int64) for i in range(18)] + [
+            ("cu", ctypes.c_void_p), ("n", ctypes.c_int64), ("is64", ctypes.c_int32), ("t", ctypes.c_int32), ("s", ctypes.c_float)]
+
+    class Step(ctypes.Structure):
+        _fields_ = [(str(i), ctypes.c_int64) for i in range(13)] + [("t", ctypes.c_int32), ("s", ctypes.c_float)]
+
+    assert _lib.DECAY_SHAPE.size == ctypes.sizeof(Decay)
+    assert _lib.DECAY_STEP_SHAPE.size == ctypes.sizeof(Step)
+    d = Decay.from_buffer_copy(_lib.DECAY_SHAPE.pack(*range(18), 77, 78, 1, 2, 0.5))
+    assert [getattr(d, str(i)) for i in range(18)] == list(range(18))
+    assert (d.cu, d.n, d.is64, d.t, d.s) == (77, 78, 1, 2, 0.5)
 
 
 @pytest.mark.parametrize("kw,error", [
@@ -94,28 +110,30 @@ def shape(**kw):
 def test_attention_entry_refuses(kw, error):
     s = shape(**kw)
     with pytest.raises(error):
-        _lib.call("trnfft_decay_attention", ctypes.byref(s), *[None] * 8, 0, None)
+        _lib.call("trnfft_decay_attention", s, *[None] * 8, 0, None)
     with pytest.raises(error):
-        _lib.call("trnfft_decay_attention_backward", ctypes.byref(s), *[None] * 12, 0, None)
+        _lib.call("trnfft_decay_attention_backward", s, *[None] * 12, 0, None)
     if kw:
-        assert _lib.load().trnfft_decay_attention_work_bytes(ctypes.byref(s), 1) == -1
+        assert _lib.load().trnfft_decay_attention_work_bytes(s, 1) == -1
     with pytest.raises(ValueError, match="null shape"):
         _lib.call("trnfft_decay_attention", None, *[None] * 8, 0, None)
 
 
 def test_attention_entry_of_nothing():
     for kw in (dict(batch=0), dict(tokens=0)):
-        _lib.call("trnfft_decay_attention", ctypes.byref(shape(**kw)), *[None] * 8, 0, None)
-        _lib.call("trnfft_decay_attention_backward", ctypes.byref(shape(**kw)), *[None] * 12, 0, None)
+        _lib.call("trnfft_decay_attention", shape(**kw), *[None] * 8, 0, None)
+        _lib.call("trnfft_decay_attention_backward", shape(**kw), *[None] * 12, 0, None)
 
 
 def test_step_entry_refuses():
     one = 4 * 8 * 6
 
     def step(state=4096, new=4096, **kw):
-        s = _lib.DecayStepShape(**{**dict(batch=2, heads=4, kv_heads=2, key_width=8, value_width=6, state_stride=one,
-                                          new_state_stride=one, dtype=0, scale=1.0), **kw})
-        _lib.call("trnfft_decay_attention_step", ctypes.byref(s), 64, 64, 64, 64, state, new, 64, 0, None)
+        s = {**dict(batch=2, heads=4, kv_heads=2, key_width=8, value_width=6, state_stride=one, new_state_stride=one, dtype=0),
+             **kw}
+        s = _lib.DECAY_STEP_SHAPE.pack(*(s[x] for x in ("batch", "heads", "kv_heads", "key_width", "value_width")), *[1] * 6,
+                                       s["state_stride"], s["new_state_stride"], s["dtype"], 1.0)
+        _lib.call("trnfft_decay_attention_step", s, 64, 64, 64, 64, state, new, 64, 0, None)
 
     for kw in (dict(dtype=7), dict(kv_heads=3), dict(key_width=0), dict(state=0), dict(state=4098),
                dict(new=4096 + 4 * one), dict(state_stride=one - 1), dict(new_state_stride=2 * one)):

@@ -12,16 +12,12 @@ bfloat16 or float16; states are float32.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 from ._device import place_layer
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_I64x3 = ctypes.c_int64 * 3
-_I64x2 = ctypes.c_int64 * 2
 
 
 def _unit_inner(t: torch.Tensor) -> torch.Tensor:
@@ -29,11 +25,11 @@ def _unit_inner(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _shape(q, k, v, o_stride, cu, nseq, scale) -> _lib.DecayShape:
+def _shape(q, k, v, o_stride, cu, nseq, scale) -> bytes:
     b, t, h, dk = q.shape
-    return _lib.DecayShape(b, t, h, k.shape[2], dk, v.shape[3], _I64x3(*q.stride()[:3]), _I64x3(*k.stride()[:3]),
-                           _I64x3(*v.stride()[:3]), _I64x3(*o_stride), None if cu is None else cu.data_ptr(), nseq,
-                           int(cu is not None and cu.dtype == torch.int64), DTYPES[q.dtype], scale)
+    return _lib.DECAY_SHAPE.pack(b, t, h, k.shape[2], dk, v.shape[3], *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                                 *o_stride, 0 if cu is None else cu.data_ptr(), nseq,
+                                 cu is not None and cu.dtype == torch.int64, DTYPES[q.dtype], scale)
 
 
 def _addr(t):
@@ -41,7 +37,7 @@ def _addr(t):
 
 
 def _work(shape, backward, device):
-    n = _lib.load().trnfft_decay_attention_work_bytes(ctypes.byref(shape), backward)
+    n = _lib.load().trnfft_decay_attention_work_bytes(shape, backward)
     if n < 0:
         _lib.raise_last("trnfft_decay_attention_work_bytes")
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
@@ -54,9 +50,9 @@ def _forward(q, k, v, log_decay, initial, cu, nseq, scale, want_state):
         last = torch.empty(nseq, q.shape[2], q.shape[3], v.shape[3], dtype=torch.float32, device=q.device)
     shape = _shape(q, k, v, (0, 0, 0), cu, nseq, scale)
     work = _work(shape, 0, q.device)
-    _lib.call("trnfft_decay_attention", ctypes.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-              log_decay.data_ptr(), _addr(initial), o.data_ptr(), _addr(last), _addr(work), q.device.index,
-              torch.cuda.current_stream(q.device).cuda_stream)
+    _lib.call("trnfft_decay_attention", shape, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+              log_decay.data_ptr(), _addr(initial), o.data_ptr(), _addr(last), _addr(work), q.get_device(),
+              _lib.raw_stream(q.get_device()))
     return o, last
 
 
@@ -82,9 +78,9 @@ class _DecayFn(torch.autograd.Function):
         dinitial = torch.empty(initial.shape, dtype=torch.float32, device=q.device) if need[4] else None
         shape = _shape(q, k, v, do.stride()[:3], cu, ctx.nseq, ctx.scale)
         work = _work(shape, 1, q.device)
-        _lib.call("trnfft_decay_attention_backward", ctypes.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        _lib.call("trnfft_decay_attention_backward", shape, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   log_decay.data_ptr(), _addr(initial), do.data_ptr(), _addr(dlast), _addr(dq), _addr(dk), _addr(dv),
-                  _addr(dinitial), _addr(work), q.device.index, torch.cuda.current_stream(q.device).cuda_stream)
+                  _addr(dinitial), _addr(work), q.get_device(), _lib.raw_stream(q.get_device()))
         return dq, dk, dv, None, dinitial, None, None, None, None
 
 
@@ -176,13 +172,14 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     dv = v.shape[2]
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, log_decay, state)):
         raise ValueError(f"{fn}: has no gradient; use decay_attention, or torch.no_grad()")
-    new_state = state if new_state is None else new_state
     one = h * dk * dv
-    for s in (state, new_state):
+    for s in (state,) if new_state is None else (state, new_state):
         if s.shape != (b, h, dk, dv) or s.dtype != torch.float32 or s.device != state.device:
             raise ValueError(f"{fn}: states must be float32 {(b, h, dk, dv)} on one device, got {s.dtype} {tuple(s.shape)}")
-        if b and (not s[0].is_contiguous() or (b > 1 and s.stride(0) < one)):
-            raise ValueError(f"{fn}: the state of each stream must be dense and its own, got strides {s.stride()}")
+        stride = s.stride()
+        if stride[1:] != (dk * dv, dv, 1) and b and not s[0].is_contiguous() or b > 1 and stride[0] < one:
+            raise ValueError(f"{fn}: the state of each stream must be dense and its own, got strides {stride}")
+    new_state = state if new_state is None else new_state
     if not state.is_cuda:  # states in host memory: update a copy on the device
         (q, k, v, log_decay, dev_state), restore = place_layer(fn, q, k, v, log_decay, state)
         o, got = decay_attention_step(q, k, v, log_decay, dev_state, scale=scale)
@@ -193,12 +190,11 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     if log_decay.dtype != torch.float32 or not log_decay.is_contiguous():
         log_decay = log_decay.float().contiguous()
     o = torch.empty(b, h, dv, dtype=q.dtype, device=q.device)
-    shape = _lib.DecayStepShape(b, h, k.shape[1], dk, dv, _I64x2(*q.stride()[:2]), _I64x2(*k.stride()[:2]),
-                                _I64x2(*v.stride()[:2]), state.stride(0) if b > 1 else one,
-                                new_state.stride(0) if b > 1 else one, DTYPES[q.dtype],
-                                dk ** -0.5 if scale is None else float(scale))
-    _lib.call("trnfft_decay_attention_step", ctypes.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-              log_decay.data_ptr(), state.data_ptr(), new_state.data_ptr(), o.data_ptr(), q.device.index,
-              torch.cuda.current_stream(q.device).cuda_stream)
+    shape = _lib.DECAY_STEP_SHAPE.pack(b, h, k.shape[1], dk, dv, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
+                                       state.stride(0) if b > 1 else one, new_state.stride(0) if b > 1 else one,
+                                       DTYPES[q.dtype], dk ** -0.5 if scale is None else scale)
+    device = q.get_device()
+    _lib.call("trnfft_decay_attention_step", shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+              state.data_ptr(), new_state.data_ptr(), o.data_ptr(), device, _lib.raw_stream(device))
     torch.autograd.graph.increment_version(new_state)
     return restore(o), new_state

@@ -47,20 +47,23 @@ def place_layer(fn: str, *ts: torch.Tensor | None):
     CUDA tensors must share one device and stay there; CPU tensors beside them are copied to it, as
     are all of them to the current device where none is on CUDA.  ``restore`` copies a result back to
     the CPU if the first tensor was there."""
-    dev = None
+    dev, host = None, False
     for t in ts:
-        if t is not None and t.is_cuda:
-            if dev is not None and t.device != dev:
-                raise ValueError(f"{fn}: the operands are on several devices ({dev} and {t.device})")
+        if t is None:
+            continue
+        if not t.is_cuda:
+            host = True
+        elif dev is None:
             dev = t.device
-    host = not ts[0].is_cuda
+        elif t.device != dev:
+            raise ValueError(f"{fn}: the operands are on several devices ({dev} and {t.device})")
+    if not host:
+        return ts, _same
     if dev is None:
         _lib.require_cuda()
         dev = torch.device("cuda", torch.cuda.current_device())
-    elif all(t is None or t.is_cuda for t in ts):
-        return ts, _same
     out = [None if t is None else t.to(device=dev) for t in ts]
-    return out, (_to_host if host else _same)
+    return out, (_same if ts[0].is_cuda else _to_host)
 
 
 def _same(t: torch.Tensor) -> torch.Tensor:

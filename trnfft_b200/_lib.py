@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -34,21 +35,10 @@ _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 
 
-class DecayShape(ctypes.Structure):
-    """trnfft_decay_shape"""
-
-    _fields_ = [(n, _I64) for n in ("batch", "tokens", "heads", "kv_heads", "key_width", "value_width")] + [
-        (n, _I64 * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + [
-        ("cu_seqlens", _P), ("num_seqs", _I64), ("cu_is64", ctypes.c_int32), ("dtype", ctypes.c_int32),
-        ("scale", ctypes.c_float)]
-
-
-class DecayStepShape(ctypes.Structure):
-    """trnfft_decay_step_shape"""
-
-    _fields_ = [(n, _I64) for n in ("batch", "heads", "kv_heads", "key_width", "value_width")] + [
-        (n, _I64 * 2) for n in ("q_stride", "k_stride", "v_stride")] + [
-        ("state_stride", _I64), ("new_state_stride", _I64), ("dtype", ctypes.c_int32), ("scale", ctypes.c_float)]
+# The shape structs of include/trnfft_b200.h, packed with C's layout; a bytes object passes as a
+# pointer to them, a tenth of the time of filling a ctypes.Structure.
+DECAY_SHAPE = struct.Struct("6q12qPqiif4x")
+DECAY_STEP_SHAPE = struct.Struct("11q2qif")
 
 
 # name -> (restype, argtypes); every symbol include/trnfft_b200.h declares
@@ -86,10 +76,10 @@ SIGNATURES = {
     "trnfft_exec_istft": (_INT, [_P, _P, _P, _I64, _I64, _I64, _P, _INT, _INT, _INT, _I64, _P, _P]),
     "trnfft_complex_mask_apply": (_INT, [_P, _P, _I64, _P, _P, _P, _P, _I64, _INT, _P]),
     "trnfft_exec_c2r": (_INT, [_P, _P, _P, _P, _I64, _P, _P]),
-    "trnfft_decay_attention_work_bytes": (_I64, [ctypes.POINTER(DecayShape), _INT]),
-    "trnfft_decay_attention": (_INT, [ctypes.POINTER(DecayShape)] + [_P] * 8 + [_INT, _P]),
-    "trnfft_decay_attention_backward": (_INT, [ctypes.POINTER(DecayShape)] + [_P] * 12 + [_INT, _P]),
-    "trnfft_decay_attention_step": (_INT, [ctypes.POINTER(DecayStepShape)] + [_P] * 7 + [_INT, _P]),
+    "trnfft_decay_attention_work_bytes": (_I64, [ctypes.c_char_p, _INT]),
+    "trnfft_decay_attention": (_INT, [ctypes.c_char_p] + [_P] * 8 + [_INT, _P]),
+    "trnfft_decay_attention_backward": (_INT, [ctypes.c_char_p] + [_P] * 12 + [_INT, _P]),
+    "trnfft_decay_attention_step": (_INT, [ctypes.c_char_p] + [_P] * 7 + [_INT, _P]),
     "trnfft_group_norm_work_bytes": (_I64, [_I64] * 4 + [_INT, _INT]),
     "trnfft_group_norm": (_INT, [_P] * 6 + [_I64] * 4 + [ctypes.c_float, _INT, _INT, _P, _INT, _P]),
     "trnfft_group_norm_backward": (_INT, [_P] * 9 + [_I64] * 4 + [_INT, _INT, _P, _INT, _P]),
@@ -163,6 +153,12 @@ def ptr(t: torch.Tensor | None):
 
 def stream_ptr(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def raw_stream(index: int) -> int:
+    """Address of the current stream of CUDA device `index` (a third of a microsecond, where the
+    Stream object of torch.cuda.current_stream takes five)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def require_cuda() -> None:

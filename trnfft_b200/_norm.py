@@ -27,8 +27,8 @@ def _forward(x, groups, weight, bias, eps, act, keep):
     work = _work(n, s, c, groups, dt, 0, x.device)
     at = stats.data_ptr() if keep else None
     _lib.call("trnfft_group_norm", x.data_ptr(), _addr(weight), _addr(bias), y.data_ptr(), at,
-              at + 4 * n * groups if keep else None, n, s, c, groups, eps, act, dt, _addr(work), x.device.index,
-              torch.cuda.current_stream(x.device).cuda_stream)
+              at + 4 * n * groups if keep else None, n, s, c, groups, eps, act, dt, _addr(work), x.get_device(),
+              _lib.raw_stream(x.get_device()))
     return y, stats
 
 
@@ -57,8 +57,8 @@ class _GroupNormFn(torch.autograd.Function):
         work = _work(n, s, c, groups, dt, 1, x.device)
         at = stats.data_ptr()
         _lib.call("trnfft_group_norm_backward", x.data_ptr(), dy.data_ptr(), _addr(w), _addr(b), at, at + 4 * n * groups,
-                  _addr(dx), _addr(dw), _addr(db), n, s, c, groups, ctx.act, dt, _addr(work), x.device.index,
-                  torch.cuda.current_stream(x.device).cuda_stream)
+                  _addr(dx), _addr(dw), _addr(db), n, s, c, groups, ctx.act, dt, _addr(work), x.get_device(),
+                  _lib.raw_stream(x.get_device()))
         dw, db = (g if g is None else g.to(t) for g, t in zip((dw, db), ctx.types))
         return dx, dw, db, None, None, None
 

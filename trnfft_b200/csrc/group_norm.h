@@ -1,4 +1,5 @@
-// Internal interface of the group normalisation kernels (group_norm.cu).
+// Internal interface of the group normalisation kernels (group_norm.cu,
+// group_norm_bwd.cu).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -15,20 +16,41 @@ enum Activation { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
 struct GroupNormArgs {
   const void* x;
   const void* dy;   // backward
-  void* y;          // forward: y, backward: dx
+  void* y;          // forward: y, backward: dx (may be null)
   const float* weight;
   const float* bias;
   float* mean;
   float* rstd;
   float* dw;
   float* db;
-  float* work;
+  void* work;
   long long batch, spots;
   int channels, groups;
   float eps;
   int act;
 };
 
+// How a call is run; it depends on the sizes, the element size and the device alone.
+struct GroupNormPlan {
+  enum Kind { kSmall, kSplit, kAny } kind;
+  int vec;         // elements of one access
+  // kSmall: one group of `lanes` threads per (sample, group), nv accesses each
+  int lanes, nv;
+  // kSplit: `parts` blocks per sample, `slots` rows of `cols` threads per block
+  int parts, slots, cols, tiles, threads, smem;
+  int grid;        // blocks (kSplit with parts > 1: all resident)
+  // work area, in bytes from its start (all 16-byte aligned)
+  long long off_stats, off_channels, channel_rows, off_sync, bytes;
+};
+
+constexpr int kNormThreads = 256;
+constexpr int kSplitThreadsPerSm = 768;
+constexpr int kMaxSplitChannels = 8192;  // two float2 each in shared memory
+constexpr int kSms = 148;
+
+// align: what all of x, y and dy are multiples of (16, 8, 4 or 2 bytes)
+GroupNormPlan plan_group_norm(ElemType t, const GroupNormArgs& a, bool backward, int align);
+int group_norm_align(const GroupNormArgs& a);
 int64_t group_norm_work_bytes(ElemType t, const GroupNormArgs& a, bool backward);
 cudaError_t launch_group_norm(ElemType t, const GroupNormArgs& a, cudaStream_t st);
 cudaError_t launch_group_norm_backward(ElemType t, const GroupNormArgs& a, cudaStream_t st);
