@@ -21,4 +21,12 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
+// Two neighbours at once (one conversion instruction).
+__device__ __forceinline__ void from_f32_pair(float x, float y, __nv_bfloat16* p) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
+}
+__device__ __forceinline__ void from_f32_pair(float x, float y, __half* p) {
+  *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x, y);
+}
+
 }  // namespace tfb

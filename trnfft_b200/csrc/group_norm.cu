@@ -7,16 +7,22 @@
 //   kSmall  a group of one sample has few values (a frame's features, the
 //           heads of an attention's output): a few threads keep them in
 //           registers between the statistics and the result.
-//   kSplit  `parts` blocks share a sample, each a run of whole rows (any
-//           number of channels, any grouping, contiguous in memory).  A
-//           block takes the statistics of its run, hands them to the others
-//           through global memory, takes those of its next sample's run
-//           while they arrive, and comes back for the first: its second
-//           read of x hits L2, because the parts are chosen so that the
-//           samples in flight fit there.
-// The variance is never a difference of large sums: a thread takes the mean
-// and the squared distances of 4 rows at a time and joins such sets by
-//   M2 = M2a + M2b + (mean_b - mean_a)^2 na nb / (na + nb).
+//   kSplit  blocks of whole rows (any number of channels, any grouping,
+//           contiguous in memory).  A sample of up to 48 KB is one block's,
+//           which reads it twice, the second time from L1 or L2.  A larger one
+//           is cut into parts: a first kernel takes their statistics (the last
+//           block of a sample joins them), a second one applies them, from
+//           the last sample to the first, since the end of x is in L2 still.
+//           Keeping parts resident that wait for one another, so that the
+//           second read always hits L2, was slower: what then fits L2 leaves
+//           each thread a dozen rows between two meetings
+//           (8 x 257 x 626 x 48 fp32: 206 us).
+// The variance is never a difference of large sums: a thread sums a channel's
+// distances d from its first value there, and their squares, and leaves
+// mean = first + sum(d) / n and M2 = sum(d^2) - sum(d)^2 / n.  However far off
+// that first value is, it is one of the values, so M2 of the group is at least
+// its own square and the difference loses at most n 2^-24 of it (n: rows of
+// one thread, some dozens).  Sets join by M2 = sum(M2_i + n_i (mean_i - mean)^2).
 #include "group_norm.cuh"
 
 #include <algorithm>
@@ -30,7 +36,7 @@ namespace gn {
 // V > 1 elements are used for one spot only.  A thread's groups are a
 // multiple of `groups` apart, so its channels and their parameters stay.
 template <typename T, int V, int NV, int ACT>
-__global__ void __launch_bounds__(kNormThreads) k_gn_small(const __grid_constant__ GroupNormArgs a, int lanes) {
+__global__ void __launch_bounds__(kNormThreads, small_blocks(NV)) k_gn_small(const __grid_constant__ GroupNormArgs a, int lanes) {
   const int w = a.channels / a.groups, count = (int)a.spots * w;
   const int per = kNormThreads / lanes, lane = threadIdx.x & (lanes - 1);
   const long long slots = (long long)gridDim.x * per / a.groups * a.groups;
@@ -50,47 +56,59 @@ __global__ void __launch_bounds__(kNormThreads) k_gn_small(const __grid_constant
     }
   }
   const float inv = 1.f / (float)count;
+  const long long step = slots / a.groups * a.spots * a.channels;  // from one of a thread's groups to its next
+  const long long base = first / a.groups * a.spots * a.channels + (long long)g * w;
+  const T* x = static_cast<const T*>(a.x) + base;
+  T* y = static_cast<T*>(a.y) + base;
   // every thread of a warp takes the same number of turns: the shuffles need them all
-  const long long turns = (total + slots - 1) / slots;
-  for (long long k = 0; k < turns; ++k) {
-    const long long id = first + k * slots;
-    const bool live = first < slots && id < total;
-    const long long base = live ? id / a.groups * a.spots * a.channels + (long long)g * w : 0;
-    const T* x = static_cast<const T*>(a.x) + base;
-    Pack<T, V> p[NV];
-    float s = 0.f;
+  int left = first < slots && first < total ? (int)((total - first + slots - 1) / slots) : 0;
+  int turns = (int)((total + slots - 1) / slots);
+  float *mean_at = a.mean ? a.mean + first : nullptr, *rstd_at = a.rstd + first;
+  typename Pack<T, V>::Raw ahead[2][NV];  // the next two groups' values, on their way
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (live && off[j] >= 0) {
-        p[j].load(x + off[j]);
-#pragma unroll
-        for (int v = 0; v < V; ++v) s += p[j].x[v];
-      }
-    }
-    const float mean = lanes_sum(s, lanes) * inv;
-    s = 0.f;
+  for (int d = 0; d < 2; ++d)
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (live && off[j] >= 0) {
+      if (left > d && off[j] >= 0) ahead[d][j] = Pack<T, V>::raw(x + d * step + off[j]);
+  for (; turns > 0; --turns, --left, x += step, y += step) {
+    Pack<T, V> p[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      p[j].unpack(ahead[0][j]);
+      ahead[0][j] = ahead[1][j];
+      if (left > 2 && off[j] >= 0) ahead[1][j] = Pack<T, V>::raw(x + 2 * step + off[j]);
+    }
+    // distances from the group's first value (see the note on the variance above)
+    const float origin = __shfl_sync(~0u, p[0].x[0], threadIdx.x & 31 & -lanes);
+    float s = 0.f, ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (off[j] >= 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          p[j].x[v] -= mean;
-          s = fmaf(p[j].x[v], p[j].x[v], s);
+          p[j].x[v] -= origin;
+          s += p[j].x[v];
+          ss = fmaf(p[j].x[v], p[j].x[v], ss);
         }
       }
-    const float rstd = __frsqrt_rn(lanes_sum(s, lanes) * inv + a.eps);
-    if (live) {
-      T* y = static_cast<T*>(a.y) + base;
+    lanes_sum(s, ss, lanes);
+    const float mean = s * inv, var = fmaxf(fmaf(-mean, mean, ss * inv), 0.f);
+    const float rstd = __frsqrt_rn((ss - ss == 0.f ? var : ss) + a.eps);  // NaN stays NaN
+    if (left > 0) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (off[j] >= 0) {
 #pragma unroll
-          for (int v = 0; v < V; ++v) p[j].x[v] = activate<T, ACT>(fmaf(p[j].x[v] * rstd, wt[j][v], bs[j][v]));
+          for (int v = 0; v < V; ++v) p[j].x[v] = activate<ACT>(fmaf((p[j].x[v] - mean) * rstd, wt[j][v], bs[j][v]));
           p[j].store(y + off[j]);
         }
-      if (lane == 0 && a.mean) {
-        a.mean[id] = mean;
-        a.rstd[id] = rstd;
+      if (mean_at) {
+        if (lane == 0) {
+          *mean_at = origin + mean;
+          *rstd_at = rstd;
+        }
+        mean_at += slots;
+        rstd_at += slots;
       }
     }
   }
@@ -98,212 +116,192 @@ __global__ void __launch_bounds__(kNormThreads) k_gn_small(const __grid_constant
 
 // ---------------------------------------------------------------- kSplit
 
-// Shared memory: per-slot sets (mean, M2) of a tile of channels, then the
-// channels' of the block's rows, then the groups' results.
-struct SplitSmem {
-  float2* red;    // slots * cols * V
-  float2* chan;   // channels
-  float2* group;  // groups: (mean, rstd)
-};
+__device__ __forceinline__ float rstd_of(float var, float eps) { return __frsqrt_rn((var < 0.f ? 0.f : var) + eps); }
 
+// The sets of the block's rows of sample n, joined for each group: out[g], as (mean, M2).
 template <typename T, int V>
-__device__ __forceinline__ void split_stats(const GroupNormArgs& a, const GroupNormPlan& p, const SplitSmem& sm,
-                                            long long n, int k, float2* part) {
-  constexpr int U = 4;
-  const int slot = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
-  long long lo, hi;
-  part_rows(a.spots, p.parts, k, lo, hi);
-  const T* x = static_cast<const T*>(a.x) + n * a.spots * a.channels;
+__device__ __forceinline__ void split_stats(const GroupNormArgs& a, const GroupNormPlan& p, float2* red,
+                                            const SplitPlace& at, SplitColumn<V>& col, long long n, float2* out) {
+  constexpr int U = rows_ahead(V * sizeof(T));
+  const T* x = static_cast<const T*>(a.x) + n * a.spots * a.channels + at.first;
   const int w = a.channels / a.groups;
   for (int tile = 0; tile < p.tiles; ++tile) {
-    const int c = (tile * p.cols + col) * V;
-    float mean[V], m2[V];
-    float cnt = 0.f;
+    if (p.tiles > 1) col.set(a, p, at, tile);
+    if (!col.live) continue;
+    const T* q = x + col.c;
+    Pack<T, V> first;
+    float s[V], ss[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) mean[v] = m2[v] = 0.f;
-    if (slot < p.slots && c < a.channels) {
-      const T* q = x + (lo + slot) * a.channels + c;
-      const long long step = (long long)p.slots * a.channels;
-      for (int left = slot_rows(lo, hi, slot, p.slots); left > 0; left -= U, q += U * step) {
-        Pack<T, V> b[U];
+    for (int v = 0; v < V; ++v) first.x[v] = s[v] = ss[v] = 0.f;
+    if (at.mine) first.load(q);
+    for (int left = at.mine; left > 0; left -= U, q += U * at.step) {
+      typename Pack<T, V>::Raw r[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (u < left) b[u].load(q + u * step);
-        const float nb = (float)min(left, U), inv = 1.f / nb, all = cnt + nb, share = nb / all, cross = cnt * share;
+      for (int u = 0; u < U; ++u)
+        if (u < left) r[u] = Pack<T, V>::raw(q + u * at.step);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float s = 0.f;
+      for (int u = 0; u < U; ++u)
+        if (u < left) {
+          Pack<T, V> b;
+          b.unpack(r[u]);
 #pragma unroll
-          for (int u = 0; u < U; ++u) s += u < left ? b[u].x[v] : 0.f;
-          const float mb = s * inv;
-          float d2 = 0.f;
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const float d = u < left ? b[u].x[v] - mb : 0.f;
-            d2 = fmaf(d, d, d2);
+          for (int v = 0; v < V; ++v) {
+            const float d = b.x[v] - first.x[v];
+            s[v] += d;
+            ss[v] = fmaf(d, d, ss[v]);
           }
-          const float d = mb - mean[v];
-          m2[v] += fmaf(d * d, cross, d2);
-          mean[v] = fmaf(d, share, mean[v]);
         }
-        cnt = all;
-      }
+    }
+    const float inv = at.mine ? 1.f / (float)at.mine : 0.f;
+    float2* to = red + at.slot * a.channels + col.c;
 #pragma unroll
-      for (int v = 0; v < V; ++v) sm.red[(slot * p.cols + col) * V + v] = make_float2(mean[v], m2[v]);
+    for (int v = 0; v < V; ++v) {
+      const float d = s[v] * inv;
+      to[v] = make_float2(first.x[v] + d, fmaf(-s[v], d, ss[v]));
     }
-    __syncthreads();
-    // join the slots: slot s has the rows lo + s, lo + s + slots, ...
-    const int width = p.cols * V;
-    for (int i = threadIdx.x; i < width && tile * width + i < a.channels; i += blockDim.x) {
-      float na = 0.f, m = 0.f, q = 0.f;
-      for (int s = 0; s < p.slots && lo + s < hi; ++s) {
-        const float nb = (float)slot_rows(lo, hi, s, p.slots), all = na + nb;
-        const float2 b = sm.red[s * width + i];
-        const float d = b.x - m;
-        q += fmaf(d * d, na * nb / all, b.y);
-        m = fmaf(d, nb / all, m);
-        na = all;
-      }
-      sm.chan[tile * width + i] = make_float2(m, q);
-    }
-    __syncthreads();
   }
-  // a group's channels have the same number of rows
-  const float rows = (float)(hi - lo);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
-  for (int g = warp; g < a.groups; g += warps) {
-    float s = 0.f;
-    for (int c = lane; c < w; c += 32) s += sm.chan[g * w + c].x;
-    const float m = warp_sum(s) / (float)w;
-    s = 0.f;
-    for (int c = lane; c < w; c += 32) {
-      const float2 b = sm.chan[g * w + c];
-      const float d = b.x - m;
-      s += fmaf(d * d, rows, b.y);
+  __syncthreads();
+  // Join the sets of a group, by `glanes` threads: the distances of their means from the first of
+  // them, as above.  Slots below `extra` have one row more than the others.
+  const int lanes = p.glanes, lane = threadIdx.x & (lanes - 1), full = at.rows / p.slots, extra = at.rows % p.slots;
+  const float inv = 1.f / ((float)at.rows * (float)w);
+  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x / lanes) {
+    const int g = g0 + threadIdx.x / lanes;
+    float t = 0.f, tt = 0.f, origin = 0.f;
+    if (g < a.groups) {
+      origin = red[g * w].x;
+      for (int j = 0, c = lane; j < p.slots; c += lanes) {
+        while (c >= w) c -= w, ++j;
+        if (j >= p.slots) break;
+        const float2 b = red[j * a.channels + g * w + c];
+        const float d = b.x - origin, nd = d * (float)(full + (j < extra));
+        t += nd;
+        tt += fmaf(nd, d, b.y);
+      }
     }
-    s = warp_sum(s);
-    if (lane == 0) {
-      if (p.parts > 1)
-        part[((long long)n * p.parts + k) * a.groups + g] = make_float2(m, s);
-      else
-        sm.group[g] = make_float2(m, s);
+    lanes_sum(t, tt, lanes);
+    if (g < a.groups && lane == 0) out[g] = make_float2(fmaf(t, inv, origin), fmaf(-t * inv, t, tt));
+  }
+}
+
+// y of the block's rows of sample n, given (mean, rstd) of its groups.
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void split_apply(const GroupNormArgs& a, const GroupNormPlan& p, const SplitPlace& at,
+                                            SplitColumn<V>& col, long long n, const float2* group) {
+  constexpr int U = rows_ahead(V * sizeof(T));
+  const long long first = n * a.spots * a.channels + at.first;
+  for (int tile = 0; tile < p.tiles; ++tile) {
+    if (p.tiles > 1) col.set(a, p, at, tile);
+    if (!col.live) continue;
+    float mean[V], gain[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float2 s = group[col.group(v)];
+      mean[v] = s.x;
+      gain[v] = s.y * col.wt[v];
+    }
+    const T* from = static_cast<const T*>(a.x) + first + col.c;
+    T* to = static_cast<T*>(a.y) + first + col.c;
+    for (int left = at.mine; left > 0; left -= U, from += U * at.step, to += U * at.step) {
+      typename Pack<T, V>::Raw r[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < left) r[u] = Pack<T, V>::raw(from + u * at.step);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < left) {
+          Pack<T, V> q;
+          q.unpack(r[u]);
+#pragma unroll
+          for (int v = 0; v < V; ++v) q.x[v] = activate<ACT>(fmaf(q.x[v] - mean[v], gain[v], col.bs[v]));
+          q.store(to + u * at.step);
+        }
     }
   }
 }
 
+// A block takes whole samples.
 template <typename T, int V, int ACT>
-__device__ __forceinline__ void split_apply(const GroupNormArgs& a, const GroupNormPlan& p, const SplitSmem& sm,
-                                            long long n, int k, const float2* part) {
-  constexpr int U = 4;
-  const int w = a.channels / a.groups;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
-  const float total = (float)(a.spots * w);
-  __syncthreads();
-  for (int g = warp; g < a.groups; g += warps) {
-    float m, q;
-    if (p.parts > 1) {
-      const float2* at = part + (long long)n * p.parts * a.groups + g;
-      float s = 0.f;
-      for (int i = lane; i < p.parts; i += 32) {
-        long long lo, hi;
-        part_rows(a.spots, p.parts, i, lo, hi);
-        s = fmaf(__ldcg(at + (long long)i * a.groups).x, (float)((hi - lo) * w) / total, s);
+__global__ void __launch_bounds__(kNormThreads, 3)
+    k_gn_whole(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  extern __shared__ __align__(16) float2 smem[];
+  float2 *red = smem, *group = red + p.slots * a.channels;
+  const SplitPlace at(a, p, 0);
+  SplitColumn<V> col;
+  col.set(a, p, at, 0);
+  const float inv = 1.f / ((float)a.spots * (float)(a.channels / a.groups));
+  for (long long n = blockIdx.x; n < a.batch; n += gridDim.x) {
+    split_stats<T, V>(a, p, red, at, col, n, group);
+    __syncthreads();
+    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
+      const float rstd = rstd_of(group[g].y * inv, a.eps);
+      group[g].y = rstd;
+      if (a.mean) {
+        a.mean[n * a.groups + g] = group[g].x;
+        a.rstd[n * a.groups + g] = rstd;
       }
-      m = warp_sum(s);
-      s = 0.f;
-      for (int i = lane; i < p.parts; i += 32) {
-        long long lo, hi;
-        part_rows(a.spots, p.parts, i, lo, hi);
-        const float2 b = __ldcg(at + (long long)i * a.groups);
-        const float d = b.x - m;
-        s += fmaf(d * d, (float)((hi - lo) * w), b.y);
-      }
-      q = warp_sum(s);
-    } else {
-      m = sm.group[g].x;
-      q = sm.group[g].y;
     }
-    const float rstd = __frsqrt_rn(q / total + a.eps);
-    __syncwarp();
-    if (lane == 0) {
-      sm.group[g] = make_float2(m, rstd);
-      if (k == 0 && a.mean) {
-        a.mean[n * a.groups + g] = m;
+    __syncthreads();
+    split_apply<T, V, ACT>(a, p, at, col, n, group);
+  }
+}
+
+// Block = part blockIdx.x % parts of sample blockIdx.x / parts: its groups' sets; the sample's last
+// block joins the parts' into (mean, rstd).
+template <typename T, int V>
+__global__ void __launch_bounds__(kNormThreads, 5)
+    k_gn_stats(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  extern __shared__ __align__(16) float2 smem[];
+  const long long n = blockIdx.x / p.parts;
+  const int k = blockIdx.x % p.parts;
+  float2* part = static_cast<float2*>(a.work) + n * p.parts * a.groups;
+  {
+    const SplitPlace at(a, p, k);
+    SplitColumn<V> col;
+    col.set(a, p, at, 0);
+    split_stats<T, V>(a, p, smem, at, col, n, part + (long long)k * a.groups);
+  }
+  unsigned* count = reinterpret_cast<unsigned*>(static_cast<char*>(a.work) + p.off_sync);
+  if (!last_of_sample(count + n, p.parts)) return;
+  float2* result = reinterpret_cast<float2*>(static_cast<char*>(a.work) + p.off_result) + n * a.groups;
+  const int w = a.channels / a.groups, lanes = p.planes, lane = threadIdx.x & (lanes - 1);
+  const float inv = 1.f / ((float)a.spots * (float)w), most = (float)p.part_rows * (float)w;
+  const float last = (float)(a.spots - (long long)(p.parts - 1) * p.part_rows) * (float)w;
+  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x / lanes) {
+    const int g = g0 + threadIdx.x / lanes;
+    float t = 0.f, tt = 0.f, origin = 0.f;
+    if (g < a.groups) {
+      origin = __ldcg(part + g).x;
+#pragma unroll 8
+      for (int i = lane; i < p.parts; i += lanes) {
+        const float2 b = __ldcg(part + (long long)i * a.groups + g);
+        const float d = b.x - origin, nd = d * (i == p.parts - 1 ? last : most);
+        t += nd;
+        tt += fmaf(nd, d, b.y);
+      }
+    }
+    lanes_sum(t, tt, lanes);
+    if (g < a.groups && lane == 0) {
+      const float mean = fmaf(t, inv, origin), rstd = rstd_of(fmaf(-t * inv, t, tt) * inv, a.eps);
+      result[g] = make_float2(mean, rstd);
+      if (a.mean) {
+        a.mean[n * a.groups + g] = mean;
         a.rstd[n * a.groups + g] = rstd;
       }
     }
   }
-  __syncthreads();
-  const int slot = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
-  long long lo, hi;
-  part_rows(a.spots, p.parts, k, lo, hi);
-  const T* x = static_cast<const T*>(a.x) + n * a.spots * a.channels;
-  T* y = static_cast<T*>(a.y) + n * a.spots * a.channels;
-  for (int tile = 0; tile < p.tiles; ++tile) {
-    const int c = (tile * p.cols + col) * V;
-    if (slot >= p.slots || c >= a.channels) continue;
-    float mean[V], gain[V], bias[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float2 s = sm.group[(c + v) / w];
-      mean[v] = s.x;
-      gain[v] = s.y * (a.weight ? a.weight[c + v] : 1.f);
-      bias[v] = a.bias ? a.bias[c + v] : 0.f;
-    }
-    const long long step = (long long)p.slots * a.channels, at = (lo + slot) * a.channels + c;
-    const T* from = x + at;
-    T* to = y + at;
-    for (int left = slot_rows(lo, hi, slot, p.slots); left > 0; left -= U, from += U * step, to += U * step) {
-      Pack<T, V> q[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u < left) q[u].load(from + u * step);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u < left) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) q[u].x[v] = activate<T, ACT>(fmaf(q[u].x[v] - mean[v], gain[v], bias[v]));
-          q[u].store(to + u * step);
-        }
-    }
-  }
-  __syncthreads();
 }
 
-// parts == 1: block = sample.  parts > 1: the grid is a multiple of `parts`
-// and resident; block b takes part b % parts of the samples b / parts,
-// b / parts + grid / parts, ...
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads, kSplitThreadsPerSm / kNormThreads) k_gn_split(const __grid_constant__ GroupNormArgs a,
-                                                  const __grid_constant__ GroupNormPlan p) {
-  extern __shared__ __align__(16) float2 smem[];
-  SplitSmem sm;
-  sm.red = smem;
-  sm.chan = sm.red + p.slots * p.cols * V;
-  sm.group = sm.chan + a.channels;
-  if (p.parts == 1) {
-    for (long long n = blockIdx.x; n < a.batch; n += gridDim.x) {
-      split_stats<T, V>(a, p, sm, n, 0, nullptr);
-      split_apply<T, V, ACT>(a, p, sm, n, 0, nullptr);
-    }
-    return;
-  }
-  float2* part = reinterpret_cast<float2*>(static_cast<char*>(a.work) + p.off_stats);
-  unsigned* sync = reinterpret_cast<unsigned*>(static_cast<char*>(a.work) + p.off_sync);
-  const int k = blockIdx.x % p.parts, step = gridDim.x / p.parts;
-  long long n = blockIdx.x / p.parts;
-  if (n >= a.batch) return;
-  split_stats<T, V>(a, p, sm, n, k, part);
-  sample_arrive(sync + n);
-  for (; n < a.batch; n += step) {
-    const long long next = n + step;
-    if (next < a.batch) {
-      split_stats<T, V>(a, p, sm, next, k, part);
-      sample_arrive(sync + next);
-    }
-    sample_wait(sync + n, (unsigned)p.parts);
-    split_apply<T, V, ACT>(a, p, sm, n, k, part);
-  }
+__global__ void __launch_bounds__(kNormThreads, 4)
+    k_gn_apply(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  const unsigned b = gridDim.x - 1 - blockIdx.x;
+  const long long n = b / p.parts;
+  const SplitPlace at(a, p, b % p.parts);
+  SplitColumn<V> col;
+  col.set(a, p, at, 0);
+  const float2* result = reinterpret_cast<const float2*>(static_cast<const char*>(a.work) + p.off_result);
+  split_apply<T, V, ACT>(a, p, at, col, n, result + n * a.groups);
 }
 
 // ---------------------------------------------------------------- kAny
@@ -328,7 +326,7 @@ __global__ void __launch_bounds__(kNormThreads) k_gn_any(const __grid_constant__
           if (pass == 1) s = fmaf(d, d, s);
           if (pass == 2) {
             const float z = fmaf(d * stat[1], a.weight ? a.weight[g * w + c] : 1.f, a.bias ? a.bias[g * w + c] : 0.f);
-            static_cast<T*>(a.y)[at] = from_f32<T>(activate<T, ACT>(z));
+            static_cast<T*>(a.y)[at] = from_f32<T>(activate<ACT>(z));
           }
         }
       if (pass == 2) break;
@@ -361,20 +359,18 @@ static cudaError_t run_small(const GroupNormArgs& a, const GroupNormPlan& p, cud
 
 template <typename T, int V, int ACT>
 static cudaError_t run_split(const GroupNormArgs& a, const GroupNormPlan& p, cudaStream_t st) {
-  cudaError_t e = cudaSuccess;
-  if (p.smem > 48 * 1024)
-    e = cudaFuncSetAttribute(k_gn_split<T, V, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
-  if (e != cudaSuccess) return e;
+  cudaError_t e;
   if (p.parts == 1) {
-    k_gn_split<T, V, ACT><<<p.grid, p.threads, p.smem, st>>>(a, p);
-    return cudaGetLastError();
+    e = allow_smem(k_gn_whole<T, V, ACT>, p.smem);
+    if (e == cudaSuccess) k_gn_whole<T, V, ACT><<<p.grid, p.threads, p.smem, st>>>(a, p);
+    return e == cudaSuccess ? cudaGetLastError() : e;
   }
-  e = cudaMemsetAsync(static_cast<char*>(a.work) + p.off_sync, 0, sizeof(unsigned) * a.batch, st);
+  e = allow_smem(k_gn_stats<T, V>, p.smem);
+  if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<char*>(a.work) + p.off_sync, 0, sizeof(unsigned) * a.batch, st);
   if (e != cudaSuccess) return e;
-  GroupNormArgs a2 = a;
-  GroupNormPlan p2 = p;
-  void* args[] = {&a2, &p2};
-  return cudaLaunchCooperativeKernel(k_gn_split<T, V, ACT>, dim3(p.grid), dim3(p.threads), args, (size_t)p.smem, st);
+  k_gn_stats<T, V><<<p.grid, p.threads, p.smem, st>>>(a, p);
+  k_gn_apply<T, V, ACT><<<p.grid, p.threads, 0, st>>>(a, p);
+  return cudaGetLastError();
 }
 
 template <typename T, int ACT>
@@ -404,6 +400,16 @@ static cudaError_t run_act(const GroupNormArgs& a, const GroupNormPlan& p, cudaS
 
 }  // namespace gn
 
+// Threads that share a sum of n terms: 4 terms each or more, in at most a warp.
+static int lanes_for(long long n) {
+  int lanes = 1;
+  while (lanes < 32 && lanes * 4 < n) lanes *= 2;
+  return lanes;
+}
+
+using gn::small_blocks;
+using gn::small_blocks_bwd;
+
 GroupNormPlan plan_group_norm(ElemType t, const GroupNormArgs& a, bool backward, int align) {
   GroupNormPlan p = {};
   const int size = t == kF32 ? 4 : 2, wide = 16 / size, w = a.channels / a.groups;
@@ -423,7 +429,7 @@ GroupNormPlan plan_group_norm(ElemType t, const GroupNormArgs& a, bool backward,
     const int per = kNormThreads / p.lanes;
     const long long blocks = (total + per - 1) / per;
     const long long least = (a.groups + per - 1) / per;  // a thread group for each group of channels
-    const long long most = std::max<long long>(least, (long long)kSms * (backward ? 4 : 8));
+    const long long most = std::max<long long>(least, (long long)kSms * (backward ? small_blocks_bwd(p.nv) : small_blocks(p.nv)));
     p.grid = (int)std::max(least, std::min(blocks, most));
     if (backward) {
       const long long slots = (long long)p.grid * per / a.groups * a.groups;
@@ -446,19 +452,24 @@ GroupNormPlan plan_group_norm(ElemType t, const GroupNormArgs& a, bool backward,
   p.tiles = (columns + p.cols - 1) / p.cols;
   p.slots = (int)std::min<long long>(kNormThreads / p.cols, a.spots);
   p.threads = std::max(64, (p.slots * p.cols + 31) / 32 * 32);
-  p.smem = (int)sizeof(float2) * (p.slots * p.cols * p.vec + (backward ? 2 : 1) * a.channels + a.groups);
-  // resident blocks per SM: the launch bounds leave registers for 768 threads
-  const int resident = std::max(1, std::min(kSplitThreadsPerSm / p.threads, 200 * 1024 / (p.smem + 1024)));
-  const long long most = (long long)kSms * resident;
+  // a block's sets (backward: and its channels' sums, of one sample and of all), the groups' results
+  p.smem = (int)sizeof(float2) * (p.slots * a.channels + (backward ? 2 * a.channels : 0) + a.groups);
+  const long long most = 8LL * kSms * kNormThreads / p.threads;  // blocks that fill the GPU, and then some
   const long long bytes = a.spots * a.channels * size * (backward ? 2 : 1);
-  // The samples in flight (two per `parts` blocks: one that is read, one that is written) stay
-  // within 48 MB of L2; with few samples their blocks fill the GPU, each with 16 KB at least.
-  long long parts = (most * bytes * 2 + (48LL << 20) - 1) / (48LL << 20);
-  parts = std::max(parts, (most + a.batch - 1) / a.batch);
-  parts = std::min({parts, most, bytes / (16 << 10), (long long)a.spots});
-  p.parts = bytes <= (48 << 10) ? 1 : (int)std::max<long long>(1, parts);
-  p.grid = (int)(p.parts == 1 ? std::min(a.batch, most) : std::min(a.batch, most / p.parts) * p.parts);
-  p.off_channels = ((p.parts > 1 ? a.batch * p.parts * a.groups * 8 : 0) + 15) & ~15LL;
+  // parts of 32 KB at least, and as many as fill the GPU
+  long long parts = 1;
+  if (bytes > (48 << 10) && !(a.batch >= 2 * kSms && bytes <= (128 << 10)))
+    parts = std::max<long long>(1, std::min({(most + a.batch - 1) / a.batch, bytes / (32 << 10), (long long)a.spots}));
+  // a block of one part only: cut large samples of a large batch as well, for the sake of L2
+  if (parts == 1 && bytes > (128 << 10)) parts = std::min<long long>(a.spots, (bytes + (128 << 10) - 1) / (128 << 10));
+  p.part_rows = (int)((a.spots + parts - 1) / parts);
+  p.parts = (int)((a.spots + p.part_rows - 1) / p.part_rows);
+  p.glanes = lanes_for((long long)(backward ? 1 : p.slots) * w);
+  p.planes = p.parts > 1 ? lanes_for(p.parts) : 1;
+  p.grid = (int)(p.parts == 1 ? std::min(a.batch, most) : a.batch * p.parts);
+  const long long result = p.parts > 1 ? a.batch * a.groups * 8 : 0;
+  p.off_result = (result * p.parts + 15) & ~15LL;
+  p.off_channels = (p.off_result + result + 15) & ~15LL;
   p.channel_rows = backward ? p.grid : 0;
   p.off_sync = p.off_channels + ((p.channel_rows * a.channels * 8 + 15) & ~15LL);
   p.bytes = p.off_sync + (p.parts > 1 ? a.batch * 4 : 0);

@@ -1,80 +1,116 @@
 // Device code shared by the forward and backward group normalisation kernels.
 #pragma once
 
+#include <type_traits>
+
 #include "elem.cuh"
 #include "group_norm.h"
-#include "tma.cuh"
 
 namespace tfb {
 namespace gn {
 
-// float32 results keep the accurate exponential and division; a 16-bit result's own rounding is
-// 2^-9 or 2^-12, where the fast ones (a few 2^-22) make no difference.
-template <typename T>
-__device__ __forceinline__ float sigmoid(float z) {
-  if (sizeof(T) == 4) return 1.f / (1.f + expf(-z));
-  return __fdividef(1.f, 1.f + __expf(-fmaxf(z, -80.f)));
+// The special function unit's 2^x and 1/x, to about 2^-22, without the handling of denormal numbers
+// that would triple their instructions (a result below 2^-126 is 0).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+
+// 1 / (1 + e^-z); e^-z = inf gives 0.
+__device__ __forceinline__ float sigmoid(float z) { return rcp_fast(1.f + exp2_fast(-kLog2E * z)); }
+
+// The normal distribution function of z, and e = exp(-z^2 / 2), from one exponential:
+// erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + 0.3275911 x), x >= 0, to 1.5e-7
+// (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26).  A library erf of twice
+// the instructions made the float32 passes bound by instructions instead of memory.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = rcp_fast(fmaf(0.3275911f, x, 1.f));
+  e = exp2_fast(x * x * -kLog2E);
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float half = 0.5f * (p * t * e);
+  return z < 0.f ? half : 1.f - half;
 }
 
-template <typename T, int ACT>
+template <int ACT>
 __device__ __forceinline__ float activate(float z) {
   if (ACT == kActRelu) return z < 0.f ? 0.f : z;  // NaN stays NaN
-  if (ACT == kActSilu) return z * sigmoid<T>(z);
-  if (ACT == kActGelu) return z * (0.5f + 0.5f * erff(z * 0.70710678118654752f));
+  if (ACT == kActSilu) return z * sigmoid(z);
+  if (ACT == kActGelu) {
+    float e;
+    return z * normal_cdf(z, e);
+  }
   return z;
 }
 
-template <typename T, int ACT>
+template <int ACT>
 __device__ __forceinline__ float slope(float z) {
   if (ACT == kActRelu) return z > 0.f ? 1.f : 0.f;
   if (ACT == kActSilu) {
-    const float s = sigmoid<T>(z);
+    const float s = sigmoid(z);
     return s * fmaf(z, 1.f - s, 1.f);
   }
   if (ACT == kActGelu) {
-    const float p = sizeof(T) == 4 ? expf(-0.5f * z * z) : __expf(-0.5f * z * z);
-    return fmaf(0.5f, erff(z * 0.70710678118654752f), 0.5f) + z * p * 0.39894228040143268f;
+    float e;
+    const float p = normal_cdf(z, e);
+    return fmaf(z * 0.39894228040143268f, e, p);
   }
   return 1.f;
 }
 
+// The bytes of one access, as loaded.
+template <int B>
+struct Bytes;
+template <>
+struct Bytes<16> { using type = uint4; };
+template <>
+struct Bytes<8> { using type = uint2; };
+template <>
+struct Bytes<4> { using type = uint32_t; };
+template <>
+struct Bytes<2> { using type = uint16_t; };
+
 // V elements of one access of V * sizeof(T) bytes, as float32.
 template <typename T, int V>
 struct Pack {
+  using Raw = typename Bytes<V * sizeof(T)>::type;
   float x[V];
-  __device__ __forceinline__ void load(const T* p) {
-    constexpr int B = V * sizeof(T);
-    if constexpr (B == 16) {
-      const uint4 r = *reinterpret_cast<const uint4*>(p);
-      unpack(reinterpret_cast<const T*>(&r));
-    } else if constexpr (B == 8) {
-      const uint2 r = *reinterpret_cast<const uint2*>(p);
-      unpack(reinterpret_cast<const T*>(&r));
-    } else if constexpr (B == 4 && V > 1) {
-      const uint32_t r = *reinterpret_cast<const uint32_t*>(p);
-      unpack(reinterpret_cast<const T*>(&r));
+  static __device__ __forceinline__ Raw raw(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ void unpack(Raw r) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value && V % 2 == 0) {
+      const uint32_t* v = reinterpret_cast<const uint32_t*>(&r);  // a bfloat16 is the upper half of its float32
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        x[2 * i] = __uint_as_float(v[i] << 16);
+        x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+      }
     } else {
-      static_assert(V == 1, "access width");
-      x[0] = to_f32(p[0]);
+      const T* v = reinterpret_cast<const T*>(&r);
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = to_f32(v[i]);
     }
   }
-  __device__ __forceinline__ void unpack(const T* v) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = to_f32(v[i]);
-  }
+  __device__ __forceinline__ void load(const T* p) { unpack(raw(p)); }
   __device__ __forceinline__ void store(T* p) const {
     alignas(16) T v[V];
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = from_f32<T>(x[i]);
-    constexpr int B = V * sizeof(T);
-    if constexpr (B == 16)
-      __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(v));
-    else if constexpr (B == 8)
-      __stcs(reinterpret_cast<uint2*>(p), *reinterpret_cast<const uint2*>(v));
-    else if constexpr (B == 4 && V > 1)
-      *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(v);
-    else
-      p[0] = v[0];
+      for (int i = 0; i < V; i += 2) from_f32_pair(x[i], x[i + 1], v + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = from_f32<T>(x[i]);
+    }
+    __stcs(reinterpret_cast<Raw*>(p), *reinterpret_cast<const Raw*>(v));
   }
 };
 
@@ -84,49 +120,81 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sum over aligned groups of `lanes` threads (a power of two).
-__device__ __forceinline__ float lanes_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
-}
-
-// The parts of one sample meet here: each block adds itself to the sample's
-// counter after writing its partial results, and waits until all have.  All
-// blocks are resident (cooperative launch), so the wait ends; it is bounded
-// all the same, and on giving up records the device status word.
-__device__ __forceinline__ void sample_arrive(unsigned* counter) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    atomicAdd(counter, 1u);
-  }
-}
-__device__ __forceinline__ void sample_wait(unsigned* counter, unsigned target) {
-  if (threadIdx.x == 0) {
-    unsigned v = 0;
-    int i = 0;
-    for (; i < (1 << 24); ++i) {
-      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(counter) : "memory");
-      if (v >= target) break;
-      __nanosleep(20);
+// Two sums over aligned groups of `lanes` threads (a power of two).
+__device__ __forceinline__ void lanes_sum(float& u, float& v, int lanes) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    if (o < lanes) {
+      u += __shfl_xor_sync(~0u, u, o);
+      v += __shfl_xor_sync(~0u, v, o);
     }
-    if (i == (1 << 24)) atomicExch(&g_dev_status, kStatusWaitTimeout);
+}
+
+// Blocks of 256 threads an SM holds with a thread's NV accesses and their parameters in registers.
+constexpr int small_blocks(int nv) { return nv == 1 ? 4 : (nv == 2 ? 3 : 2); }
+constexpr int small_blocks_bwd(int nv) { return nv == 1 ? 3 : (nv == 2 ? 2 : 1); }
+
+// True in the block that is the last of its sample's `parts` to come here; it sees what all of
+// them wrote before.
+__device__ __forceinline__ bool last_of_sample(unsigned* counter, int parts) {
+  __shared__ unsigned before;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    before = atomicAdd(counter, 1u);
     __threadfence();
   }
   __syncthreads();
+  return before == parts - 1;
 }
 
-// Rows of part k of a sample of `spots` rows cut into `parts`.
-__device__ __forceinline__ void part_rows(long long spots, int parts, int k, long long& lo, long long& hi) {
-  lo = spots * k / parts;
-  hi = spots * (k + 1) / parts;
+template <typename K>
+static cudaError_t allow_smem(K kernel, int bytes) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-// How many rows of [lo, hi) slot s has: lo + s, lo + s + slots, ...
-__device__ __forceinline__ int slot_rows(long long lo, long long hi, int s, int slots) {
-  const int n = (int)(hi - lo);
-  return n > s ? (n - s + slots - 1) / slots : 0;
-}
+// c / w for 0 <= c < 2^14, w >= 1, where inv = 1.f / w: (c + 1/2) / w is at least 1 / (2 w) from a whole
+// number, and the rounding is below 2^14 / w * 2^-22.
+__device__ __forceinline__ int quotient(int c, float inv) { return (int)(((float)c + 0.5f) * inv); }
+
+// A block's rows of a sample, part k, and a thread's place among them: its column of a tile of
+// channels, and the rows slot, slot + slots, ... of which there are `mine`.
+struct SplitPlace {
+  int rows, slot, col, mine;
+  long long step;   // elements between two rows of a slot
+  long long first;  // element of a thread's first row, channel 0, in sample 0
+  __device__ __forceinline__ SplitPlace(const GroupNormArgs& a, const GroupNormPlan& p, int k) {
+    rows = k == p.parts - 1 ? (int)(a.spots - (long long)k * p.part_rows) : p.part_rows;
+    slot = threadIdx.x / p.cols;
+    col = threadIdx.x % p.cols;
+    mine = slot < p.slots && rows > slot ? (rows - slot + p.slots - 1) / p.slots : 0;
+    step = (long long)p.slots * a.channels;
+    first = ((long long)k * p.part_rows + slot) * a.channels;
+  }
+};
+
+// A thread's V channels of one tile: the first, and their parameters.  With one tile (up to 1024
+// channels) they are read once for all samples.
+template <int V>
+struct SplitColumn {
+  int c;
+  float inv_w;
+  float wt[V], bs[V];
+  bool live;
+  __device__ __forceinline__ int group(int v) const { return quotient(c + v, inv_w); }
+  __device__ __forceinline__ void set(const GroupNormArgs& a, const GroupNormPlan& p, const SplitPlace& at, int tile) {
+    c = (tile * p.cols + at.col) * V;
+    live = at.slot < p.slots && c < a.channels;
+    if (!live) return;
+    inv_w = 1.f / (float)(a.channels / a.groups);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      wt[v] = a.weight ? a.weight[c + v] : 1.f;
+      bs[v] = a.bias ? a.bias[c + v] : 0.f;
+    }
+  }
+};
 
 }  // namespace gn
 }  // namespace tfb

@@ -30,23 +30,25 @@ struct GroupNormArgs {
   int act;
 };
 
-// How a call is run; it depends on the sizes, the element size and the device alone.
+// How a call is run; it depends on the sizes, the element size and the alignment alone.
 struct GroupNormPlan {
   enum Kind { kSmall, kSplit, kAny } kind;
   int vec;         // elements of one access
   // kSmall: one group of `lanes` threads per (sample, group), nv accesses each
   int lanes, nv;
-  // kSplit: `parts` blocks per sample, `slots` rows of `cols` threads per block
-  int parts, slots, cols, tiles, threads, smem;
-  int grid;        // blocks (kSplit with parts > 1: all resident)
-  // work area, in bytes from its start (all 16-byte aligned)
-  long long off_stats, off_channels, channel_rows, off_sync, bytes;
+  // kSplit: `parts` blocks of `part_rows` rows per sample, `slots` rows of `cols` threads per block
+  int parts, part_rows, slots, cols, tiles, threads, smem;
+  int glanes, planes;  // threads that join a group's sets within a block, across the parts
+  int grid;
+  // work area, in bytes from its start (all 16-byte aligned); the parts' sets come first
+  long long off_result, off_channels, channel_rows, off_sync, bytes;
 };
 
 constexpr int kNormThreads = 256;
-constexpr int kSplitThreadsPerSm = 768;
-constexpr int kMaxSplitChannels = 8192;  // two float2 each in shared memory
+constexpr int kMaxSplitChannels = 8192;  // three float2 each in shared memory
 constexpr int kSms = 148;
+// Rows of `bytes` that a thread of kSplit has on their way at a time.
+constexpr int rows_ahead(int bytes) { return 64 / bytes < 4 ? 64 / bytes : 4; }
 
 // align: what all of x, y and dy are multiples of (16, 8, 4 or 2 bytes)
 GroupNormPlan plan_group_norm(ElemType t, const GroupNormArgs& a, bool backward, int align);

@@ -14,7 +14,7 @@ namespace tfb {
 namespace gn {
 
 template <typename T, int V, int NV, int ACT>
-__global__ void __launch_bounds__(kNormThreads) k_gn_small_bwd(const __grid_constant__ GroupNormArgs a, int lanes) {
+__global__ void __launch_bounds__(kNormThreads, small_blocks_bwd(NV)) k_gn_small_bwd(const __grid_constant__ GroupNormArgs a, int lanes) {
   const int w = a.channels / a.groups, count = (int)a.spots * w;
   const int per = kNormThreads / lanes, lane = threadIdx.x & (lanes - 1);
   const long long slots = (long long)gridDim.x * per / a.groups * a.groups;
@@ -35,29 +35,52 @@ __global__ void __launch_bounds__(kNormThreads) k_gn_small_bwd(const __grid_cons
     }
   }
   const float inv = 1.f / (float)count;
-  const long long turns = (total + slots - 1) / slots;
-  for (long long k = 0; k < turns; ++k) {
-    const long long id = first + k * slots;
-    const bool live = first < slots && id < total;
-    const long long base = live ? id / a.groups * a.spots * a.channels + (long long)g * w : 0;
-    const T* x = static_cast<const T*>(a.x) + base;
-    const T* dy = static_cast<const T*>(a.dy) + base;
-    Pack<T, V> h[NV], u[NV];
+  const long long step = slots / a.groups * a.spots * a.channels;  // from one of a thread's groups to its next
+  const long long base = first / a.groups * a.spots * a.channels + (long long)g * w;
+  const T* x = static_cast<const T*>(a.x) + base;
+  const T* dy = static_cast<const T*>(a.dy) + base;
+  T* dx = static_cast<T*>(a.y) + base;
+  int left = first < slots && first < total ? (int)((total - first + slots - 1) / slots) : 0;
+  int turns = (int)((total + slots - 1) / slots);
+  const float *mean_at = a.mean + first, *rstd_at = a.rstd + first;
+  typename Pack<T, V>::Raw ahead_x[NV], ahead_dy[NV];
+  float next_mean = 0.f, next_rstd = 0.f;
+  if (left > 0) {
+    next_mean = *mean_at;
+    next_rstd = *rstd_at;
+  }
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (live && off[j] >= 0) {
-        h[j].load(x + off[j]);
-        u[j].load(dy + off[j]);
+  for (int j = 0; j < NV; ++j)
+    if (left > 0 && off[j] >= 0) {
+      ahead_x[j] = Pack<T, V>::raw(x + off[j]);
+      ahead_dy[j] = Pack<T, V>::raw(dy + off[j]);
+    }
+  for (; turns > 0; --turns, --left, x += step, dy += step, dx += step) {
+    Pack<T, V> h[NV], u[NV];
+    const float mean = next_mean, rstd = next_rstd;
+    if (left > 1) {
+      mean_at += slots;
+      rstd_at += slots;
+      next_mean = *mean_at;
+      next_rstd = *rstd_at;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      h[j].unpack(ahead_x[j]);
+      u[j].unpack(ahead_dy[j]);
+      if (left > 1 && off[j] >= 0) {
+        ahead_x[j] = Pack<T, V>::raw(x + step + off[j]);
+        ahead_dy[j] = Pack<T, V>::raw(dy + step + off[j]);
       }
-    const float mean = live ? a.mean[id] : 0.f, rstd = live ? a.rstd[id] : 0.f;
+    }
     float su = 0.f, suh = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (live && off[j] >= 0) {
+      if (left > 0 && off[j] >= 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float hv = (h[j].x[v] - mean) * rstd;
-          const float dz = u[j].x[v] * slope<T, ACT>(fmaf(hv, wt[j][v], bs[j][v]));
+          const float dz = u[j].x[v] * slope<ACT>(fmaf(hv, wt[j][v], bs[j][v]));
           db[j][v] += dz;
           dw[j][v] = fmaf(dz, hv, dw[j][v]);
           h[j].x[v] = hv;
@@ -67,10 +90,10 @@ __global__ void __launch_bounds__(kNormThreads) k_gn_small_bwd(const __grid_cons
         }
       }
     if (!a.y) continue;
-    su = lanes_sum(su, lanes) * inv;
-    suh = lanes_sum(suh, lanes) * inv;
-    if (live) {
-      T* dx = static_cast<T*>(a.y) + base;
+    lanes_sum(su, suh, lanes);
+    su *= inv;
+    suh *= inv;
+    if (left > 0) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (off[j] >= 0) {
@@ -92,7 +115,7 @@ __global__ void __launch_bounds__(kNormThreads) k_gn_small_bwd(const __grid_cons
 }
 
 struct SplitBwdSmem {
-  float2* red;    // slots * cols * V: sums of (dz h, dz) of a slot
+  float2* red;    // slots * channels: sums of (dz h, dz) of a slot
   float2* chan;   // channels: of the block's rows of one sample
   float2* acc;    // channels: of all its samples
   float2* group;  // groups: (mean of u, mean of u h)
@@ -100,207 +123,218 @@ struct SplitBwdSmem {
 
 template <typename T, int V, int ACT>
 __device__ __forceinline__ void split_sums(const GroupNormArgs& a, const GroupNormPlan& p, const SplitBwdSmem& sm,
-                                           long long n, int k, float2* part) {
-  constexpr int U = 2;
-  const int slot = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
-  long long lo, hi;
-  part_rows(a.spots, p.parts, k, lo, hi);
-  const T* x = static_cast<const T*>(a.x) + n * a.spots * a.channels;
-  const T* dy = static_cast<const T*>(a.dy) + n * a.spots * a.channels;
+                                           const SplitPlace& at, SplitColumn<V>& col, long long n, float2* out) {
+  constexpr int U = rows_ahead(2 * V * sizeof(T));
+  const long long base = n * a.spots * a.channels + at.first;
   const int w = a.channels / a.groups;
   for (int tile = 0; tile < p.tiles; ++tile) {
-    const int c = (tile * p.cols + col) * V;
-    if (slot < p.slots && c < a.channels) {
-      float mean[V], rstd[V], wt[V], bs[V], sw[V], sb[V];
+    if (p.tiles > 1) col.set(a, p, at, tile);
+    if (!col.live) continue;
+    float mean[V], gain[V], sw[V], sb[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const long long at = n * a.groups + (c + v) / w;
-        mean[v] = a.mean[at];
-        rstd[v] = a.rstd[at];
-        wt[v] = a.weight ? a.weight[c + v] : 1.f;
-        bs[v] = a.bias ? a.bias[c + v] : 0.f;
-        sw[v] = sb[v] = 0.f;
-      }
-      const long long step = (long long)p.slots * a.channels, at = (lo + slot) * a.channels + c;
-      const T *px = x + at, *pd = dy + at;
-      for (int left = slot_rows(lo, hi, slot, p.slots); left > 0; left -= U, px += U * step, pd += U * step) {
-        Pack<T, V> q[U], d[U];
+    for (int v = 0; v < V; ++v) {
+      const long long g = n * a.groups + col.group(v);
+      mean[v] = a.mean[g];
+      gain[v] = a.rstd[g] * col.wt[v];
+      sw[v] = sb[v] = 0.f;
+    }
+    const T* px = static_cast<const T*>(a.x) + base + col.c;
+    const T* pd = static_cast<const T*>(a.dy) + base + col.c;
+    for (int left = at.mine; left > 0; left -= U, px += U * at.step, pd += U * at.step) {
+      typename Pack<T, V>::Raw rx[U], rd[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i)
-          if (i < left) {
-            q[i].load(px + i * step);
-            d[i].load(pd + i * step);
+      for (int i = 0; i < U; ++i)
+        if (i < left) {
+          rx[i] = Pack<T, V>::raw(px + i * at.step);
+          rd[i] = Pack<T, V>::raw(pd + i * at.step);
+        }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (i < left) {
+          Pack<T, V> q, d;
+          q.unpack(rx[i]);
+          d.unpack(rd[i]);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float e = q.x[v] - mean[v], dz = d.x[v] * slope<ACT>(fmaf(e, gain[v], col.bs[v]));
+            sb[v] += dz;
+            sw[v] = fmaf(dz, e, sw[v]);
           }
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-          if (i < left) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-              const float h = (q[i].x[v] - mean[v]) * rstd[v];
-              const float dz = d[i].x[v] * slope<T, ACT>(fmaf(h, wt[v], bs[v]));
-              sb[v] += dz;
-              sw[v] = fmaf(dz, h, sw[v]);
-            }
-          }
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) sm.red[(slot * p.cols + col) * V + v] = make_float2(sw[v], sb[v]);
+        }
     }
-    __syncthreads();
-    const int width = p.cols * V;
-    for (int i = threadIdx.x; i < width && tile * width + i < a.channels; i += blockDim.x) {
-      float2 s = make_float2(0.f, 0.f);
-      for (int j = 0; j < p.slots; ++j) {
-        const float2 b = sm.red[j * width + i];
-        s.x += b.x;
-        s.y += b.y;
-      }
-      sm.chan[tile * width + i] = s;
-      float2& acc = sm.acc[tile * width + i];
-      acc.x += s.x;
-      acc.y += s.y;
-    }
-    __syncthreads();
+    float2* red = sm.red + at.slot * a.channels + col.c;
+#pragma unroll
+    for (int v = 0; v < V; ++v) red[v] = make_float2(sw[v] * a.rstd[n * a.groups + col.group(v)], sb[v]);
   }
-  if (!a.y) return;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
-  for (int g = warp; g < a.groups; g += warps) {
-    float su = 0.f, suh = 0.f;
-    for (int c = lane; c < w; c += 32) {
-      const float2 b = sm.chan[g * w + c];
-      const float wc = a.weight ? a.weight[g * w + c] : 1.f;
-      su = fmaf(b.y, wc, su);
-      suh = fmaf(b.x, wc, suh);
-    }
-    su = warp_sum(su);
-    suh = warp_sum(suh);
-    if (lane == 0) {
-      if (p.parts > 1)
-        part[((long long)n * p.parts + k) * a.groups + g] = make_float2(su, suh);
-      else
-        sm.group[g] = make_float2(su, suh);
-    }
-  }
-}
-
-template <typename T, int V, int ACT>
-__device__ __forceinline__ void split_dx(const GroupNormArgs& a, const GroupNormPlan& p, const SplitBwdSmem& sm, long long n,
-                                         int k, const float2* part) {
-  constexpr int U = 2;
-  const int w = a.channels / a.groups;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
-  const float inv = 1.f / (float)(a.spots * w);
   __syncthreads();
-  for (int g = warp; g < a.groups; g += warps) {
+  for (int i = threadIdx.x; i < a.channels; i += blockDim.x) {
+    float2 s = make_float2(0.f, 0.f);
+    for (int j = 0; j < p.slots; ++j) {
+      const float2 b = sm.red[j * a.channels + i];
+      s.x += b.x;
+      s.y += b.y;
+    }
+    float2& acc = sm.acc[i];
+    acc.x += s.x;
+    acc.y += s.y;
+    const float wc = a.weight ? a.weight[i] : 1.f;
+    sm.chan[i] = make_float2(s.y * wc, s.x * wc);
+  }
+  __syncthreads();
+  if (!out) return;
+  const int lanes = p.glanes, lane = threadIdx.x & (lanes - 1);
+  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x / lanes) {
+    const int g = g0 + threadIdx.x / lanes;
     float su = 0.f, suh = 0.f;
-    if (p.parts > 1) {
-      const float2* at = part + (long long)n * p.parts * a.groups + g;
-      for (int i = lane; i < p.parts; i += 32) {
-        const float2 b = __ldcg(at + (long long)i * a.groups);
+    if (g < a.groups)
+      for (int c = lane; c < w; c += lanes) {
+        const float2 b = sm.chan[g * w + c];
         su += b.x;
         suh += b.y;
       }
-      su = warp_sum(su);
-      suh = warp_sum(suh);
-    } else {
-      su = sm.group[g].x;
-      suh = sm.group[g].y;
-    }
-    __syncwarp();
-    if (lane == 0) sm.group[g] = make_float2(su * inv, suh * inv);
+    lanes_sum(su, suh, lanes);
+    if (g < a.groups && lane == 0) out[g] = make_float2(su, suh);
   }
-  __syncthreads();
-  const int slot = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
-  long long lo, hi;
-  part_rows(a.spots, p.parts, k, lo, hi);
-  const long long base = n * a.spots * a.channels;
-  const T* x = static_cast<const T*>(a.x) + base;
-  const T* dy = static_cast<const T*>(a.dy) + base;
-  T* dx = static_cast<T*>(a.y) + base;
-  for (int tile = 0; tile < p.tiles; ++tile) {
-    const int c = (tile * p.cols + col) * V;
-    if (slot >= p.slots || c >= a.channels) continue;
-    float mean[V], rstd[V], wt[V], bs[V], mu[V], muh[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int g = (c + v) / w;
-      mean[v] = a.mean[n * a.groups + g];
-      rstd[v] = a.rstd[n * a.groups + g];
-      wt[v] = a.weight ? a.weight[c + v] : 1.f;
-      bs[v] = a.bias ? a.bias[c + v] : 0.f;
-      mu[v] = sm.group[g].x;
-      muh[v] = sm.group[g].y;
-    }
-    const long long step = (long long)p.slots * a.channels, at = (lo + slot) * a.channels + c;
-    const T *px = x + at, *pd = dy + at;
-    T* to = dx + at;
-    for (int left = slot_rows(lo, hi, slot, p.slots); left > 0;
-         left -= U, px += U * step, pd += U * step, to += U * step) {
-      Pack<T, V> q[U], d[U];
-#pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (i < left) {
-          q[i].load(px + i * step);
-          d[i].load(pd + i * step);
-        }
-#pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (i < left) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const float h = (q[i].x[v] - mean[v]) * rstd[v];
-            const float u = d[i].x[v] * slope<T, ACT>(fmaf(h, wt[v], bs[v])) * wt[v];
-            q[i].x[v] = rstd[v] * (u - mu[v] - h * muh[v]);
-          }
-          q[i].store(to + i * step);
-        }
-    }
-  }
-  __syncthreads();
 }
 
+// dx of the block's rows of sample n, given the sums of (u, u h) over its groups times `inv`.
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads, kSplitThreadsPerSm / kNormThreads)
-    k_gn_split_bwd(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
-  extern __shared__ __align__(16) float2 smem[];
+__device__ __forceinline__ void split_dx(const GroupNormArgs& a, const GroupNormPlan& p, const SplitPlace& at,
+                                         SplitColumn<V>& col, long long n, const float2* group, float inv) {
+  constexpr int U = rows_ahead(2 * V * sizeof(T));
+  const long long first = n * a.spots * a.channels + at.first;
+  for (int tile = 0; tile < p.tiles; ++tile) {
+    if (p.tiles > 1) col.set(a, p, at, tile);
+    if (!col.live) continue;
+    // with e = x - mean: dx = gain dz - rstd mean(u) - e rstd^2 mean(u h)
+    float mean[V], gain[V], mu[V], muh[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int g = col.group(v);
+      const float rstd = a.rstd[n * a.groups + g];
+      const float2 m = group[g];
+      mean[v] = a.mean[n * a.groups + g];
+      gain[v] = rstd * col.wt[v];
+      mu[v] = rstd * (m.x * inv);
+      muh[v] = rstd * rstd * (m.y * inv);
+    }
+    const T* px = static_cast<const T*>(a.x) + first + col.c;
+    const T* pd = static_cast<const T*>(a.dy) + first + col.c;
+    T* to = static_cast<T*>(a.y) + first + col.c;
+    for (int left = at.mine; left > 0; left -= U, px += U * at.step, pd += U * at.step, to += U * at.step) {
+      typename Pack<T, V>::Raw rx[U], rd[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (i < left) {
+          rx[i] = Pack<T, V>::raw(px + i * at.step);
+          rd[i] = Pack<T, V>::raw(pd + i * at.step);
+        }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (i < left) {
+          Pack<T, V> q, d;
+          q.unpack(rx[i]);
+          d.unpack(rd[i]);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float e = q.x[v] - mean[v], dz = d.x[v] * slope<ACT>(fmaf(e, gain[v], col.bs[v]));
+            q.x[v] = fmaf(-e, muh[v], fmaf(dz, gain[v], -mu[v]));
+          }
+          q.store(to + i * at.step);
+        }
+    }
+  }
+}
+
+__device__ __forceinline__ SplitBwdSmem bwd_smem(const GroupNormArgs& a, const GroupNormPlan& p, float2* smem) {
   SplitBwdSmem sm;
   sm.red = smem;
-  sm.chan = sm.red + p.slots * p.cols * V;
+  sm.chan = sm.red + p.slots * a.channels;
   sm.acc = sm.chan + a.channels;
   sm.group = sm.acc + a.channels;
   for (int c = threadIdx.x; c < a.channels; c += blockDim.x) sm.acc[c] = make_float2(0.f, 0.f);
   __syncthreads();
-  if (p.parts == 1) {
-    for (long long n = blockIdx.x; n < a.batch; n += gridDim.x) {
-      split_sums<T, V, ACT>(a, p, sm, n, 0, nullptr);
-      if (a.y) split_dx<T, V, ACT>(a, p, sm, n, 0, nullptr);
-    }
-  } else {
-    float2* part = static_cast<float2*>(a.work);
-    unsigned* sync = reinterpret_cast<unsigned*>(static_cast<char*>(a.work) + p.off_sync);
-    const int k = blockIdx.x % p.parts, step = gridDim.x / p.parts;
-    long long n = blockIdx.x / p.parts;
-    split_sums<T, V, ACT>(a, p, sm, n, k, part);
-    if (a.y) sample_arrive(sync + n);
-    for (; n < a.batch; n += step) {
-      const long long next = n + step;
-      if (next < a.batch) {
-        split_sums<T, V, ACT>(a, p, sm, next, k, part);
-        if (a.y) sample_arrive(sync + next);
-      }
-      if (a.y) {
-        sample_wait(sync + n, (unsigned)p.parts);
-        split_dx<T, V, ACT>(a, p, sm, n, k, part);
-      }
-    }
-  }
+  return sm;
+}
+
+__device__ __forceinline__ void leave_channels(const GroupNormArgs& a, const GroupNormPlan& p, const SplitBwdSmem& sm) {
   __syncthreads();
   float2* out = reinterpret_cast<float2*>(static_cast<char*>(a.work) + p.off_channels) + (long long)blockIdx.x * a.channels;
   for (int c = threadIdx.x; c < a.channels; c += blockDim.x) out[c] = sm.acc[c];
 }
 
+// A block takes whole samples.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 3)
+    k_gn_whole_bwd(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  extern __shared__ __align__(16) float2 smem[];
+  const SplitBwdSmem sm = bwd_smem(a, p, smem);
+  const SplitPlace at(a, p, 0);
+  SplitColumn<V> col;
+  col.set(a, p, at, 0);
+  const float inv = 1.f / ((float)a.spots * (float)(a.channels / a.groups));
+  for (long long n = blockIdx.x; n < a.batch; n += gridDim.x) {
+    split_sums<T, V, ACT>(a, p, sm, at, col, n, sm.group);
+    __syncthreads();
+    if (a.y) split_dx<T, V, ACT>(a, p, at, col, n, sm.group, inv);
+  }
+  leave_channels(a, p, sm);
+}
+
+// Block = part blockIdx.x % parts of sample blockIdx.x / parts: its channels' and groups' sums; the
+// sample's last block adds up the groups'.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 3)
+    k_gn_sums(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  extern __shared__ __align__(16) float2 smem[];
+  const SplitBwdSmem sm = bwd_smem(a, p, smem);
+  const long long n = blockIdx.x / p.parts;
+  const int k = blockIdx.x % p.parts;
+  float2* part = static_cast<float2*>(a.work) + n * p.parts * a.groups;
+  {
+    const SplitPlace at(a, p, k);
+    SplitColumn<V> col;
+    col.set(a, p, at, 0);
+    split_sums<T, V, ACT>(a, p, sm, at, col, n, a.y ? part + (long long)k * a.groups : nullptr);
+  }
+  leave_channels(a, p, sm);
+  if (!a.y) return;
+  unsigned* count = reinterpret_cast<unsigned*>(static_cast<char*>(a.work) + p.off_sync);
+  if (!last_of_sample(count + n, p.parts)) return;
+  float2* result = reinterpret_cast<float2*>(static_cast<char*>(a.work) + p.off_result) + n * a.groups;
+  const int lanes = p.planes, lane = threadIdx.x & (lanes - 1);
+  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x / lanes) {
+    const int g = g0 + threadIdx.x / lanes;
+    float su = 0.f, suh = 0.f;
+    if (g < a.groups) {
+#pragma unroll 8
+      for (int i = lane; i < p.parts; i += lanes) {
+        const float2 b = __ldcg(part + (long long)i * a.groups + g);
+        su += b.x;
+        suh += b.y;
+      }
+    }
+    lanes_sum(su, suh, lanes);
+    if (g < a.groups && lane == 0) result[g] = make_float2(su, suh);
+  }
+}
+
+// From the last sample to the first: the end of x and dy is in L2 still.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 3)
+    k_gn_dx(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  const unsigned b = gridDim.x - 1 - blockIdx.x;
+  const long long n = b / p.parts;
+  const SplitPlace at(a, p, b % p.parts);
+  SplitColumn<V> col;
+  col.set(a, p, at, 0);
+  const float2* result = reinterpret_cast<const float2*>(static_cast<const char*>(a.work) + p.off_result);
+  const float inv = 1.f / ((float)a.spots * (float)(a.channels / a.groups));
+  split_dx<T, V, ACT>(a, p, at, col, n, result + n * a.groups, inv);
+}
+
 // dw, db = the sums of the blocks' rows of channel sums.
-constexpr int kSumCols = 16, kSumRows = 32;
+constexpr int kSumCols = 8, kSumRows = 64;
 __global__ void __launch_bounds__(kSumCols * kSumRows) k_gn_sum_rows(const float2* __restrict__ rows, long long count,
                                                                      int channels, float* __restrict__ dw,
                                                                      float* __restrict__ db) {
@@ -308,7 +342,7 @@ __global__ void __launch_bounds__(kSumCols * kSumRows) k_gn_sum_rows(const float
   const int col = threadIdx.x % kSumCols, slot = threadIdx.x / kSumCols, c = blockIdx.x * kSumCols + col;
   float2 s = make_float2(0.f, 0.f);
   if (c < channels) {
-#pragma unroll 4
+#pragma unroll 8
     for (long long r = slot; r < count; r += kSumRows) {
       const float2 b = rows[r * channels + c];
       s.x += b.x;
@@ -361,7 +395,7 @@ __global__ void __launch_bounds__(kNormThreads) k_gn_any_dx(const __grid_constan
           const long long at = base + r * a.channels + i;
           const int c = g * w + i;
           const float wc = a.weight ? a.weight[c] : 1.f, h = (to_f32(static_cast<const T*>(a.x)[at]) - mean) * rstd;
-          const float u = to_f32(static_cast<const T*>(a.dy)[at]) * slope<T, ACT>(fmaf(h, wc, a.bias ? a.bias[c] : 0.f)) * wc;
+          const float u = to_f32(static_cast<const T*>(a.dy)[at]) * slope<ACT>(fmaf(h, wc, a.bias ? a.bias[c] : 0.f)) * wc;
           if (pass) {
             static_cast<T*>(a.y)[at] = from_f32<T>(rstd * (u - su - h * suh));
           } else {
@@ -382,7 +416,7 @@ __global__ void __launch_bounds__(kNormThreads) k_gn_any_dw(const __grid_constan
   for (long long i = threadIdx.x; i < a.batch * a.spots; i += kNormThreads) {
     const long long n = i / a.spots * a.groups + g;
     const float h = (to_f32(static_cast<const T*>(a.x)[i * a.channels + c]) - a.mean[n]) * a.rstd[n];
-    const float dz = to_f32(static_cast<const T*>(a.dy)[i * a.channels + c]) * slope<T, ACT>(fmaf(h, wc, bc));
+    const float dz = to_f32(static_cast<const T*>(a.dy)[i * a.channels + c]) * slope<ACT>(fmaf(h, wc, bc));
     sb += dz;
     sw = fmaf(dz, h, sw);
   }
@@ -408,20 +442,18 @@ static cudaError_t run_small(const GroupNormArgs& a, const GroupNormPlan& p, cud
 
 template <typename T, int V, int ACT>
 static cudaError_t run_split(const GroupNormArgs& a, const GroupNormPlan& p, cudaStream_t st) {
-  cudaError_t e = cudaSuccess;
-  if (p.smem > 48 * 1024)
-    e = cudaFuncSetAttribute(k_gn_split_bwd<T, V, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
-  if (e != cudaSuccess) return e;
+  cudaError_t e;
   if (p.parts == 1) {
-    k_gn_split_bwd<T, V, ACT><<<p.grid, p.threads, p.smem, st>>>(a, p);
-    return cudaGetLastError();
+    e = allow_smem(k_gn_whole_bwd<T, V, ACT>, p.smem);
+    if (e == cudaSuccess) k_gn_whole_bwd<T, V, ACT><<<p.grid, p.threads, p.smem, st>>>(a, p);
+    return e == cudaSuccess ? cudaGetLastError() : e;
   }
-  e = cudaMemsetAsync(static_cast<char*>(a.work) + p.off_sync, 0, sizeof(unsigned) * a.batch, st);
+  e = allow_smem(k_gn_sums<T, V, ACT>, p.smem);
+  if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<char*>(a.work) + p.off_sync, 0, sizeof(unsigned) * a.batch, st);
   if (e != cudaSuccess) return e;
-  GroupNormArgs a2 = a;
-  GroupNormPlan p2 = p;
-  void* args[] = {&a2, &p2};
-  return cudaLaunchCooperativeKernel(k_gn_split_bwd<T, V, ACT>, dim3(p.grid), dim3(p.threads), args, (size_t)p.smem, st);
+  k_gn_sums<T, V, ACT><<<p.grid, p.threads, p.smem, st>>>(a, p);
+  if (a.y) k_gn_dx<T, V, ACT><<<p.grid, p.threads, 0, st>>>(a, p);
+  return cudaGetLastError();
 }
 
 template <typename T, int ACT>
