@@ -94,6 +94,20 @@ def test_ends_of_the_decay(kind, dtype):
     assert bool(torch.isfinite(dq).all())
 
 
+def test_very_slow_decay_over_many_tokens():
+    """The factor of a chunk is kept to more than 32 bits: thousands of them must not add up."""
+    t = 20000
+    q, k, v, _ = inputs(1, t, 1, 1, 32, 32, torch.float32)
+    g = torch.tensor([-1.0 / 3e5]).cuda()
+    o, s = trnfft.decay_attention(q, k, v, g, return_state=True)
+    pos = torch.arange(t, device="cuda", dtype=torch.float64)
+    w = torch.exp(g.double() * (t - 1 - pos))[:, None]
+    want = (k[0, :, 0].double() * w).mT @ v[0, :, 0].double()
+    assert float((s[0, 0].double() - want).norm() / want.norm()) < 2e-6
+    last = q[0, -1, 0].double() @ want * 32 ** -0.5
+    assert float((o[0, -1, 0].double() - last).norm() / last.norm()) < 5e-6
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("size", SIZES)
 @pytest.mark.parametrize("carried", [False, True])
@@ -299,6 +313,33 @@ def test_step(size, dtype):
     check(wide, ws, ts, dtype, 4, "state", fp32_out=True)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,b,h", [(5000, 1, 1), (9001, 1, 3), (3000, 2, 5)])
+def test_long_sequences_in_segments(t, b, h, dtype):
+    """Few heads and a long axis: the sequences are cut, forwards and backwards."""
+    d = 32
+    q, k, v, do = inputs(b, t, h, h, d, d, dtype, seed=11)
+    g = rates(h)
+    first, dlast = (torch.randn(b, h, d, d, device="cuda") for _ in range(2))
+    leaves = [x.requires_grad_() for x in (q, k, v, first)]
+    o, s = trnfft.decay_attention(q, k, v, g, initial_state=first, return_state=True)
+    got = torch.autograd.grad((o, s), leaves, (do, dlast))
+    xs = [x.detach().double().requires_grad_() for x in leaves]
+    pos = torch.arange(t, device="cuda", dtype=torch.float64)
+    behind = pos[:, None] - pos
+    w = torch.exp(g.double()[:, None, None] * behind.clamp_min(0)) * (behind >= 0)
+    qd, kd, vd = (x.transpose(1, 2) for x in xs[:3])
+    ahead = torch.exp(g.double()[:, None] * (pos + 1))[None, :, :, None]
+    wo = ((qd @ kd.mT * w) @ vd + (qd @ xs[3]) * ahead) * d ** -0.5
+    left = torch.exp(g.double()[:, None] * (t - 1 - pos))[None, :, :, None]
+    ws = (kd * left).mT @ vd + xs[3] * torch.exp(g.double() * t)[:, None, None]
+    wg = torch.autograd.grad((wo.transpose(1, 2), ws), xs, (do.double(), dlast.double()))
+    rel = {torch.float32: 3e-6, torch.bfloat16: 5e-3, torch.float16: 1e-3}
+    for name, x, y in zip(("o", "state", "dq", "dk", "dv", "dinitial"), (o, s, *got), (wo.transpose(1, 2), ws, *wg)):
+        off = float((x.detach().double() - y).norm() / y.norm())
+        assert off < rel[torch.float32 if name in ("state", "dinitial") else dtype], (name, off)
+
+
 def test_step_refuses_overlap():
     s = torch.zeros(3, 2, 8, 8, device="cuda")
     q = torch.zeros(2, 2, 8, device="cuda")
@@ -339,6 +380,8 @@ def test_other_values_stay_in_their_rows():
         o = trnfft.decay_attention(q, k, v2, g)
         assert torch.equal(o[0], want[0]) and torch.equal(o[1, :, 1], want[1, :, 1])
         assert not bool(torch.isfinite(o[1, 100, 0]).any())
+        assert bool(torch.isfinite(o[1, :100, 0]).all()), "a token's value reaches no row before it"
+        assert float((o[1, :100, 0].float() - want[1, :100, 0].float()).abs().max()) <= 0.02 * float(want.float().abs().max())
         packed = trnfft.decay_attention(*(x.reshape(1, 400, 2, 64) for x in (q, k, v2)), g,
                                         cu_seqlens=torch.tensor([0, 150, 290, 310, 400], device="cuda"))
         assert bool(torch.isfinite(packed[0, :290]).all()) and bool(torch.isfinite(packed[0, 310:]).all())

@@ -67,8 +67,8 @@ int check_shape(const char* fn, const trnfft_decay_shape* s) {
   if (s->cu_seqlens && misaligned(s->cu_seqlens, s->cu_is64 ? 8 : 4))
     return bad(TRNFFT_INVALID_VALUE, "%s: misaligned cu_seqlens", fn);
   const int64_t n = s->cu_seqlens ? s->num_seqs : s->batch;
-  if (s->heads > 65535 || n > INT_MAX / 2 || s->tokens > INT_MAX / 2)
-    return bad(TRNFFT_UNSUPPORTED, "%s: more than 65535 heads, 2^30 sequences or 2^30 tokens", fn);
+  if (s->heads > 65535 || n >= (1 << 30) / s->heads || s->tokens > INT_MAX / 2)
+    return bad(TRNFFT_UNSUPPORTED, "%s: more than 65535 heads, 2^30 states or 2^30 tokens", fn);
   return TRNFFT_SUCCESS;
 }
 
@@ -130,7 +130,7 @@ int check_operands(const char* fn, const trnfft_decay_shape* s, std::initializer
 // float32 gradients of the query heads' own keys and values, before the heads of a group are summed
 int64_t head_grad_bytes(const trnfft_decay_shape* s) {
   if (s->heads == s->kv_heads) return 0;
-  return 4 * s->batch * s->tokens * s->heads * (s->key_width + s->value_width);
+  return (4 * s->batch * s->tokens * s->heads * (s->key_width + s->value_width) + 15) & ~(int64_t)15;
 }
 
 }  // namespace
@@ -142,7 +142,25 @@ extern "C" {
 
 int64_t trnfft_decay_attention_work_bytes(const trnfft_decay_shape* s, int backward) {
   if (check_shape("decay_attention_work_bytes", s)) return -1;
-  return backward ? head_grad_bytes(s) : 0;
+  DecayArgs a = base_args(s, nullptr);
+  const int wk = (int)s->key_width, wv = (int)s->value_width;
+  if (!backward) {
+    a.roles = 1;
+    a.role[0].wk = wk;
+    a.role[0].wv = wv;
+    return plan_decay_attention((ElemType)s->dtype, a);
+  }
+  // whichever of the gradients are asked for
+  int64_t most = 0;
+  for (a.roles = 1; a.roles <= kMaxRoles; ++a.roles) {
+    for (int i = 0; i < a.roles; ++i) {
+      a.role[i].wk = wk;
+      a.role[i].wv = wv;
+    }
+    const int64_t bytes = plan_decay_attention((ElemType)s->dtype, a);
+    most = bytes > most ? bytes : most;
+  }
+  return head_grad_bytes(s) + most;
 }
 
 int trnfft_decay_attention(const trnfft_decay_shape* s, const void* q, const void* k, const void* v, const float* log_decay,
@@ -163,10 +181,11 @@ int trnfft_decay_attention(const trnfft_decay_shape* s, const void* q, const voi
   a.role[0].a = a.role[0].r = s->scale;
   a.role[0].first = initial;
   a.role[0].last = final_state;
-  (void)work;
+  if (!work && trnfft_decay_attention_work_bytes(s, 0)) return bad(TRNFFT_INVALID_VALUE, "%s: null work area", fn);
+  if (work && misaligned(work, 16)) return bad(TRNFFT_INVALID_VALUE, "%s: misaligned work area", fn);
   OnDevice d(device);
   if (!d.ok) return bad(TRNFFT_CUDA_ERROR, "%s: cannot select device %d", fn, device);
-  cudaError_t e = launch_decay_attention((ElemType)s->dtype, a, reinterpret_cast<cudaStream_t>(stream));
+  cudaError_t e = launch_decay_attention((ElemType)s->dtype, a, work, reinterpret_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? TRNFFT_SUCCESS : cuda_bad(e, fn);
 }
 
@@ -182,7 +201,7 @@ int trnfft_decay_attention_backward(const trnfft_decay_shape* s, const void* q, 
   if (!rows && (a.nseq == 0 || !d_initial)) return TRNFFT_SUCCESS;
   if (!log_decay || (rows && (!q || !k || !v || !d_o)))
     return bad(TRNFFT_INVALID_VALUE, "%s: null pointer", fn);
-  if (head_grad_bytes(s) && !work) return bad(TRNFFT_INVALID_VALUE, "%s: null work area", fn);
+  if (!work && trnfft_decay_attention_work_bytes(s, 1)) return bad(TRNFFT_INVALID_VALUE, "%s: null work area", fn);
   rc = check_operands(fn, s, {q, k, v, d_o, dq, dk, dv}, {log_decay, initial, d_final, d_initial});
   if (rc) return rc;
   if (work && misaligned(work, 16)) return bad(TRNFFT_INVALID_VALUE, "%s: misaligned work area", fn);
@@ -220,7 +239,7 @@ int trnfft_decay_attention_backward(const trnfft_decay_shape* s, const void* q, 
   OnDevice d(device);
   if (!d.ok) return bad(TRNFFT_CUDA_ERROR, "%s: cannot select device %d", fn, device);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_decay_attention((ElemType)s->dtype, a, st);
+  cudaError_t e = launch_decay_attention((ElemType)s->dtype, a, static_cast<char*>(work) + head_grad_bytes(s), st);
   if (e == cudaSuccess && grouped && rows) {
     const long long n = s->batch * s->tokens;
     if (dv) e = launch_sum_heads((ElemType)s->dtype, dv_heads, dv, n, (int)s->kv_heads, g, wv, st);

@@ -13,118 +13,84 @@
 #include "elem.cuh"
 #include "kernels.h"
 
+#include <algorithm>
+
+using std::max;
+
 namespace tfb {
 
-__device__ __forceinline__ long long cu_at(const DecayArgs& a, int i) {
-  long long x = a.cu64 ? static_cast<const long long*>(a.cu)[i] : (long long)static_cast<const int*>(a.cu)[i];
-  return x < 0 ? 0 : (x > a.tokens ? a.tokens : x);  // no value of cu leads outside the tensors
+namespace {
+
+constexpr int kChunk = 64;
+constexpr int kSms = 148;
+
+// Bits of DecayRole::wide.
+int wide_bits(const DecayRole& r, int size) {
+  auto rows = [&](const void* p, const long long* s, int w) {
+    return (reinterpret_cast<uintptr_t>(p) | s[0] * size | s[1] * size | s[2] * size | (long long)w * size) % 16 == 0;
+  };
+  const int osize = r.o_f32 ? 4 : size;
+  const bool o = (reinterpret_cast<uintptr_t>(r.o) | (long long)r.os[0] * osize | r.os[1] * osize | r.os[2] * osize |
+                  (long long)r.wv * osize) % (2 * osize) == 0;
+  return (rows(r.q, r.qs, r.wk) ? 1 : 0) | (rows(r.k, r.ks, r.wk) ? 2 : 0) | (rows(r.v, r.vs, r.wv) ? 4 : 0) | (o ? 8 : 0);
 }
 
-// One block per (head, sequence, role): the recurrence token by token, one
-// column of the state per thread in shared memory.  Right for every size; one
-// read of the operands, bound by the latency of its steps.
-template <typename T>
-__global__ void __launch_bounds__(128) k_decay_simple(const __grid_constant__ DecayArgs a) {
-  extern __shared__ float sm[];
-  const DecayRole& r = a.role[blockIdx.z];
-  const int h = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
-  const T* q = static_cast<const T*>(r.q) + (long long)(h / r.qdiv) * r.qs[2];
-  const T* k = static_cast<const T*>(r.k) + (long long)(h / r.kdiv) * r.ks[2];
-  const T* v = static_cast<const T*>(r.v) + (long long)(h / r.vdiv) * r.vs[2];
-  long long row0, n, obase = (long long)h * r.os[2];
-  if (a.cu) {
-    row0 = 0;
-    n = 0;
-    if (seq < a.nseq) {
-      row0 = cu_at(a, seq);
-      n = cu_at(a, seq + 1) - row0;
-    } else if (r.o) {  // the rows of no sequence
-      const long long head_rows = cu_at(a, 0), tail = cu_at(a, a.nseq);
-      for (long long t = 0; t < a.tokens; ++t)
-        if (t < head_rows || t >= tail)
-          for (int j = tid; j < r.wv; j += blockDim.x) {
-            const long long at = obase + t * r.os[1] + j;
-            if (r.o_f32)
-              static_cast<float*>(r.o)[at] = 0.f;
-            else
-              static_cast<T*>(r.o)[at] = from_f32<T>(0.f);
-          }
-      return;
-    }
-    if (n < 0) n = 0;
-  } else {
-    row0 = 0;
-    n = a.tokens;
-    q += seq * r.qs[0];
-    k += seq * r.ks[0];
-    v += seq * r.vs[0];
-    obase += seq * r.os[0];
-  }
-  if (seq >= a.nseq) return;
-  float* S = sm;                        // wk x wv
-  float* sq = S + r.wk * r.wv;          // wk
-  float* sk = sq + r.wk;                // wk
-  const long long sbase = ((long long)seq * a.heads + h) * r.wk * r.wv;
-  for (int i = 0; i < r.wk; ++i)
-    for (int j = tid; j < r.wv; j += blockDim.x)
-      S[i * r.wv + j] = r.first ? r.first[sbase + i * r.first_sk + j * r.first_sv] : 0.f;
-  const double gd = exp((double)a.log_decay[h]);
-  const float ghi = (float)gd, glo = (float)(gd - (double)ghi);
-  for (long long i = 0; i < n; ++i) {
-    const long long t = row0 + (r.back ? n - 1 - i : i);
-    __syncthreads();
-    for (int c = tid; c < r.wk; c += blockDim.x) {
-      sq[c] = r.o ? to_f32(q[t * r.qs[1] + c]) : 0.f;
-      sk[c] = to_f32(k[t * r.ks[1] + c]);
-    }
-    __syncthreads();
-    for (int j = tid; j < r.wv; j += blockDim.x) {
-      const float vj = to_f32(v[t * r.vs[1] + j]) * r.c;
-      float acc = 0.f;
-      for (int c = 0; c < r.wk; ++c) {
-        float s = S[c * r.wv + j];
-        if (!(r.back && i == 0)) s = fmaf(s, ghi, s * glo);
-        s = fmaf(sk[c], vj, s);
-        S[c * r.wv + j] = s;
-        acc = fmaf(sq[c], s, acc);
-      }
-      if (r.o) {
-        const long long at = obase + t * r.os[1] + j;
-        acc *= r.r;
-        if (r.o_f32)
-          static_cast<float*>(r.o)[at] = acc;
-        else
-          static_cast<T*>(r.o)[at] = from_f32<T>(acc);
-      }
+}  // namespace
+
+// A sequence is walked chunk by chunk, so with few (sequence, head, role) the GPU is filled by cutting
+// sequences into segments, at the cost of a pass that takes the segments' own states (it reads k and v
+// once more and does about 0.6 of a chunk's work) and a scan of these (about 3 chunks' time).  The
+// segment length, in chunks, is the one of least time by that count.
+int64_t plan_decay_attention(ElemType t, DecayArgs& a) {
+  const long long total = ((a.cu ? a.tokens : a.tokens) + kChunk - 1) / kChunk;  // chunks, of one dense or all packed sequences
+  int wide = 0;
+  for (int i = 0; i < a.roles; ++i) wide = max(wide, max(a.role[i].wk, a.role[i].wv));
+  const long long slots = (long long)kSms * (wide <= 64 ? 2 : 1), walks = (long long)a.heads * max(a.roles, 1);
+  // packed: how the rows fall on the sequences is on the device; take the longest for four times the mean
+  const long long longest = a.cu ? (a.nseq ? std::min(total, 4 * total / a.nseq + 1) : 0) : total;
+  auto units = [&](long long s) {
+    return a.cu ? (s >= total ? a.nseq : std::min<long long>(total / s + a.nseq, total + a.nseq)) : a.nseq * ((total + s - 1) / s);
+  };
+  auto time = [&](long long s) {
+    const double waves = (double)((units(s) * walks + slots - 1) / slots);
+    return s >= total ? std::max((double)longest, waves * total * (a.cu ? 1.0 / std::max(1, a.nseq) : 1.0))
+                      : waves * std::min(s, longest) * 1.6 + 3.0;
+  };
+  long long best = std::max<long long>(total, 1);
+  double least = time(best);
+  for (long long s = 1; s < total; s *= 2) {
+    const double x = time(s);
+    if (x < 0.95 * least && units(s) * a.heads < (1LL << 30)) {
+      least = x;
+      best = s;
     }
   }
-  if (r.last)
-    for (int i = 0; i < r.wk; ++i)
-      for (int j = tid; j < r.wv; j += blockDim.x) {
-        float s = S[i * r.wv + j];
-        if (r.back && n > 0) s = fmaf(s, ghi, s * glo);
-        r.last[sbase + i * r.wv + j] = s;
-      }
+  a.split = best < total;
+  a.seg_len = (int)(best * kChunk);
+  a.segs = a.cu ? 1 : (int)std::max<long long>(1, (total + best - 1) / best);
+  a.units = (int)(a.split ? units(best) : a.nseq);
+  if (!a.split) return 0;
+  int64_t bytes = 0;
+  for (int i = 0; i < a.roles; ++i) bytes += (4LL * a.units * a.heads * a.role[i].wk * a.role[i].wv + 15) & ~15LL;
+  (void)t;
+  return bytes;
 }
 
-template <typename T>
-static cudaError_t run_simple(const DecayArgs& a, cudaStream_t st) {
-  size_t smem = 0;
+cudaError_t launch_decay_attention(ElemType t, DecayArgs a, void* work, cudaStream_t st) {
+  plan_decay_attention(t, a);
+  char* p = static_cast<char*>(work);
   for (int i = 0; i < a.roles; ++i) {
-    const size_t b = sizeof(float) * ((size_t)a.role[i].wk * a.role[i].wv + 2 * a.role[i].wk);
-    smem = b > smem ? b : smem;
+    DecayRole& r = a.role[i];
+    r.wide = wide_bits(r, t == kF32 ? 4 : 2);
+    if (a.split) {
+      r.seg = reinterpret_cast<float*>(p);
+      p += (4LL * a.units * a.heads * r.wk * r.wv + 15) & ~15LL;
+    }
   }
-  cudaError_t e = cudaFuncSetAttribute(k_decay_simple<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
-  k_decay_simple<T><<<dim3(a.heads, a.nseq + (a.cu ? 1 : 0), a.roles), 128, smem, st>>>(a);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_decay_attention(ElemType t, const DecayArgs& a, cudaStream_t st) {
   switch (t) {
-    case kF32: return run_simple<float>(a, st);
-    case kBF16: return run_simple<__nv_bfloat16>(a, st);
-    default: return run_simple<__half>(a, st);
+    case kF32: return launch_decay_chunks_f32(a, st);
+    case kBF16: return launch_decay_chunks_bf16(a, st);
+    default: return launch_decay_chunks_f16(a, st);
   }
 }
 

@@ -30,6 +30,7 @@ struct DecayRole {
   long long first_sk, first_sv;  //   (seq*heads + head)*wk*wv + k*first_sk + v*first_sv
   float* last;                 // final state (wk x wv, row-major) or null
   float* seg;                  // states of the segments, (unit, head, wk, wv)
+  int wide;                    // bits: q, k, v rows are multiples of 16 bytes from aligned addresses; o of element pairs
 };
 
 constexpr int kMaxRoles = 3;
@@ -48,13 +49,22 @@ struct DecayArgs {
   // work units: a unit is one segment (seg_len tokens, a multiple of the
   // chunk) of one sequence; dense: seq = unit / segs.  packed: found from cu;
   // `units` bounds their number, and unit index `units` zeroes the rows of o
-  // that belong to no sequence.
+  // that belong to no sequence.  split: sequences may have several segments,
+  // whose states then take a pass of their own.
   int seg_len;
   int segs;
   int units;
+  int split;
 };
 
-cudaError_t launch_decay_attention(ElemType t, const DecayArgs& a, cudaStream_t st);
+// Cuts the sequences into segments (seg_len, segs, units, split) by the sizes alone, and says how many
+// bytes the segments' states take (roles that are there: the widths in `a`).
+int64_t plan_decay_attention(ElemType t, DecayArgs& a);
+// `work` holds the bytes that plan_decay_attention said.
+cudaError_t launch_decay_attention(ElemType t, DecayArgs a, void* work, cudaStream_t st);
+cudaError_t launch_decay_chunks_f32(const DecayArgs& a, cudaStream_t st);
+cudaError_t launch_decay_chunks_bf16(const DecayArgs& a, cudaStream_t st);
+cudaError_t launch_decay_chunks_f16(const DecayArgs& a, cudaStream_t st);
 
 // out[row][hk][w] = sum over g < group of in[row][hk*group + g][w], float32 in, element type out.
 cudaError_t launch_sum_heads(ElemType t, const float* in, void* out, long long rows, int kv_heads, int group, int width,

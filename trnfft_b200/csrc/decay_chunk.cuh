@@ -1,0 +1,641 @@
+// Decayed linear attention in chunks of 64 tokens, on the warp-level tensor
+// core instructions: every type, head widths up to 128 and any decay.
+//
+// With C the state carried into a chunk of n tokens, row i of it:
+//   P_ij = a g^{i-j} (q_i . k_j)  for j <= i, else 0
+//   o    = P v + r g^{i+1-back} (q C)
+//   C'   = g^n C + sum_j (c g^{n-1-j+back} k_j) v_j^T
+// One block of 8 warps walks the chunks of one (segment, head, role).  A warp
+// owns 16 rows of P, which stay in its registers as the A operand of P v, and
+// a block of C, which stays in its registers in float32; C goes to shared
+// memory once per chunk as the B operand of q C.
+//
+// Precision.  float32 operands are split in two TF32 parts each and multiplied
+// as hi hi + hi lo + lo hi (2^-22).  16-bit operands are exact in TF32 (and
+// q . k runs on their own type); P and C are rounded to TF32 where they are
+// multiplied (2^-12, a sixteenth of a float16 step or less), and the scaled k,
+// which the state accumulates, is split in two parts.  The tensor core
+// truncates as it accumulates, so C never is an accumulator over chunks: a
+// chunk's sum starts from 0 and is added to the scaled C in round-to-nearest,
+// with g^n as the sum of two float32.
+#pragma once
+
+#include "decay_attn.h"
+#include "elem.cuh"
+#include "tma.cuh"
+
+namespace tfb {
+namespace chunk {
+
+constexpr int kC = 64;
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ uint32_t tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+__device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A TF32 operand in PARTS parts: hi, and what is left of it.
+template <int N, int PARTS>
+struct Frag {
+  uint32_t p[PARTS][N];
+  __device__ __forceinline__ void set(int i, float x) {
+    p[0][i] = tf32(x);
+    if constexpr (PARTS > 1) p[1][i] = tf32(x - __uint_as_float(p[0][i]));
+  }
+  // a value that TF32 holds exactly
+  __device__ __forceinline__ void exact(int i, float x) {
+    static_assert(PARTS == 1, "one part");
+    p[0][i] = __float_as_uint(x);
+  }
+};
+template <int PA, int PB>
+__device__ __forceinline__ void mma_parts(float (&d)[4], const Frag<4, PA>& a, const Frag<2, PB>& b) {
+  if constexpr (PB > 1) mma_tf32(d, a.p[0], b.p[1][0], b.p[1][1]);
+  if constexpr (PA > 1) mma_tf32(d, a.p[1], b.p[0][0], b.p[0][1]);
+  mma_tf32(d, a.p[0], b.p[0][0], b.p[0][1]);
+}
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <typename T>
+constexpr int pitch(int d) { return d + 16 / (int)sizeof(T); }  // 4 words past a multiple of 32: conflict-free columns
+
+template <typename T, int DK, int DV>
+struct Shape {
+  static constexpr bool kSplit = sizeof(T) == 4;          // float32: every operand in two parts
+  static constexpr int kPK = pitch<T>(DK), kPV = pitch<T>(DV), kPS = DV + 4;
+  static constexpr int kTile = kC * (2 * kPK + kPV) * sizeof(T);  // q, k, v of one chunk
+  static constexpr int kState = DK * kPS * 4;
+  static constexpr int kTable = 2 * (kC + 1) * 4 + 24;
+  static constexpr int kStages = 2 * kTile + kState + kTable <= 113 * 1024 || sizeof(T) == 2 ? 2 : 1;
+  static constexpr int kSmem = kStages * kTile + kState + kTable;
+  static constexpr int kBlocks = kSmem <= 113 * 1024 && DK * DV <= 64 * 64 ? 2 : 1;  // per SM
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  // state: warps tile DK in blocks of 16 rows, the rest of them the columns
+  static constexpr int kSRows = DK / 16 < 8 ? DK / 16 : 8, kSCols = 8 / kSRows;
+  static constexpr int kSTiles = DV / 8 / kSCols;          // 8-column tiles of a warp
+  static_assert(DK / 16 <= 8 && kSTiles >= 1, "state layout");
+  // output: 4 blocks of 16 rows, two halves of the columns
+  static constexpr int kOTiles = DV / 16;
+};
+
+// The rows of one chunk of one operand into shared memory, zeros behind its width and length.
+template <typename T, int D, int P>
+__device__ __forceinline__ void load_rows(T* dst, const T* src, long long row_stride, int rows, int width, bool back,
+                                          bool wide) {
+  constexpr int V = 16 / sizeof(T), PER = D / V;
+  if (wide) {
+    for (int i = threadIdx.x; i < kC * PER; i += kThreads) {
+      const int r = i / PER, c = i % PER * V;
+      const bool in = r < rows && c < width;
+      const T* p = src + (in ? (long long)(back ? -r : r) * row_stride + c : 0);
+      cp_async16(dst + r * P + c, p, in ? 16 : 0);
+    }
+  } else {
+    for (int i = threadIdx.x; i < kC * D; i += kThreads) {
+      const int r = i / D, c = i % D;
+      dst[r * P + c] = r < rows && c < width ? src[(long long)(back ? -r : r) * row_stride + c] : from_f32<T>(0.f);
+    }
+  }
+}
+
+__device__ __forceinline__ long long cu_value(const DecayArgs& a, int i) {
+  const long long x = a.cu64 ? static_cast<const long long*>(a.cu)[i] : (long long)static_cast<const int*>(a.cu)[i];
+  return x < 0 ? 0 : (x > a.tokens ? a.tokens : x);  // no value of cu leads outside the tensors
+}
+
+// The segment of a unit: its sequence, first token and length, whether it is the sequence's last,
+// and how long the sequence is.  seq < 0: none.
+struct Segment {
+  long long first, len, start, total;  // of the segment; of its sequence
+  int seq;
+};
+
+// Called by warp 0.
+__device__ __forceinline__ Segment find_segment(const DecayArgs& a, int unit) {
+  Segment s;
+  s.seq = -1;
+  s.first = s.len = s.start = s.total = 0;
+  if (!a.cu) {
+    s.seq = unit / a.segs;
+    s.total = a.tokens;
+    s.first = (long long)(unit % a.segs) * a.seg_len;
+    s.len = min((long long)a.seg_len, a.tokens - s.first);
+    return s;
+  }
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int i0 = 0; i0 < a.nseq; i0 += 32) {
+    const int i = i0 + lane;
+    long long lo = 0, n = 0;
+    int count = 0;
+    if (i < a.nseq) {
+      lo = cu_value(a, i);
+      n = cu_value(a, i + 1) - lo;
+      if (n < 0) n = 0;
+      count = max(1, (int)((n + a.seg_len - 1) / a.seg_len));
+    }
+    int upto = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const bool here = i < a.nseq && unit >= before + upto - count && unit < before + upto;
+    const unsigned who = __ballot_sync(~0u, here);
+    if (who) {
+      const int l = __ffs(who) - 1;
+      lo = __shfl_sync(~0u, lo, l);
+      n = __shfl_sync(~0u, n, l);
+      const int k = unit - before - __shfl_sync(~0u, upto - count, l);
+      s.seq = i0 + l;
+      s.start = lo;
+      s.total = n;
+      s.first = (long long)k * a.seg_len;
+      s.len = min((long long)a.seg_len, n - s.first);
+      return s;
+    }
+    before += __shfl_sync(~0u, upto, 31);
+  }
+  return s;
+}
+
+// What a launch does: whole sequences, the segments' own final states (from 0), or the segments'
+// outputs from the states carried into them.
+enum Pass { kWhole, kLocal, kCarried };
+
+template <typename T, int DK, int DV>
+__global__ void __launch_bounds__(kThreads, (Shape<T, DK, DV>::kBlocks))
+    k_decay_chunk(const __grid_constant__ DecayArgs a, int pass, int only) {
+  using S = Shape<T, DK, DV>;
+  constexpr int PK = S::kPK, PV = S::kPV, PS = S::kPS, STAGES = S::kStages;
+  extern __shared__ __align__(128) unsigned char sm[];
+  float* state = reinterpret_cast<float*>(sm + STAGES * S::kTile);
+  float* dec = state + DK * PS;      // g^n, n <= 64, and what float32 loses of it
+  float* dec_lo = dec + kC + 1;
+  __shared__ Segment seg_shared;
+
+  const DecayRole& R = a.role[only >= 0 ? only : blockIdx.z];
+  const int h = blockIdx.x % a.heads, unit = blockIdx.x / a.heads;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+
+  if (a.cu && unit == a.units) {  // the rows of no sequence
+    if (!R.o || pass == kLocal) return;
+    const long long lo = cu_value(a, 0), hi = max(lo, cu_value(a, a.nseq));
+    for (long long r = warp; r < lo + (a.tokens - hi); r += 8) {
+      const long long at = (long long)h * R.os[2] + (r < lo ? r : hi + r - lo) * R.os[1];
+      for (int c = lane; c < R.wv; c += 32) {
+        if (R.o_f32)
+          static_cast<float*>(R.o)[at + c] = 0.f;
+        else
+          static_cast<T*>(R.o)[at + c] = from_f32<T>(0.f);
+      }
+    }
+    return;
+  }
+  if (warp == 0) {
+    const Segment s = find_segment(a, unit);
+    if (lane == 0) seg_shared = s;
+  }
+  {
+    const double ld = a.log_decay[h];
+    for (int n = threadIdx.x; n <= kC; n += kThreads) {
+      const double x = n ? exp(ld * n) : 1.0;
+      dec[n] = (float)x;
+      dec_lo[n] = x - (double)(float)x == x - (double)(float)x ? (float)(x - (double)(float)x) : 0.f;
+    }
+  }
+  __syncthreads();
+  const Segment seg = seg_shared;
+  if (seg.seq < 0) return;
+  const int back = R.back, len = (int)seg.len;
+  const bool want_o = R.o && pass != kLocal;
+  // row i of the segment is token row0 + i, or row0 - i from the sequence's end
+  const long long row0 = seg.start + (back ? seg.total - 1 - seg.first : seg.first);
+  const long long batch = a.cu ? 0 : seg.seq;
+  const T* q = static_cast<const T*>(R.q) + batch * R.qs[0] + (long long)(h / R.qdiv) * R.qs[2] + row0 * R.qs[1];
+  const T* k = static_cast<const T*>(R.k) + batch * R.ks[0] + (long long)(h / R.kdiv) * R.ks[2] + row0 * R.ks[1];
+  const T* v = static_cast<const T*>(R.v) + batch * R.vs[0] + (long long)(h / R.vdiv) * R.vs[2] + row0 * R.vs[1];
+  const long long obase = batch * R.os[0] + (long long)h * R.os[2] + row0 * R.os[1];
+  const long long sbase = ((long long)seg.seq * a.heads + h) * R.wk * R.wv;
+  float* seg_state = R.seg ? R.seg + ((long long)unit * a.heads + h) * R.wk * R.wv : nullptr;
+  // a kLocal pass of a sequence's last segment serves its final state alone
+  if (pass == kLocal && !R.last && seg.first + seg.len >= seg.total) return;
+
+  auto load = [&](int c, int stage) {
+    T* dst = reinterpret_cast<T*>(sm + stage * S::kTile);
+    const int rows = min(kC, len - c * kC);
+    const long long skip = (long long)(back ? -c : c) * kC;
+    if (want_o) load_rows<T, DK, PK>(dst, q + skip * R.qs[1], R.qs[1], rows, R.wk, back, R.wide & 1);
+    load_rows<T, DK, PK>(dst + kC * PK, k + skip * R.ks[1], R.ks[1], rows, R.wk, back, R.wide & 2);
+    load_rows<T, DV, PV>(dst + 2 * kC * PK, v + skip * R.vs[1], R.vs[1], rows, R.wv, back, R.wide & 4);
+    cp_commit();
+  };
+  const int chunks = (len + kC - 1) / kC;
+  if (chunks > 0) load(0, 0);
+
+  // the state: rows sr + g (+ 8), columns sc + 8 j + 2 t (+ 1)
+  const int sr = warp % S::kSRows * 16, sc = warp / S::kSRows * (S::kSTiles * 8);
+  float st[S::kSTiles][4];
+  {
+    const float* from = pass == kCarried ? seg_state : (pass == kWhole ? R.first : nullptr);
+    const long long sk = pass == kCarried ? R.wv : R.first_sk, sv = pass == kCarried ? 1 : R.first_sv;
+    const long long base = pass == kCarried ? 0 : sbase;
+#pragma unroll
+    for (int j = 0; j < S::kSTiles; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = sr + g + (e >> 1) * 8, col = sc + j * 8 + 2 * t + (e & 1);
+        st[j][e] = from && row < R.wk && col < R.wv ? from[base + row * sk + col * sv] : 0.f;
+      }
+  }
+  auto put_state = [&] {
+#pragma unroll
+    for (int j = 0; j < S::kSTiles; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        float2 x = make_float2(st[j][e], st[j][e + 1]);
+        if (!S::kSplit) x = make_float2(__uint_as_float(tf32(x.x)), __uint_as_float(tf32(x.y)));
+        *reinterpret_cast<float2*>(state + (sr + g + (e >> 1) * 8) * PS + sc + j * 8 + 2 * t) = x;
+      }
+  };
+  if (want_o) put_state();
+
+  // rows of P and o: two of the warps that share a scheduler have 5 blocks of 16 keys together
+  const int mi = warp < 4 ? warp : 7 - warp, oc = warp / 4 * (DV / 2);
+  constexpr int PARTS = S::kSplit ? 2 : 1;
+
+  for (int c = 0; c < chunks; ++c) {
+    const int stage = STAGES == 2 ? c & 1 : 0, rows = min(kC, len - c * kC);
+    if (STAGES == 2 && c + 1 < chunks) {
+      load(c + 1, stage ^ 1);
+      cp_wait<1>();
+    } else {
+      cp_wait<0>();
+    }
+    __syncthreads();
+    const T* sq = reinterpret_cast<const T*>(sm + stage * S::kTile);
+    const T* sk = sq + kC * PK;
+    const T* sv = sk + kC * PK;
+    if (want_o && mi * 16 < rows) {
+      const T* qrow = sq + (mi * 16 + g) * PK;
+      float acc[S::kOTiles][4];
+#pragma unroll
+      for (int j = 0; j < S::kOTiles; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+      // q C, then its rows times r g^(i+1-back)
+#pragma unroll 4
+      for (int kk = 0; kk < DK / 8; ++kk) {
+        Frag<4, PARTS> fa;
+        const T* p = qrow + kk * 8 + 2 * t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = to_f32(p[(e & 1) * 8 * PK + (e >> 1)]);
+          if constexpr (S::kSplit) fa.set(e, x);
+          else fa.exact(e, x);
+        }
+        const float* sp = state + (kk * 8 + 2 * t) * PS + oc + g;
+#pragma unroll
+        for (int j = 0; j < S::kOTiles; ++j) {
+          Frag<2, PARTS> fb;
+          if constexpr (S::kSplit) {
+            fb.set(0, sp[j * 8]);
+            fb.set(1, sp[PS + j * 8]);
+          } else {
+            fb.exact(0, sp[j * 8]);
+            fb.exact(1, sp[PS + j * 8]);
+          }
+          mma_parts(acc[j], fa, fb);
+        }
+      }
+      const int i0 = mi * 16 + g;
+      const float f0 = R.r * dec[i0 + 1 - back], f1 = R.r * dec[i0 + 9 - back];
+#pragma unroll
+      for (int j = 0; j < S::kOTiles; ++j) {
+        acc[j][0] *= f0;
+        acc[j][1] *= f0;
+        acc[j][2] *= f1;
+        acc[j][3] *= f1;
+      }
+      // P, 16 rows by 8 keys at a time, straight into P v
+      for (int n = 0; n < 2 * mi + 2; ++n) {
+        float p[4] = {0.f, 0.f, 0.f, 0.f};
+        const T* krow = sk + (n * 8 + g) * PK;
+        if constexpr (S::kSplit) {
+#pragma unroll 4
+          for (int kk = 0; kk < DK / 8; ++kk) {
+            Frag<4, 2> fa;
+            Frag<2, 2> fb;
+            const int at = kk * 8 + 2 * t;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) fa.set(e, to_f32(qrow[at + (e & 1) * 8 * PK + (e >> 1)]));
+            fb.set(0, to_f32(krow[at]));
+            fb.set(1, to_f32(krow[at + 1]));
+            mma_parts(p, fa, fb);
+          }
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < DK / 16; ++kk) {
+            const T* x = qrow + kk * 16 + 2 * t;
+            const uint32_t fa[4] = {*reinterpret_cast<const uint32_t*>(x), *reinterpret_cast<const uint32_t*>(x + 8 * PK),
+                                    *reinterpret_cast<const uint32_t*>(x + 8),
+                                    *reinterpret_cast<const uint32_t*>(x + 8 * PK + 8)};
+            const T* y = krow + kk * 16 + 2 * t;
+            mma_16<T>(p, fa, *reinterpret_cast<const uint32_t*>(y), *reinterpret_cast<const uint32_t*>(y + 8));
+          }
+        }
+        Frag<4, PARTS> fp;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = mi * 16 + g + (e >> 1) * 8 - (n * 8 + 2 * t + (e & 1));
+          // C layout (row, 2t + e&1) to A layout (row, slot t + 4 (e&1)): key 2t + s sits in slot t + 4 s
+          fp.set((e >> 1) + (e & 1) * 2, d >= 0 ? p[e] * (R.a * dec[max(d, 0)]) : 0.f);
+        }
+        const T* vp = sv + (n * 8 + 2 * t) * PV + oc + g;
+#pragma unroll
+        for (int j = 0; j < S::kOTiles; ++j) {
+          Frag<2, PARTS> fb;
+          if constexpr (S::kSplit) {
+            fb.set(0, to_f32(vp[j * 8]));
+            fb.set(1, to_f32(vp[PV + j * 8]));
+          } else {
+            fb.exact(0, to_f32(vp[j * 8]));
+            fb.exact(1, to_f32(vp[PV + j * 8]));
+          }
+          mma_parts(acc[j], fp, fb);
+        }
+      }
+      // Keys behind a row have weight 0 in P, but 0 times an infinite or NaN value is NaN: where a
+      // result is not finite, its rows are taken again from the keys before them alone.
+      float bad = 0.f;
+#pragma unroll
+      for (int j = 0; j < S::kOTiles; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad = fmaf(acc[j][e], 0.f, bad);
+      if (__any_sync(~0u, bad != 0.f)) {
+        for (int r = 0; r < 16 && mi * 16 + r < rows; ++r) {
+          const int i = mi * 16 + r;
+          const T* qr = sq + i * PK;
+          for (int c0 = oc; c0 < min(oc + DV / 2, R.wv); c0 += 32) {
+            const int col = c0 + lane;
+            const bool in = col < min(oc + DV / 2, R.wv);
+            float x = 0.f;
+            for (int d = 0; d < R.wk; ++d) x = fmaf(to_f32(qr[d]), in ? state[d * PS + col] : 0.f, x);
+            x *= R.r * dec[i + 1 - back];
+            for (int j = 0; j <= i; ++j) {
+              float w = 0.f;
+              for (int d = lane; d < R.wk; d += 32) w = fmaf(to_f32(qr[d]), to_f32(sk[j * PK + d]), w);
+#pragma unroll
+              for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(~0u, w, o);
+              x = fmaf(w * (R.a * dec[i - j]), in ? to_f32(sv[j * PV + col]) : 0.f, x);
+            }
+            const long long at = obase + (long long)(back ? -(c * kC + i) : c * kC + i) * R.os[1] + col;
+            if (in) {
+              if (R.o_f32) static_cast<float*>(R.o)[at] = x;
+              else static_cast<T*>(R.o)[at] = from_f32<T>(x);
+            }
+          }
+        }
+      } else
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        const int i = i0 + (e >> 1) * 8;
+        if (i >= rows) continue;
+        const long long at = obase + (long long)(back ? -(c * kC + i) : c * kC + i) * R.os[1] + oc + 2 * t;
+        const int w = R.wv - oc - 2 * t;  // columns from here on
+#pragma unroll
+        for (int j = 0; j < S::kOTiles; ++j) {
+          const float x = acc[j][e], y = acc[j][e + 1];
+          if (R.o_f32) {
+            float* o = static_cast<float*>(R.o) + at + j * 8;
+            if (R.wide & 8) {
+              if (j * 8 + 1 < w) *reinterpret_cast<float2*>(o) = make_float2(x, y);
+            } else {
+              if (j * 8 < w) o[0] = x;
+              if (j * 8 + 1 < w) o[1] = y;
+            }
+          } else {
+            T* o = static_cast<T*>(R.o) + at + j * 8;
+            if (R.wide & 8) {
+              if (j * 8 + 1 < w) {
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(o) = make_float2(x, y);
+                else from_f32_pair(x, y, o);
+              }
+            } else {
+              if (j * 8 < w) o[0] = from_f32<T>(x);
+              if (j * 8 + 1 < w) o[1] = from_f32<T>(y);
+            }
+          }
+        }
+      }
+    }
+    // C' = g^n C + (scaled k)^T v
+    {
+      float d[S::kSTiles][4];
+#pragma unroll
+      for (int j = 0; j < S::kSTiles; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[j][e] = 0.f;
+      const int blocks = (rows + 7) / 8;
+#pragma unroll 2
+      for (int kk = 0; kk < blocks; ++kk) {
+        const int j0 = kk * 8 + 2 * t;
+        const float w0 = R.c * dec[max(rows - 1 - j0 + back, 0)], w1 = R.c * dec[max(rows - 2 - j0 + back, 0)];
+        Frag<4, 2> fa;
+        const T* p = sk + j0 * PK + sr + g;
+        fa.set(0, to_f32(p[0]) * w0);
+        fa.set(1, to_f32(p[8]) * w0);
+        fa.set(2, to_f32(p[PK]) * w1);
+        fa.set(3, to_f32(p[PK + 8]) * w1);
+        const T* vp = sv + j0 * PV + sc + g;
+#pragma unroll
+        for (int j = 0; j < S::kSTiles; ++j) {
+          Frag<2, PARTS> fb;
+          if constexpr (S::kSplit) {
+            fb.set(0, to_f32(vp[j * 8]));
+            fb.set(1, to_f32(vp[PV + j * 8]));
+          } else {
+            fb.exact(0, to_f32(vp[j * 8]));
+            fb.exact(1, to_f32(vp[PV + j * 8]));
+          }
+          mma_parts(d[j], fa, fb);
+        }
+      }
+      const float hi = dec[rows], lo = dec_lo[rows];
+#pragma unroll
+      for (int j = 0; j < S::kSTiles; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[j][e] = fmaf(st[j][e], hi, fmaf(st[j][e], lo, d[j][e]));
+    }
+    if (c + 1 < chunks) {
+      __syncthreads();  // all have read the stage and the state
+      if (want_o) put_state();
+      if (STAGES == 1) load(c + 1, 0);
+    }
+  }
+  float* to = pass == kLocal ? seg_state : (pass == kWhole && R.last ? R.last + sbase : nullptr);
+  if (to) {
+#pragma unroll
+    for (int j = 0; j < S::kSTiles; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = sr + g + (e >> 1) * 8, col = sc + j * 8 + 2 * t + (e & 1);
+        if (row < R.wk && col < R.wv) to[row * R.wv + col] = st[j][e];
+      }
+  }
+}
+
+// The states carried into the segments of one (sequence, head, role), in place of the segments' own
+// final states, and the sequence's final state.
+template <typename T>
+__global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant__ DecayArgs a) {
+  const DecayRole& R = a.role[blockIdx.z];
+  const int h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
+  __shared__ int first_unit;
+  __shared__ long long shared_total;
+  if (threadIdx.x < 32) {
+    long long n = a.tokens;
+    int before = seq * a.segs;
+    if (a.cu) {
+      before = 0;
+      for (int i = threadIdx.x; i < seq; i += 32) {
+        const long long m = cu_value(a, i + 1) - cu_value(a, i);
+        before += max(1, (int)(((m < 0 ? 0 : m) + a.seg_len - 1) / a.seg_len));
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
+      n = cu_value(a, seq + 1) - cu_value(a, seq);
+      if (n < 0) n = 0;
+    }
+    if (threadIdx.x == 0) {
+      first_unit = before;
+      shared_total = n;
+    }
+  }
+  __syncthreads();
+  const long long total = shared_total, size = (long long)R.wk * R.wv;
+  const int e = blockIdx.y * 256 + threadIdx.x;
+  const int segs = max(1, (int)((total + a.seg_len - 1) / a.seg_len));
+  // (units: what the work area holds; only lengths that are not ascending lead past it)
+  if (e >= size || first_unit + segs > a.units) return;
+  const double ld = a.log_decay[h];
+  const double gd = exp(ld * a.seg_len);
+  const float hi = (float)gd, lo = (float)(gd - (double)hi);
+  float s = 0.f;
+  const long long sbase = ((long long)seq * a.heads + h) * size;
+  if (R.first) s = R.first[sbase + e / R.wv * R.first_sk + e % R.wv * R.first_sv];
+  float* p = R.seg + ((long long)first_unit * a.heads + h) * size + e;
+  const long long step = a.heads * size;
+  int i = 0;
+  for (; i + 4 < segs; i += 4, p += 4 * step) {
+    float x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = p[u * step];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      p[u * step] = s;
+      s = fmaf(s, hi, fmaf(s, lo, x[u]));
+    }
+  }
+  for (; i < segs; ++i, p += step) {
+    const bool end = i == segs - 1;
+    const float x = end && !R.last ? 0.f : *p;
+    *p = s;
+    if (!end) {
+      s = fmaf(s, hi, fmaf(s, lo, x));
+    } else if (R.last) {
+      const long long n = total - (long long)i * a.seg_len;
+      const double gn = n ? exp(ld * n) : 1.0;
+      const float h2 = (float)gn, l2 = (float)(gn - (double)h2);
+      R.last[sbase + e] = fmaf(s, h2, fmaf(s, l2, x));
+    }
+  }
+}
+
+template <typename T, int DK, int DV>
+static cudaError_t run_widths(const DecayArgs& a, Pass pass, int only, cudaStream_t st) {
+  using S = Shape<T, DK, DV>;
+  cudaError_t e = cudaFuncSetAttribute(k_decay_chunk<T, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (e != cudaSuccess) return e;
+  const unsigned units = (unsigned)a.units + (a.cu && pass != kLocal ? 1 : 0);
+  k_decay_chunk<T, DK, DV><<<dim3(units * a.heads, 1, only >= 0 ? 1 : a.roles), kThreads, S::kSmem, st>>>(a, pass, only);
+  return cudaGetLastError();
+}
+
+inline int padded(int w) { return w <= 32 ? 32 : (w <= 64 ? 64 : 128); }
+
+template <typename T, int DK>
+static cudaError_t run_dv(const DecayArgs& a, int dv, Pass pass, int only, cudaStream_t st) {
+  switch (dv) {
+    case 32: return run_widths<T, DK, 32>(a, pass, only, st);
+    case 64: return run_widths<T, DK, 64>(a, pass, only, st);
+    default: return run_widths<T, DK, 128>(a, pass, only, st);
+  }
+}
+
+// All roles in one launch where their padded widths agree, else one launch each.
+template <typename T>
+cudaError_t run_chunks(const DecayArgs& a, Pass pass, cudaStream_t st) {
+  bool same = true;
+  for (int i = 1; i < a.roles; ++i)
+    same = same && padded(a.role[i].wk) == padded(a.role[0].wk) && padded(a.role[i].wv) == padded(a.role[0].wv);
+  for (int i = 0; i < (same ? 1 : a.roles); ++i) {
+    const int dk = padded(a.role[i].wk), dv = padded(a.role[i].wv), only = same ? -1 : i;
+    cudaError_t e;
+    switch (dk) {
+      case 32: e = run_dv<T, 32>(a, dv, pass, only, st); break;
+      case 64: e = run_dv<T, 64>(a, dv, pass, only, st); break;
+      default: e = run_dv<T, 128>(a, dv, pass, only, st);
+    }
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+template <typename T>
+cudaError_t run_all(const DecayArgs& a, cudaStream_t st) {
+  if (!a.split) return run_chunks<T>(a, kWhole, st);
+  cudaError_t e = run_chunks<T>(a, kLocal, st);
+  if (e != cudaSuccess) return e;
+  int size = 0;
+  for (int i = 0; i < a.roles; ++i) size = max(size, a.role[i].wk * a.role[i].wv);
+  k_decay_scan<T><<<dim3((unsigned)a.nseq * a.heads, (size + 255) / 256, a.roles), 256, 0, st>>>(a);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? run_chunks<T>(a, kCarried, st) : e;
+}
+
+}  // namespace chunk
+}  // namespace tfb
