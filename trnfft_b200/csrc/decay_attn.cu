@@ -39,27 +39,22 @@ int wide_bits(const DecayRole& r, int size) {
 
 // A sequence is walked chunk by chunk, so with few (sequence, head, role) the GPU is filled by cutting
 // sequences into segments, at the cost of a pass that takes the segments' own states (it reads k and v
-// once more and does about 0.6 of a chunk's work) and a scan of these (about 3 chunks' time).  The
-// segment length, in chunks, is the one of least time by that count.
+// once more and does about 0.6 of a chunk's work), of the states' way through memory and each block's
+// start (about 3 chunks' time for each wave of blocks) and of a scan (about 2).  The segment length, in
+// chunks, is the one of least time by that count.
 int64_t plan_decay_attention(ElemType t, DecayArgs& a) {
-  const long long total = ((a.cu ? a.tokens : a.tokens) + kChunk - 1) / kChunk;  // chunks, of one dense or all packed sequences
+  const long long total = (a.tokens + kChunk - 1) / kChunk;  // chunks, of one dense or of all packed sequences
   int wide = 0;
   for (int i = 0; i < a.roles; ++i) wide = max(wide, max(a.role[i].wk, a.role[i].wv));
   const long long slots = (long long)kSms * (wide <= 64 ? 2 : 1), walks = (long long)a.heads * max(a.roles, 1);
   // packed: how the rows fall on the sequences is on the device; take the longest for four times the mean
   const long long longest = a.cu ? (a.nseq ? std::min(total, 4 * total / a.nseq + 1) : 0) : total;
-  auto units = [&](long long s) {
-    return a.cu ? (s >= total ? a.nseq : std::min<long long>(total / s + a.nseq, total + a.nseq)) : a.nseq * ((total + s - 1) / s);
-  };
-  auto time = [&](long long s) {
-    const double waves = (double)((units(s) * walks + slots - 1) / slots);
-    return s >= total ? std::max((double)longest, waves * total * (a.cu ? 1.0 / std::max(1, a.nseq) : 1.0))
-                      : waves * std::min(s, longest) * 1.6 + 3.0;
-  };
+  auto units = [&](long long s) { return a.cu ? total / s + a.nseq : a.nseq * ((total + s - 1) / s); };
+  auto waves = [&](long long n) { return (double)((n * walks + slots - 1) / slots); };
   long long best = std::max<long long>(total, 1);
-  double least = time(best);
+  double least = std::max((double)longest, waves(a.nseq) * (a.cu ? (double)total / std::max(1, a.nseq) : (double)total));
   for (long long s = 1; s < total; s *= 2) {
-    const double x = time(s);
+    const double x = waves(units(s)) * (std::min(s, longest) * 1.6 + 3.0) + 2.0;
     if (x < 0.95 * least && units(s) * a.heads < (1LL << 30)) {
       least = x;
       best = s;

@@ -57,6 +57,8 @@ struct DecayArgs {
   int split;
 };
 
+constexpr int padded_width(int w) { return w <= 32 ? 32 : (w <= 64 ? 64 : 128); }
+
 // Cuts the sequences into segments (seg_len, segs, units, split) by the sizes alone, and says how many
 // bytes the segments' states take (roles that are there: the widths in `a`).
 int64_t plan_decay_attention(ElemType t, DecayArgs& a);

@@ -197,17 +197,14 @@ __device__ __forceinline__ Segment find_segment(const DecayArgs& a, int unit) {
 enum Pass { kWhole, kLocal, kCarried };
 
 template <typename T, int DK, int DV>
-__global__ void __launch_bounds__(kThreads, (Shape<T, DK, DV>::kBlocks))
-    k_decay_chunk(const __grid_constant__ DecayArgs a, int pass, int only) {
+__device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int pass, unsigned char* sm) {
   using S = Shape<T, DK, DV>;
   constexpr int PK = S::kPK, PV = S::kPV, PS = S::kPS, STAGES = S::kStages;
-  extern __shared__ __align__(128) unsigned char sm[];
   float* state = reinterpret_cast<float*>(sm + STAGES * S::kTile);
   float* dec = state + DK * PS;      // g^n, n <= 64, and what float32 loses of it
   float* dec_lo = dec + kC + 1;
   __shared__ Segment seg_shared;
 
-  const DecayRole& R = a.role[only >= 0 ? only : blockIdx.z];
   const int h = blockIdx.x % a.heads, unit = blockIdx.x / a.heads;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
 
@@ -518,6 +515,19 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, DK, DV>::kBlocks))
   }
 }
 
+// Widths padded to D0 <= D1: the roles of one call have both orders (the gradients of q and k have
+// keys of the values' width), and run in one launch.
+template <typename T, int D0, int D1>
+__global__ void __launch_bounds__(kThreads, (Shape<T, D0, D1>::kBlocks))
+    k_decay_chunk(const __grid_constant__ DecayArgs a, int pass) {
+  extern __shared__ __align__(128) unsigned char sm[];
+  const DecayRole& R = a.role[blockIdx.z];
+  if (D0 == D1 || R.wk <= D0)
+    walk<T, D0, D1>(a, R, pass, sm);
+  else if constexpr (D0 != D1)
+    walk<T, D1, D0>(a, R, pass, sm);
+}
+
 // The states carried into the segments of one (sequence, head, role), in place of the segments' own
 // final states, and the sequence's final state.
 template <typename T>
@@ -585,44 +595,23 @@ __global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant__ Deca
   }
 }
 
-template <typename T, int DK, int DV>
-static cudaError_t run_widths(const DecayArgs& a, Pass pass, int only, cudaStream_t st) {
-  using S = Shape<T, DK, DV>;
-  cudaError_t e = cudaFuncSetAttribute(k_decay_chunk<T, DK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+template <typename T, int D0, int D1>
+static cudaError_t run_widths(const DecayArgs& a, Pass pass, cudaStream_t st) {
+  constexpr int smem = Shape<T, D0, D1>::kSmem > Shape<T, D1, D0>::kSmem ? Shape<T, D0, D1>::kSmem : Shape<T, D1, D0>::kSmem;
+  cudaError_t e = cudaFuncSetAttribute(k_decay_chunk<T, D0, D1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const unsigned units = (unsigned)a.units + (a.cu && pass != kLocal ? 1 : 0);
-  k_decay_chunk<T, DK, DV><<<dim3(units * a.heads, 1, only >= 0 ? 1 : a.roles), kThreads, S::kSmem, st>>>(a, pass, only);
+  k_decay_chunk<T, D0, D1><<<dim3(units * a.heads, 1, a.roles), kThreads, smem, st>>>(a, pass);
   return cudaGetLastError();
 }
 
-inline int padded(int w) { return w <= 32 ? 32 : (w <= 64 ? 64 : 128); }
-
-template <typename T, int DK>
-static cudaError_t run_dv(const DecayArgs& a, int dv, Pass pass, int only, cudaStream_t st) {
-  switch (dv) {
-    case 32: return run_widths<T, DK, 32>(a, pass, only, st);
-    case 64: return run_widths<T, DK, 64>(a, pass, only, st);
-    default: return run_widths<T, DK, 128>(a, pass, only, st);
-  }
-}
-
-// All roles in one launch where their padded widths agree, else one launch each.
 template <typename T>
 cudaError_t run_chunks(const DecayArgs& a, Pass pass, cudaStream_t st) {
-  bool same = true;
-  for (int i = 1; i < a.roles; ++i)
-    same = same && padded(a.role[i].wk) == padded(a.role[0].wk) && padded(a.role[i].wv) == padded(a.role[0].wv);
-  for (int i = 0; i < (same ? 1 : a.roles); ++i) {
-    const int dk = padded(a.role[i].wk), dv = padded(a.role[i].wv), only = same ? -1 : i;
-    cudaError_t e;
-    switch (dk) {
-      case 32: e = run_dv<T, 32>(a, dv, pass, only, st); break;
-      case 64: e = run_dv<T, 64>(a, dv, pass, only, st); break;
-      default: e = run_dv<T, 128>(a, dv, pass, only, st);
-    }
-    if (e != cudaSuccess) return e;
-  }
-  return cudaSuccess;
+  const int lo = padded_width(min(a.role[0].wk, a.role[0].wv)), hi = padded_width(max(a.role[0].wk, a.role[0].wv));
+  if (hi == 32) return run_widths<T, 32, 32>(a, pass, st);
+  if (hi == 64) return lo == 32 ? run_widths<T, 32, 64>(a, pass, st) : run_widths<T, 64, 64>(a, pass, st);
+  if (lo == 32) return run_widths<T, 32, 128>(a, pass, st);
+  return lo == 64 ? run_widths<T, 64, 128>(a, pass, st) : run_widths<T, 128, 128>(a, pass, st);
 }
 
 template <typename T>
