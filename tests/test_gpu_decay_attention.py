@@ -253,9 +253,11 @@ def test_layouts_and_alignment(dtype):
     for x in (q, k, v):
         y = torch.empty(x.numel() + 1, dtype=dtype, device="cuda")[1:].view(x.shape)
         shifted.append(y.copy_(x))
-    assert torch.equal(trnfft.decay_attention(*shifted, g), want)
+    exact, _ = decay_ref(q, k, v, g, dk ** -0.5)
+    total, _ = decay_ref(q, k, v, g, dk ** -0.5, absolute=True)
+    check(trnfft.decay_attention(*shifted, g), exact, total, dtype, terms_of(t, dk, dv), "off the 16-byte grid")
     gaps = [torch.nn.functional.pad(x, (1, 2))[..., 1:-2] for x in (q, k, v)]
-    assert torch.equal(trnfft.decay_attention(*gaps, g), want)
+    check(trnfft.decay_attention(*gaps, g), exact, total, dtype, terms_of(t, dk, dv), "rows at odd distances")
     inner = [x.transpose(-1, -2).contiguous().transpose(-1, -2) for x in (q, k, v)]
     assert torch.equal(trnfft.decay_attention(*inner, g), want)
     k1, v1 = k[:, :, :1].expand(-1, -1, hk, -1), v[:, :1].expand(-1, t, -1, -1)

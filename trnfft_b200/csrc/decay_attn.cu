@@ -21,7 +21,8 @@ namespace tfb {
 
 namespace {
 
-constexpr int kChunk = 64;
+// Tokens of a chunk: of the tensor-core kernel for bfloat16 (a multiple of the other kernel's), of the other one.
+constexpr int chunk_of(ElemType t) { return t == kBF16 ? 128 : 64; }
 constexpr int kSms = 148;
 
 // Bits of DecayRole::wide.
@@ -35,6 +36,17 @@ int wide_bits(const DecayRole& r, int size) {
   return (rows(r.q, r.qs, r.wk) ? 1 : 0) | (rows(r.k, r.ks, r.wk) ? 2 : 0) | (rows(r.v, r.vs, r.wv) ? 4 : 0) | (o ? 8 : 0);
 }
 
+int64_t flag_bytes(const DecayArgs& a) { return (4LL * a.roles * a.units * a.heads + 15) & ~15LL; }
+
+// Whether the roles' operands are as the tensor-core kernel loads and stores them: 16 bytes at a time.
+bool tc_ok(const DecayArgs& a) {
+  for (int i = 0; i < a.roles; ++i) {
+    const DecayRole& r = a.role[i];
+    if ((r.wide & 7) != 7 || r.wv % 8 || reinterpret_cast<uintptr_t>(r.o) % 16) return false;
+  }
+  return true;
+}
+
 }  // namespace
 
 // A sequence is walked chunk by chunk, so with few (sequence, head, role) the GPU is filled by cutting
@@ -43,7 +55,8 @@ int wide_bits(const DecayRole& r, int size) {
 // start (about 3 chunks' time for each wave of blocks) and of a scan (about 2).  The segment length, in
 // chunks, is the one of least time by that count.
 int64_t plan_decay_attention(ElemType t, DecayArgs& a) {
-  const long long total = (a.tokens + kChunk - 1) / kChunk;  // chunks, of one dense or of all packed sequences
+  const int chunk = chunk_of(t);
+  const long long total = (a.tokens + chunk - 1) / chunk;  // chunks, of one dense or of all packed sequences
   int wide = 0;
   for (int i = 0; i < a.roles; ++i) wide = max(wide, max(a.role[i].wk, a.role[i].wv));
   const long long slots = (long long)kSms * (wide <= 64 ? 2 : 1), walks = (long long)a.heads * max(a.roles, 1);
@@ -61,13 +74,12 @@ int64_t plan_decay_attention(ElemType t, DecayArgs& a) {
     }
   }
   a.split = best < total;
-  a.seg_len = (int)(best * kChunk);
+  a.seg_len = (int)(best * chunk);
   a.segs = a.cu ? 1 : (int)std::max<long long>(1, (total + best - 1) / best);
   a.units = (int)(a.split ? units(best) : a.nseq);
-  if (!a.split) return 0;
-  int64_t bytes = 0;
+  int64_t bytes = t == kBF16 ? flag_bytes(a) : 0;
+  if (!a.split) return bytes;
   for (int i = 0; i < a.roles; ++i) bytes += (4LL * a.units * a.heads * a.role[i].wk * a.role[i].wv + 15) & ~15LL;
-  (void)t;
   return bytes;
 }
 
@@ -84,7 +96,10 @@ cudaError_t launch_decay_attention(ElemType t, DecayArgs a, void* work, cudaStre
   }
   switch (t) {
     case kF32: return launch_decay_chunks_f32(a, st);
-    case kBF16: return launch_decay_chunks_bf16(a, st);
+    case kBF16:
+      if (!tc_ok(a)) return launch_decay_chunks_bf16(a, st);
+      a.flags = reinterpret_cast<int*>(p);
+      return launch_decay_tc(a, st);
     default: return launch_decay_chunks_f16(a, st);
   }
 }

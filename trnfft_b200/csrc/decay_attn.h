@@ -55,6 +55,7 @@ struct DecayArgs {
   int segs;
   int units;
   int split;
+  int* flags;  // (role, unit, head): blocks that the tensor-core kernel leaves to the other one, or null
 };
 
 constexpr int padded_width(int w) { return w <= 32 ? 32 : (w <= 64 ? 64 : 128); }
@@ -67,6 +68,7 @@ cudaError_t launch_decay_attention(ElemType t, DecayArgs a, void* work, cudaStre
 cudaError_t launch_decay_chunks_f32(const DecayArgs& a, cudaStream_t st);
 cudaError_t launch_decay_chunks_bf16(const DecayArgs& a, cudaStream_t st);
 cudaError_t launch_decay_chunks_f16(const DecayArgs& a, cudaStream_t st);
+cudaError_t launch_decay_tc(const DecayArgs& a, cudaStream_t st);
 
 // out[row][hk][w] = sum over g < group of in[row][hk*group + g][w], float32 in, element type out.
 cudaError_t launch_sum_heads(ElemType t, const float* in, void* out, long long rows, int kv_heads, int group, int width,

@@ -208,6 +208,8 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
   const int h = blockIdx.x % a.heads, unit = blockIdx.x / a.heads;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
 
+  // (with flags: only what an earlier kernel left to this one)
+  if (a.flags && (unit == a.units || !a.flags[((long long)blockIdx.z * a.units + unit) * a.heads + h])) return;
   if (a.cu && unit == a.units) {  // the rows of no sequence
     if (!R.o || pass == kLocal) return;
     const long long lo = cu_value(a, 0), hi = max(lo, cu_value(a, a.nseq));
@@ -530,8 +532,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, D0, D1>::kBlocks))
 
 // The states carried into the segments of one (sequence, head, role), in place of the segments' own
 // final states, and the sequence's final state.
-template <typename T>
-__global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant__ DecayArgs a) {
+static __global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant__ DecayArgs a) {
   const DecayRole& R = a.role[blockIdx.z];
   const int h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
   __shared__ int first_unit;
@@ -614,15 +615,18 @@ cudaError_t run_chunks(const DecayArgs& a, Pass pass, cudaStream_t st) {
   return lo == 64 ? run_widths<T, 64, 128>(a, pass, st) : run_widths<T, 128, 128>(a, pass, st);
 }
 
+inline cudaError_t run_scan(const DecayArgs& a, cudaStream_t st) {
+  int size = 0;
+  for (int i = 0; i < a.roles; ++i) size = max(size, a.role[i].wk * a.role[i].wv);
+  k_decay_scan<<<dim3((unsigned)a.nseq * a.heads, (size + 255) / 256, a.roles), 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t run_all(const DecayArgs& a, cudaStream_t st) {
   if (!a.split) return run_chunks<T>(a, kWhole, st);
   cudaError_t e = run_chunks<T>(a, kLocal, st);
-  if (e != cudaSuccess) return e;
-  int size = 0;
-  for (int i = 0; i < a.roles; ++i) size = max(size, a.role[i].wk * a.role[i].wv);
-  k_decay_scan<T><<<dim3((unsigned)a.nseq * a.heads, (size + 255) / 256, a.roles), 256, 0, st>>>(a);
-  e = cudaGetLastError();
+  if (e == cudaSuccess) e = run_scan(a, st);
   return e == cudaSuccess ? run_chunks<T>(a, kCarried, st) : e;
 }
 
