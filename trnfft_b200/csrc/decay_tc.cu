@@ -17,19 +17,26 @@
 // state, a float32 result, would be off by 2^-9.  C itself stays in float32
 // registers and is scaled by g^n as a sum of two float32.
 //
-// One block per (segment, head, role), 13 warps:
+// One block per (segment, head, role), 12 warps:
 //   0-3   P: read from TMEM, weigh, split, write back as the A operand of P v
 //   4-7   k': in place of k, and its other two parts beside it
-//   0-7   o, half of the columns each; the state, likewise
+//   0-7   o, half of the columns each, through the state's place in shared
+//         memory to whole lines of global memory; the state, likewise
 //   8     one thread issues every product
-//   9-12  loads: cp.async, row by row (any strides, either direction, zeros
-//         behind a sequence's end); q as soon as X is done, k and v after E
+//   9     loads by TMA; q as soon as X is done, k and v after E.  Packed
+//         sequences (a box would reach into a neighbour) and operands that no
+//         tensor map describes are loaded row by row by warps 9-11 (cp.async).
+// Tiles hold tokens in their natural order for either direction; backwards in
+// time the mask and the weights are those of the mirrored row.
 // What bounds it: at 128 x 128 a chunk's products take 4096 cycles of the
-// tensor pipe, its bytes 5700 at 1/148 of the measured bandwidth.
+// tensor pipe, its bytes 5700 at 1/148 of the measured bandwidth, and k and v
+// have one buffer (227 KB are full), so their load is not hidden.
 //
 // A masked P is 0, and 0 times an infinite or NaN value is NaN: blocks whose o
 // is not finite somewhere say so, and the walk of decay_chunk.cuh, which looks
 // at such rows one by one, takes them again.
+#include <cuda.h>
+
 #include "decay_attn.h"
 #include "decay_chunk.cuh"
 
@@ -37,23 +44,29 @@ namespace tfb {
 namespace tc {
 
 constexpr int kC = 128;
-constexpr int kComputeWarps = 8, kMmaWarp = 8;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kLoaders = 96;
+constexpr int kThreads = 384;
 constexpr uint32_t kBlockBytes = kC * 128;  // 64 columns of a tile
 
 template <int D>
 struct Shape {
-  static constexpr int kLoadWarps = D == 128 ? 4 : 2;
-  static constexpr int kThreads = 32 * (kComputeWarps + 1 + kLoadWarps);
   static constexpr int kTile = kC * D * 2, kState = D * D * 2;
   static constexpr int kQ = 0, kK = kTile, kV = 2 * kTile, kMid = 3 * kTile, kLo = 4 * kTile;
   static constexpr int kSHi = 5 * kTile, kSLo = kSHi + kState, kTable = kSLo + kState;
-  static constexpr int kSmem = kTable + 2 * (kC + 1) * 4 + 56 + 10 * 8 + 64 + 48;
+  static constexpr int kSmem = kTable + (int)sizeof(float) * 2 * 132 + 128 + 10 * 8 + 64;
   // TMEM columns: P (also in two bfloat16 parts), O, X, E.  With D = 64, E shares X's, so that two
   // blocks fit on an SM; X is then read before E is issued.
   static constexpr int kP = 0, kO = 128, kX = 128 + D, kE = D == 64 ? kX : kX + D;
   static constexpr int kColumns = D == 64 ? 256 : 512;
   static constexpr bool kShared = D == 64;
   static_assert(kSmem <= 227 * 1024, "shared memory");
+  static_assert(8 * 32 * D <= 2 * kState, "o is staged in the state's place");
+};
+
+// Tensor maps of the roles' q, k and v: (width, tokens, heads, batch), boxes of 64 columns by 128 tokens.
+struct Maps {
+  CUtensorMap m[kMaxRoles][3];
+  int used;
 };
 
 enum Bar { kFull, kQK, kQS, kPV, kKV, kPDone, kKDone, kSReady, kXRead, kBars };
@@ -144,17 +157,32 @@ __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
 __device__ __forceinline__ float low_f32(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high_f32(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int token, int head, int batch,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          dst),
+      "l"(map), "r"(x), "r"(token), "r"(head), "r"(batch), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map, int x, int token, int head, int batch) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(x), "r"(token),
+               "r"(head), "r"(batch)
+               : "memory");
+}
+
 template <int D>
-__global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? 2 : 1)
-    k_decay_tc(const __grid_constant__ DecayArgs a, int pass) {
+__global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
+    k_decay_tc(const __grid_constant__ DecayArgs a, const __grid_constant__ Maps maps, int pass) {
   using S = Shape<D>;
   using chunk::kCarried;
   using chunk::kLocal;
   using chunk::kWhole;
   extern __shared__ __align__(1024) unsigned char sm[];
   float* dec = reinterpret_cast<float*>(sm + S::kTable);
-  float* dec_lo = dec + kC + 1;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + ((S::kTable + 2 * (kC + 1) * 4 + 7) & ~7));
+  float* dec_lo = dec + 132;
+  float* mirror = dec_lo + 132;  // dec[31 - j]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(mirror + 32);
   chunk::Segment* seg_shared = reinterpret_cast<chunk::Segment*>(bars + 10);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seg_shared + 1);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -167,7 +195,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? 2 : 1)
   if (a.cu && unit == a.units) {  // the rows of no sequence
     if (!R.o || pass == kLocal) return;
     const long long lo = chunk::cu_value(a, 0), hi = max(lo, chunk::cu_value(a, a.nseq));
-    for (long long r = warp; r < lo + (a.tokens - hi); r += S::kThreads / 32) {
+    for (long long r = warp; r < lo + (a.tokens - hi); r += kThreads / 32) {
       const long long at = (long long)h * R.os[2] + (r < lo ? r : hi + r - lo) * R.os[1];
       for (int c = lane; c < R.wv; c += 32) {
         if (R.o_f32) static_cast<float*>(R.o)[at + c] = 0.f;
@@ -182,15 +210,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? 2 : 1)
   }
   {
     const double ld = a.log_decay[h];
-    for (int n = threadIdx.x; n <= kC; n += S::kThreads) {
+    for (int n = threadIdx.x; n <= kC; n += kThreads) {
       const double x = n ? exp(ld * n) : 1.0, rest = x - (double)(float)x;
       dec[n] = (float)x;
       dec_lo[n] = rest == rest ? (float)rest : 0.f;
+      if (n < 32) mirror[31 - n] = (float)x;
     }
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const int count = i == kFull ? 32 * S::kLoadWarps
+      const int count = i == kFull ? (maps.used ? 1 : kLoaders)
                                    : (i == kPDone || i == kKDone ? 128 : (i == kSReady || i == kXRead ? 256 : 1));
       mbar_init(&bars[i], count);
     }
@@ -219,57 +248,70 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? 2 : 1)
   fence_after();
   const uint32_t tmem = *tmem_slot, base = smem_u32(sm);
   const bool want_o = R.o && pass != kLocal;
-  const long long row0 = seg.start + (back ? seg.total - 1 - seg.first : seg.first);
   const long long batch = a.cu ? 0 : seg.seq;
   const int chunks = (len + kC - 1) / kC;
+  // token of row 0 of chunk c (backwards it may lie before the sequence), and the rows that belong to it
+  auto first_token = [&](int c) {
+    return seg.start + (back ? seg.total - seg.first - (long long)(c + 1) * kC : seg.first + (long long)c * kC);
+  };
 
   if (warp > kMmaWarp) {
     // ---------------- loads
-    const int t = threadIdx.x - 32 * (kMmaWarp + 1);
-    constexpr int kLoaders = 32 * S::kLoadWarps, kVecs = D / 8;
-    const int sign = back ? -1 : 1;
-    auto rows_in = [&](int tile, const void* p, const long long* stride, int div, int width, int c) {
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p) + batch * stride[0] + (long long)(h / div) * stride[2] +
-                                 (row0 + (long long)sign * c * kC) * stride[1];
-      const int rows = min(kC, len - c * kC);
-      const long long step = sign * stride[1];
-      // a thread keeps its column and walks down the rows
-      const int cc = t % kVecs, r0 = t / kVecs;
-      const bool in = cc * 8 < width;
-      const __nv_bfloat16* from = src + cc * 8;
-      unsigned char* to = sm + tile + cc / 8 * kBlockBytes;
+    if (maps.used) {
+      if (warp == kLoadWarp && lane == 0) {
+        const CUtensorMap *mq = &maps.m[blockIdx.z][0], *mk = &maps.m[blockIdx.z][1], *mv = &maps.m[blockIdx.z][2];
+        const int hq = h / R.qdiv, hk = h / R.kdiv, hv = h / R.vdiv, b = (int)batch;
+        for (int c = 0; c < chunks; ++c) {
+          const int token = (int)first_token(c);
+          if (want_o) {
+            if (c > 0 && !wait(&bars[kQS], (c - 1) & 1, gave_up)) break;
+            mbar_arrive_expect_tx(&bars[kFull], 3 * S::kTile);
+            for (int x = 0; x < D; x += 64) tma_load(base + S::kQ + x / 64 * kBlockBytes, mq, x, token, hq, b, &bars[kFull]);
+          }
+          if (c > 0 && !wait(&bars[kKV], (c - 1) & 1, gave_up)) break;
+          if (!want_o) mbar_arrive_expect_tx(&bars[kFull], 2 * S::kTile);
+          for (int x = 0; x < D; x += 64) tma_load(base + S::kK + x / 64 * kBlockBytes, mk, x, token, hk, b, &bars[kFull]);
+          for (int x = 0; x < D; x += 64) tma_load(base + S::kV + x / 64 * kBlockBytes, mv, x, token, hv, b, &bars[kFull]);
+          if (c + 1 < chunks) {
+            const int next = (int)first_token(c + 1);
+            for (int x = 0; x < D; x += 64) tma_prefetch(mk, x, next, hk, b);
+            for (int x = 0; x < D; x += 64) tma_prefetch(mv, x, next, hv, b);
+          }
+        }
+      }
+    } else {
+      const int t = threadIdx.x - 32 * kLoadWarp;
+      constexpr int kVecs = D / 8;
+      auto rows_in = [&](int tile, const void* p, const long long* stride, int div, int width, int c) {
+        const long long token = first_token(c);
+        const __nv_bfloat16* src =
+            static_cast<const __nv_bfloat16*>(p) + batch * stride[0] + (long long)(h / div) * stride[2];
+        const int rows = min(kC, len - c * kC), lo = back ? kC - rows : 0, hi = back ? kC : rows;
+        // a thread keeps its column and walks down the rows
+        const int cc = t % kVecs;
+        unsigned char* to = sm + tile + cc / 8 * kBlockBytes;
 #pragma unroll 4
-      for (int r = r0; r < kC; r += kLoaders / kVecs) {
-        const bool live = in && r < rows;
-        chunk::cp_async16(to + r * 128 + ((cc % 8) ^ (r & 7)) * 16, live ? from + r * step : src, live ? 16 : 0);
-      }
-    };
-    auto touch = [&](const void* p, const long long* stride, int div, int width, int c) {  // into L2
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p) + batch * stride[0] + (long long)(h / div) * stride[2] +
-                                 (row0 + (long long)sign * c * kC) * stride[1];
-      const int rows = min(kC, len - c * kC);
-      for (int r = t; r < rows; r += kLoaders)
-        for (int x = 0; x < width; x += 64)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(src + (long long)sign * r * stride[1] + x));
-    };
-    for (int c = 0; c < chunks; ++c) {
-      if (want_o) {
-        if (c > 0 && !wait_warp(&bars[kQS], (c - 1) & 1, gave_up)) break;
-        rows_in(S::kQ, R.q, R.qs, R.qdiv, R.wk, c);
-      }
-      if (c > 0 && !wait_warp(&bars[kKV], (c - 1) & 1, gave_up)) break;
-      rows_in(S::kK, R.k, R.ks, R.kdiv, R.wk, c);
-      rows_in(S::kV, R.v, R.vs, R.vdiv, R.wv, c);
-      chunk::cp_commit();
-      if (c + 1 < chunks) {
-        touch(R.k, R.ks, R.kdiv, R.wk, c + 1);
-        touch(R.v, R.vs, R.vdiv, R.wv, c + 1);
+        for (int r = t / kVecs; r < kC; r += kLoaders / kVecs) {
+          const bool live = cc * 8 < width && r >= lo && r < hi;
+          chunk::cp_async16(to + r * 128 + ((cc % 8) ^ (r & 7)) * 16, live ? src + (token + r) * stride[1] + cc * 8 : src,
+                            live ? 16 : 0);
+        }
+      };
+      for (int c = 0; c < chunks; ++c) {
+        if (want_o) {
+          if (c > 0 && !wait_warp(&bars[kQS], (c - 1) & 1, gave_up)) break;
+          rows_in(S::kQ, R.q, R.qs, R.qdiv, R.wk, c);
+        }
+        if (c > 0 && !wait_warp(&bars[kKV], (c - 1) & 1, gave_up)) break;
+        rows_in(S::kK, R.k, R.ks, R.kdiv, R.wk, c);
+        rows_in(S::kV, R.v, R.vs, R.vdiv, R.wv, c);
+        chunk::cp_commit();
+        chunk::cp_wait<0>();
+        fence_proxy_async();
+        arrive(&bars[kFull]);
       }
       chunk::cp_wait<0>();
-      fence_proxy_async();
-      arrive(&bars[kFull]);
     }
-    chunk::cp_wait<0>();
   } else if (warp == kMmaWarp) {
     // ---------------- products
     if (lane == 0) {
@@ -367,26 +409,40 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? 2 : 1)
           fence_after();
 #pragma unroll 1
           for (int p = 0; p < 4; ++p) {
-            uint32_t v[32];
             const uint32_t at = tmem + S::kP + p * 32 + lanes;
-            if (p <= warp) {
+            uint32_t v[32], out[32];
+            if (p == warp) {  // the diagonal: g^d, d tokens from the key to the row
               tmem_ld32(v, at);
               tmem_ld_wait();
-              uint32_t out[32];
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const int d = row - p * 32 - j;
-                const float x = d >= 0 ? __uint_as_float(v[j]) * (R.a * dec[max(d, 0)]) : 0.f;
-                const float y = d >= 1 ? __uint_as_float(v[j + 1]) * (R.a * dec[max(d - 1, 0)]) : 0.f;
-                out[j / 2] = pack_bf16(x, y);
-                out[16 + j / 2] = pack_bf16(x - low_f32(out[j / 2]), y - high_f32(out[j / 2]));
+              for (int j = 0; j < 32; ++j) {
+                const int d = back ? j - lane : lane - j;
+                v[j] = d >= 0 ? __float_as_uint(__uint_as_float(v[j]) * (R.a * dec[d])) : 0;
               }
-              tmem_st32(at, out);
+            } else if ((p < warp) != (back != 0)) {  // g^(from the piece's last key on) g^(to that key)
+              tmem_ld32(v, at);
+              const float f = R.a * dec[back ? p * 32 - row : row - p * 32 - 31];
+              const float4* tab = reinterpret_cast<const float4*>(back ? dec : mirror);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                const float4 w = tab[j / 4];
+                v[j] = __float_as_uint(__uint_as_float(v[j]) * f * w.x);
+                v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) * f * w.y);
+                v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) * f * w.z);
+                v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) * f * w.w);
+              }
             } else {  // keys behind all of this warp's rows
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = 0;
-              tmem_st32(at, v);
             }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float x = __uint_as_float(v[2 * j]), y = __uint_as_float(v[2 * j + 1]);
+              out[j] = pack_bf16(x, y);
+              out[16 + j] = pack_bf16(x - low_f32(out[j]), y - high_f32(out[j]));
+            }
+            tmem_st32(at, out);
           }
           tmem_st_wait();
           fence_before();
@@ -395,10 +451,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? 2 : 1)
       } else {
         if (!wait_warp(want_o ? &bars[kQK] : &bars[kFull], ph, gave_up)) break;
         const int t = threadIdx.x - 128;
-#pragma unroll 2
+#pragma unroll 4
         for (int i = t; i < S::kTile / 16; i += 128) {
-          const int j = i / 8 % kC;
-          const float w = R.c * dec[max(rows - 1 - j + back, 0)];
+          const int j = i / 8 % kC;  // rows that belong to no token are zero
+          const float w = R.c * dec[max(back ? rows - (kC - 1) + j : rows - 1 - j, 0)];
           uint4* at = reinterpret_cast<uint4*>(sm + S::kK) + i;
           const uint4 k = *at;
           const uint32_t in[4] = {k.x, k.y, k.z, k.w};
@@ -439,9 +495,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? 2 : 1)
         }
         if (!wait_warp(&bars[kPV], ph, gave_up)) break;
         fence_after();
-        const float f = R.r * dec[row + 1 - back];
-        const long long at = batch * R.os[0] + (long long)h * R.os[2] +
-                             (row0 + (long long)(back ? -(c * kC + row) : c * kC + row)) * R.os[1] + c0;
+        const float f = R.r * dec[back ? kC - 1 - row : row + 1];
+        const bool mine = back ? row >= kC - rows : row < rows;
+        const long long to = batch * R.os[0] + (long long)h * R.os[2] + first_token(c) * R.os[1] + c0;
+        // o goes through this warp's part of the state's place: X has been taken from it
+        unsigned char* stage = sm + S::kSHi + warp * (32 * D);
+        const int twist = D == 128 ? lane & 7 : lane >> 1 & 3;
         float bad = 0.f;
 #pragma unroll
         for (int j = 0; j < D / 2; j += kW) {
@@ -457,39 +516,52 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? 2 : 1)
             y[e] = fmaf(xe, f, __uint_as_float(o[e]));
             bad = fmaf(y[e], 0.f, bad);
           }
-          if (row < rows) {
-            if (R.o_f32) {
+          if (R.o_f32) {
+            if (mine) {
 #pragma unroll
               for (int e = 0; e < kW; e += 4)
                 if (c0 + j + e < R.wv)
-                  *reinterpret_cast<float4*>(static_cast<float*>(R.o) + at + j + e) =
+                  *reinterpret_cast<float4*>(static_cast<float*>(R.o) + to + row * R.os[1] + j + e) =
                       make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < kW; e += 8)
-                if (c0 + j + e < R.wv)
-                  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(R.o) + at + j + e) =
-                      make_uint4(pack_bf16(y[e], y[e + 1]), pack_bf16(y[e + 2], y[e + 3]), pack_bf16(y[e + 4], y[e + 5]),
-                                 pack_bf16(y[e + 6], y[e + 7]));
             }
+          } else {
+#pragma unroll
+            for (int e = 0; e < kW; e += 8)
+              *reinterpret_cast<uint4*>(stage + lane * D + (((j + e) / 8) ^ twist) * 16) =
+                  make_uint4(pack_bf16(y[e], y[e + 1]), pack_bf16(y[e + 2], y[e + 3]), pack_bf16(y[e + 4], y[e + 5]),
+                             pack_bf16(y[e + 6], y[e + 7]));
           }
         }
-        strange = strange || (row < rows && bad != 0.f);
+        strange = strange || (mine && bad != 0.f);
+        if (!R.o_f32) {
+          __syncwarp();
+          constexpr int kPer = D / 16, kRows = 32 / kPer;  // 16-byte pieces of a row's half; rows of one access
+          const int piece = lane % kPer;
+          __nv_bfloat16* from_row = static_cast<__nv_bfloat16*>(R.o) + to + piece * 8;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int r = i * kRows + lane / kPer, all = warp % 4 * 32 + r;
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + r * D + (piece ^ (D == 128 ? r & 7 : r >> 1 & 3)) * 16);
+            if ((back ? all >= kC - rows : all < rows) && c0 + piece * 8 < R.wv)
+              *reinterpret_cast<uint4*>(from_row + all * R.os[1]) = x;
+          }
+        }
       }
       if (!wait_warp(&bars[kKV], ph, gave_up)) break;
       fence_after();
       const float hi = dec[rows], lo = dec_lo[rows];
       __syncwarp();
 #pragma unroll
-      for (int j = 0; j < D / 2; j += 16) {
-        uint32_t v[16];
-        tmem_ld16(v, tmem + S::kE + c0 + j + lanes);
+      for (int j = 0; j < D / 2; j += 32) {
+        uint32_t v[32];
+        tmem_ld32(v, tmem + S::kE + c0 + j + lanes);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) st[j + e] = fmaf(st[j + e], hi, fmaf(st[j + e], lo, __uint_as_float(v[e])));
+        for (int e = 0; e < 32; ++e) st[j + e] = fmaf(st[j + e], hi, fmaf(st[j + e], lo, __uint_as_float(v[e])));
       }
       if (c + 1 < chunks) {
         if (want_o) {
+          asm volatile("bar.sync 1, 256;" ::: "memory");  // all warps have taken their o from there
           put_state();
         } else {
           fence_before();
@@ -517,13 +589,48 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, D == 64 ? 2 : 1)
   }
 }
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encoder() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return (EncodeTiled) nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// (width, tokens, heads, batch) of one operand; false where no map describes it (rows shared by tokens,
+// heads or sequences, or distances past a map's range).
+static bool operand_map(CUtensorMap* m, const void* p, const long long* stride, int width, long long tokens, int heads,
+                        long long batch) {
+  const long long sizes[3] = {tokens, heads, batch}, steps[3] = {stride[1], stride[2], stride[0]};
+  cuuint64_t dims[4] = {(cuuint64_t)width, 1, 1, 1}, strides[3];
+  for (int i = 0; i < 3; ++i) {
+    dims[i + 1] = (cuuint64_t)sizes[i];
+    const long long bytes = sizes[i] > 1 ? 2 * steps[i] : 2LL * width;
+    if (bytes <= 0 || bytes % 16 || bytes >= (1LL << 40) || sizes[i] < 1) return false;
+    strides[i] = (cuuint64_t)bytes;
+  }
+  const cuuint32_t box[4] = {64, kC, 1, 1}, each[4] = {1, 1, 1, 1};
+  EncodeTiled fn = encoder();
+  return fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, each,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D>
-static cudaError_t run_tc(const DecayArgs& a, chunk::Pass pass, cudaStream_t st) {
+static cudaError_t run_tc(const DecayArgs& a, const Maps& maps, chunk::Pass pass, cudaStream_t st) {
   using S = Shape<D>;
   cudaError_t e = cudaFuncSetAttribute(k_decay_tc<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   if (e != cudaSuccess) return e;
   const unsigned units = (unsigned)a.units + (a.cu && pass != chunk::kLocal ? 1 : 0);
-  k_decay_tc<D><<<dim3(units * a.heads, 1, a.roles), S::kThreads, S::kSmem, st>>>(a, pass);
+  k_decay_tc<D><<<dim3(units * a.heads, 1, a.roles), kThreads, S::kSmem, st>>>(a, maps, pass);
   return cudaGetLastError();
 }
 
@@ -531,17 +638,25 @@ static cudaError_t run_tc(const DecayArgs& a, chunk::Pass pass, cudaStream_t st)
 
 cudaError_t launch_decay_tc(const DecayArgs& a, cudaStream_t st) {
   int wide = 0;
-  for (int i = 0; i < a.roles; ++i) wide = max(wide, max(a.role[i].wk, a.role[i].wv));
+  tc::Maps maps;
+  maps.used = a.cu == nullptr && a.tokens > 0;
+  for (int i = 0; i < a.roles; ++i) {
+    const DecayRole& r = a.role[i];
+    wide = max(wide, max(r.wk, r.wv));
+    maps.used = maps.used && tc::operand_map(&maps.m[i][0], r.q, r.qs, r.wk, a.tokens, a.heads / r.qdiv, a.nseq) &&
+                tc::operand_map(&maps.m[i][1], r.k, r.ks, r.wk, a.tokens, a.heads / r.kdiv, a.nseq) &&
+                tc::operand_map(&maps.m[i][2], r.v, r.vs, r.wv, a.tokens, a.heads / r.vdiv, a.nseq);
+  }
   const chunk::Pass last = a.split ? chunk::kCarried : chunk::kWhole;
   cudaError_t e = cudaSuccess;
-  DecayArgs b = a;
   if (a.split) {
+    DecayArgs b = a;
     b.flags = nullptr;
-    e = wide <= 64 ? tc::run_tc<64>(b, chunk::kLocal, st) : tc::run_tc<128>(b, chunk::kLocal, st);
+    e = wide <= 64 ? tc::run_tc<64>(b, maps, chunk::kLocal, st) : tc::run_tc<128>(b, maps, chunk::kLocal, st);
     if (e == cudaSuccess) e = chunk::run_scan(a, st);
     if (e != cudaSuccess) return e;
   }
-  e = wide <= 64 ? tc::run_tc<64>(a, last, st) : tc::run_tc<128>(a, last, st);
+  e = wide <= 64 ? tc::run_tc<64>(a, maps, last, st) : tc::run_tc<128>(a, maps, last, st);
   if (e != cudaSuccess) return e;
   return chunk::run_chunks<__nv_bfloat16>(a, last, st);  // the blocks that said so, and no others
 }
