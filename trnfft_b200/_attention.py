@@ -43,6 +43,18 @@ def _work(shape, backward, device):
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
+def once(run):
+    """The backward of a Function whose gradients are no graph.  torch's once_differentiable says so to
+    whoever differentiates them, at a tenth of a small step's time, and is needed only where a graph of
+    the gradients is made at all."""
+    careful = torch.autograd.function.once_differentiable(run)
+
+    def backward(ctx, *grads):
+        return (careful if torch.is_grad_enabled() else run)(ctx, *grads)
+
+    return backward
+
+
 def _forward(q, k, v, log_decay, initial, cu, nseq, scale, want_state):
     o = torch.empty(q.shape[:3] + v.shape[3:], dtype=q.dtype, device=q.device)
     last = None
@@ -65,7 +77,7 @@ class _DecayFn(torch.autograd.Function):
         return _forward(q, k, v, log_decay, initial, cu, nseq, scale, want_state)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, do, dlast):
         q, k, v, log_decay, initial, cu = ctx.saved_tensors
         if do is None and dlast is None:
@@ -73,8 +85,9 @@ class _DecayFn(torch.autograd.Function):
         do = torch.zeros(q.shape[:3] + v.shape[3:], dtype=q.dtype, device=q.device) if do is None else _unit_inner(do)
         dlast = None if dlast is None else dlast.contiguous()
         need = ctx.needs_input_grad
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) if n else None
-                      for x, n in zip((q, k, v), need))
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need[0] else None
+        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device) if need[1] else None
+        dv = torch.empty(v.shape, dtype=q.dtype, device=q.device) if need[2] else None
         dinitial = torch.empty(initial.shape, dtype=torch.float32, device=q.device) if need[4] else None
         shape = _shape(q, k, v, do.stride()[:3], cu, ctx.nseq, ctx.scale)
         work = _work(shape, 1, q.device)

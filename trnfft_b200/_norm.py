@@ -2,20 +2,32 @@
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
-from ._attention import DTYPES, _addr
+from ._attention import DTYPES, _addr, once
 from ._device import place_layer
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
-def _work(n, s, c, groups, dtype, backward, device):
+@functools.lru_cache(maxsize=4096)
+def _work_bytes(n, s, c, groups, dtype, backward):
     size = _lib.load().trnfft_group_norm_work_bytes(n, s, c, groups, dtype, backward)
     if size < 0:
         _lib.raise_last("trnfft_group_norm_work_bytes")
+    return size
+
+
+def _work(n, s, c, groups, dtype, backward, device):
+    size = _work_bytes(n, s, c, groups, dtype, backward)
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def _float(p):
+    return p if p is None or p.dtype == torch.float32 else p.float()
 
 
 def _forward(x, groups, weight, bias, eps, act, keep):
@@ -35,8 +47,7 @@ def _forward(x, groups, weight, bias, eps, act, keep):
 class _GroupNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act):
-        w = None if weight is None else weight.float()
-        b = None if bias is None else bias.float()
+        w, b = _float(weight), _float(bias)
         y, stats = _forward(x, groups, w, b, eps, act, True)
         ctx.save_for_backward(x, w, b, stats)
         ctx.groups, ctx.act = groups, act
@@ -44,7 +55,7 @@ class _GroupNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dy):
         x, w, b, stats = ctx.saved_tensors
         groups, need = ctx.groups, ctx.needs_input_grad
@@ -52,14 +63,18 @@ class _GroupNormFn(torch.autograd.Function):
         s = x.numel() // (n * c) if n else 0
         dy = dy.contiguous()
         dx = torch.empty_like(x) if need[0] else None
-        dw, db = (torch.empty(c, dtype=torch.float32, device=x.device) if f else None for f in need[1:3])
+        dw = torch.empty(c, dtype=torch.float32, device=x.device) if need[1] else None
+        db = torch.empty(c, dtype=torch.float32, device=x.device) if need[2] else None
         dt = DTYPES[x.dtype]
         work = _work(n, s, c, groups, dt, 1, x.device)
         at = stats.data_ptr()
         _lib.call("trnfft_group_norm_backward", x.data_ptr(), dy.data_ptr(), _addr(w), _addr(b), at, at + 4 * n * groups,
                   _addr(dx), _addr(dw), _addr(db), n, s, c, groups, ctx.act, dt, _addr(work), x.get_device(),
                   _lib.raw_stream(x.get_device()))
-        dw, db = (g if g is None else g.to(t) for g, t in zip((dw, db), ctx.types))
+        if dw is not None and ctx.types[0] != torch.float32:
+            dw = dw.to(ctx.types[0])
+        if db is not None and ctx.types[1] != torch.float32:
+            db = db.to(ctx.types[1])
         return dx, dw, db, None, None, None
 
 
@@ -94,5 +109,5 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and any(p is not None and p.requires_grad for p in (x, weight, bias)):
         return restore(_GroupNormFn.apply(x, weight, bias, num_groups, eps, act))
-    w, b = (None if p is None else p.float() for p in (weight, bias))
+    w, b = _float(weight), _float(bias)
     return restore(_forward(x, num_groups, w, b, eps, act, False)[0])

@@ -20,6 +20,8 @@
 // with g^n as the sum of two float32.
 #pragma once
 
+#include <type_traits>
+
 #include "decay_attn.h"
 #include "elem.cuh"
 #include "tma.cuh"
@@ -78,6 +80,64 @@ __device__ __forceinline__ void mma_parts(float (&d)[4], const Frag<4, PA>& a, c
   if constexpr (PB > 1) mma_tf32(d, a.p[0], b.p[1][0], b.p[1][1]);
   if constexpr (PA > 1) mma_tf32(d, a.p[1], b.p[0][0], b.p[0][1]);
   mma_tf32(d, a.p[0], b.p[0][0], b.p[0][1]);
+}
+
+// N (1, 2 or 4) blocks of 8 x 8 16-bit elements from shared memory, block i's row r at the address that
+// lane 8 i + r gives: a thread gets elements (row lane/4, columns 2 (lane%4) and the next), or, with
+// kTrans, (rows 2 (lane%4) and the next, column lane/4).
+template <int N, bool kTrans>
+__device__ __forceinline__ void load_blocks(uint32_t (&r)[N], const void* at) {
+  const uint32_t p = smem_u32(at);
+  if constexpr (N == 4 && kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+  else if constexpr (N == 4)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
+  else if constexpr (N == 2)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(p) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x1.trans.shared.b16 {%0}, [%1];" : "=r"(r[0]) : "r"(p) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack(uint32_t x) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
+// d[j] += A B_j for TILES neighbouring blocks of 8 columns, B the 8 rows of v from `rows` on, of which
+// A's slot t holds row 2t and its slot t + 4 row 2t + 1.
+template <typename T, int TILES, int PA, int PITCH>
+__device__ __forceinline__ void mma_rows(float (&d)[TILES][4], const Frag<4, PA>& a, const T* rows) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (sizeof(T) == 4) {
+    const T* p = rows + lane % 4 * 2 * PITCH + lane / 4;
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) {
+      Frag<2, 2> b;
+      b.set(0, p[j * 8]);
+      b.set(1, p[PITCH + j * 8]);
+      mma_parts(d[j], a, b);
+    }
+  } else {
+    constexpr int N = TILES % 4 == 0 ? 4 : TILES % 2 == 0 ? 2 : 1;
+    const T* p = rows + lane % 8 * PITCH + lane / 8 % N * 8;
+#pragma unroll
+    for (int j = 0; j < TILES; j += N) {
+      uint32_t r[N];
+      load_blocks<N, true>(r, p + j * 8);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float2 x = unpack<T>(r[i]);
+        Frag<2, 1> b;
+        b.exact(0, x.x);
+        b.exact(1, x.y);
+        mma_parts(d[j + i], a, b);
+      }
+    }
+  }
 }
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
@@ -309,35 +369,67 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
     const T* sk = sq + kC * PK;
     const T* sv = sk + kC * PK;
     if (want_o && mi * 16 < rows) {
-      const T* qrow = sq + (mi * 16 + g) * PK;
-      float acc[S::kOTiles][4];
+      float acc[S::kOTiles][4], pr[8][4];
 #pragma unroll
       for (int j = 0; j < S::kOTiles; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-      // q C, then its rows times r g^(i+1-back)
-#pragma unroll 4
-      for (int kk = 0; kk < DK / 8; ++kk) {
-        Frag<4, PARTS> fa;
-        const T* p = qrow + kk * 8 + 2 * t;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = to_f32(p[(e & 1) * 8 * PK + (e >> 1)]);
-          if constexpr (S::kSplit) fa.set(e, x);
-          else fa.exact(e, x);
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pr[n][e] = 0.f;
+      // q k^T, for the 8-key blocks n that are not behind all rows, and q C, from the same parts of q
+      if constexpr (S::kSplit) {
+        const T* qrow = sq + (mi * 16 + g) * PK;
+#pragma unroll 2
+        for (int kk = 0; kk < DK / 8; ++kk) {
+          Frag<4, 2> fa;
+          const int at = kk * 8 + 2 * t;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) fa.set(e, to_f32(qrow[at + (e & 1) * 8 * PK + (e >> 1)]));
+          const T* krow = sk + g * PK + at;
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            if (n < 2 * mi + 2) {
+              Frag<2, 2> fb;
+              fb.set(0, to_f32(krow[n * 8 * PK]));
+              fb.set(1, to_f32(krow[n * 8 * PK + 1]));
+              mma_parts(pr[n], fa, fb);
+            }
+          mma_rows<float, S::kOTiles, 2, PS>(acc, fa, state + kk * 8 * PS + oc);
         }
-        const float* sp = state + (kk * 8 + 2 * t) * PS + oc + g;
+      } else {
+        const T* qp = sq + (mi * 16 + lane % 16) * PK + lane / 16 * 8;
+        const T* kp = sk + (lane / 16 * 8 + lane % 8) * PK + lane / 8 % 2 * 8;
+#pragma unroll 2
+        for (int kb = 0; kb < DK / 16; ++kb) {
+          uint32_t fq[4];
+          load_blocks<4, false>(fq, qp + kb * 16);
 #pragma unroll
-        for (int j = 0; j < S::kOTiles; ++j) {
-          Frag<2, PARTS> fb;
-          if constexpr (S::kSplit) {
-            fb.set(0, sp[j * 8]);
-            fb.set(1, sp[PS + j * 8]);
-          } else {
-            fb.exact(0, sp[j * 8]);
-            fb.exact(1, sp[PS + j * 8]);
+          for (int n = 0; n < 8; n += 2)
+            if (n < 2 * mi + 2) {
+              uint32_t fk[4];
+              load_blocks<4, false>(fk, kp + n * 8 * PK + kb * 16);
+              mma_16<T>(pr[n], fq, fk[0], fk[1]);
+              mma_16<T>(pr[n + 1], fq, fk[2], fk[3]);
+            }
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float2 x = unpack<T>(fq[2 * half]), y = unpack<T>(fq[2 * half + 1]);
+            Frag<4, 1> fa;
+            fa.exact(0, x.x);
+            fa.exact(1, y.x);
+            fa.exact(2, x.y);
+            fa.exact(3, y.y);
+            const float* sp = state + (kb * 16 + half * 8 + 2 * t) * PS + oc + g;
+#pragma unroll
+            for (int j = 0; j < S::kOTiles; ++j) {
+              Frag<2, 1> fb;
+              fb.exact(0, sp[j * 8]);
+              fb.exact(1, sp[PS + j * 8]);
+              mma_parts(acc[j], fa, fb);
+            }
           }
-          mma_parts(acc[j], fa, fb);
         }
       }
       const int i0 = mi * 16 + g;
@@ -349,54 +441,19 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
         acc[j][2] *= f1;
         acc[j][3] *= f1;
       }
-      // P, 16 rows by 8 keys at a time, straight into P v
-      for (int n = 0; n < 2 * mi + 2; ++n) {
-        float p[4] = {0.f, 0.f, 0.f, 0.f};
-        const T* krow = sk + (n * 8 + g) * PK;
-        if constexpr (S::kSplit) {
-#pragma unroll 4
-          for (int kk = 0; kk < DK / 8; ++kk) {
-            Frag<4, 2> fa;
-            Frag<2, 2> fb;
-            const int at = kk * 8 + 2 * t;
+      // + P v
 #pragma unroll
-            for (int e = 0; e < 4; ++e) fa.set(e, to_f32(qrow[at + (e & 1) * 8 * PK + (e >> 1)]));
-            fb.set(0, to_f32(krow[at]));
-            fb.set(1, to_f32(krow[at + 1]));
-            mma_parts(p, fa, fb);
+      for (int n = 0; n < 8; ++n)
+        if (n < 2 * mi + 2) {
+          Frag<4, PARTS> fp;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = mi * 16 + g + (e >> 1) * 8 - (n * 8 + 2 * t + (e & 1));
+            // C layout (row, 2t + e&1) to A layout (row, slot t + 4 (e&1)): key 2t + s sits in slot t + 4 s
+            fp.set((e >> 1) + (e & 1) * 2, d >= 0 ? pr[n][e] * (R.a * dec[max(d, 0)]) : 0.f);
           }
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < DK / 16; ++kk) {
-            const T* x = qrow + kk * 16 + 2 * t;
-            const uint32_t fa[4] = {*reinterpret_cast<const uint32_t*>(x), *reinterpret_cast<const uint32_t*>(x + 8 * PK),
-                                    *reinterpret_cast<const uint32_t*>(x + 8),
-                                    *reinterpret_cast<const uint32_t*>(x + 8 * PK + 8)};
-            const T* y = krow + kk * 16 + 2 * t;
-            mma_16<T>(p, fa, *reinterpret_cast<const uint32_t*>(y), *reinterpret_cast<const uint32_t*>(y + 8));
-          }
+          mma_rows<T, S::kOTiles, PARTS, PV>(acc, fp, sv + n * 8 * PV + oc);
         }
-        Frag<4, PARTS> fp;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = mi * 16 + g + (e >> 1) * 8 - (n * 8 + 2 * t + (e & 1));
-          // C layout (row, 2t + e&1) to A layout (row, slot t + 4 (e&1)): key 2t + s sits in slot t + 4 s
-          fp.set((e >> 1) + (e & 1) * 2, d >= 0 ? p[e] * (R.a * dec[max(d, 0)]) : 0.f);
-        }
-        const T* vp = sv + (n * 8 + 2 * t) * PV + oc + g;
-#pragma unroll
-        for (int j = 0; j < S::kOTiles; ++j) {
-          Frag<2, PARTS> fb;
-          if constexpr (S::kSplit) {
-            fb.set(0, to_f32(vp[j * 8]));
-            fb.set(1, to_f32(vp[PV + j * 8]));
-          } else {
-            fb.exact(0, to_f32(vp[j * 8]));
-            fb.exact(1, to_f32(vp[PV + j * 8]));
-          }
-          mma_parts(acc[j], fp, fb);
-        }
-      }
       // Keys behind a row have weight 0 in P, but 0 times an infinite or NaN value is NaN: where a
       // result is not finite, its rows are taken again from the keys before them alone.
       float bad = 0.f;
@@ -468,29 +525,30 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
       for (int j = 0; j < S::kSTiles; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[j][e] = 0.f;
-      const int blocks = (rows + 7) / 8;
-#pragma unroll 2
-      for (int kk = 0; kk < blocks; ++kk) {
-        const int j0 = kk * 8 + 2 * t;
-        const float w0 = R.c * dec[max(rows - 1 - j0 + back, 0)], w1 = R.c * dec[max(rows - 2 - j0 + back, 0)];
-        Frag<4, 2> fa;
-        const T* p = sk + j0 * PK + sr + g;
-        fa.set(0, to_f32(p[0]) * w0);
-        fa.set(1, to_f32(p[8]) * w0);
-        fa.set(2, to_f32(p[PK]) * w1);
-        fa.set(3, to_f32(p[PK + 8]) * w1);
-        const T* vp = sv + j0 * PV + sc + g;
+      const int blocks = (rows + 15) / 16;
+#pragma unroll 1
+      for (int kb = 0; kb < blocks; ++kb) {
+        uint32_t fk[4];
+        if constexpr (!S::kSplit) load_blocks<4, true>(fk, sk + (kb * 16 + lane / 16 * 8 + lane % 8) * PK + sr + lane / 8 % 2 * 8);
 #pragma unroll
-        for (int j = 0; j < S::kSTiles; ++j) {
-          Frag<2, PARTS> fb;
+        for (int half = 0; half < 2; ++half) {
+          const int j0 = kb * 16 + half * 8 + 2 * t;
+          const float w0 = R.c * dec[max(rows - 1 - j0 + back, 0)], w1 = R.c * dec[max(rows - 2 - j0 + back, 0)];
+          Frag<4, 2> fa;
           if constexpr (S::kSplit) {
-            fb.set(0, to_f32(vp[j * 8]));
-            fb.set(1, to_f32(vp[PV + j * 8]));
+            const T* p = sk + j0 * PK + sr + g;
+            fa.set(0, to_f32(p[0]) * w0);
+            fa.set(1, to_f32(p[8]) * w0);
+            fa.set(2, to_f32(p[PK]) * w1);
+            fa.set(3, to_f32(p[PK + 8]) * w1);
           } else {
-            fb.exact(0, to_f32(vp[j * 8]));
-            fb.exact(1, to_f32(vp[PV + j * 8]));
+            const float2 x = unpack<T>(fk[2 * half]), y = unpack<T>(fk[2 * half + 1]);
+            fa.set(0, x.x * w0);
+            fa.set(1, y.x * w0);
+            fa.set(2, x.y * w1);
+            fa.set(3, y.y * w1);
           }
-          mma_parts(d[j], fa, fb);
+          mma_rows<T, S::kSTiles, 2, PV>(d, fa, sv + (kb * 16 + half * 8) * PV + sc);
         }
       }
       const float hi = dec[rows], lo = dec_lo[rows];

@@ -18,12 +18,13 @@
 // registers and is scaled by g^n as a sum of two float32.
 //
 // One block per (segment, head, role), 12 warps:
-//   0-3   P: read from TMEM, weigh, split, write back as the A operand of P v
-//   4-7   k': in place of k, and its other two parts beside it
-//   0-7   o, half of the columns each, through the state's place in shared
-//         memory to whole lines of global memory; the state, likewise
+//   0-7   P: read from TMEM, weigh, split, write back as the A operand of P v;
+//         k': in place of k, and its other two parts beside it;
+//         o, through the state's place in shared memory to whole lines of
+//         global memory; the state.  Two warps share 32 rows and split the columns.
 //   8     one thread issues every product
-//   9     loads by TMA; q as soon as X is done, k and v after E.  Packed
+//   9     loads by TMA; q as soon as X is done, k after the first
+//         part of E, v after all of it.  Packed
 //         sequences (a box would reach into a neighbour) and operands that no
 //         tensor map describes are loaded row by row by warps 9-11 (cp.async).
 // Tiles hold tokens in their natural order for either direction; backwards in
@@ -53,7 +54,7 @@ struct Shape {
   static constexpr int kTile = kC * D * 2, kState = D * D * 2;
   static constexpr int kQ = 0, kK = kTile, kV = 2 * kTile, kMid = 3 * kTile, kLo = 4 * kTile;
   static constexpr int kSHi = 5 * kTile, kSLo = kSHi + kState, kTable = kSLo + kState;
-  static constexpr int kSmem = kTable + (int)sizeof(float) * 2 * 132 + 128 + 10 * 8 + 64;
+  static constexpr int kSmem = kTable + (int)sizeof(float) * 2 * 132 + 12 * 8 + 64;
   // TMEM columns: P (also in two bfloat16 parts), O, X, E.  With D = 64, E shares X's, so that two
   // blocks fit on an SM; X is then read before E is issued.
   static constexpr int kP = 0, kO = 128, kX = 128 + D, kE = D == 64 ? kX : kX + D;
@@ -69,7 +70,7 @@ struct Maps {
   int used;
 };
 
-enum Bar { kFull, kQK, kQS, kPV, kKV, kPDone, kKDone, kSReady, kXRead, kBars };
+enum Bar { kFull, kVFull, kQK, kQS, kPV, kKFree, kKV, kPDone, kKDone, kSReady, kXRead, kBars };
 
 __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
   uint64_t d = (uint64_t)((addr >> 4) & 0x3FFF);
@@ -148,7 +149,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Two neighbours as bfloat16 (the first in the lower half), and what that loses of them.
+// Two neighbours as bfloat16, the first in the lower half.
 __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
@@ -156,6 +157,33 @@ __device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
 }
 __device__ __forceinline__ float low_f32(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high_f32(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
+// Their leading 8 bits as bfloat16, which they lose: the parts before the last are cut off, not
+// rounded (what is cut goes into the next part exactly), which takes a byte permutation for two.
+__device__ __forceinline__ uint32_t take_bf16(float& x, float& y) {
+  const uint32_t r = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+  x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+  return r;
+}
+
+// Weighs 32 neighbouring values of a row of P by a g^d, d tokens from the key to the row, by steps of
+// one token in registers: the products keep shared memory busy.  kDiagonal: the row's own key is
+// number `own` of them; else w is the weight of the nearest.
+template <bool kBack, bool kDiagonal>
+__device__ __forceinline__ void weigh(uint32_t (&v)[32], float w, float a, float g, int own) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const int j = kBack ? i : 31 - i;
+    if (kDiagonal) {
+      w = j == own ? a : w;
+      const float x = __uint_as_float(v[j]) * w;
+      v[j] = __float_as_uint((kBack ? j < own : j > own) ? 0.f : x);
+    } else {
+      v[j] = __float_as_uint(__uint_as_float(v[j]) * w);
+    }
+    w *= g;
+  }
+}
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int token, int head, int batch,
                                          uint64_t* bar) {
@@ -181,9 +209,8 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
   extern __shared__ __align__(1024) unsigned char sm[];
   float* dec = reinterpret_cast<float*>(sm + S::kTable);
   float* dec_lo = dec + 132;
-  float* mirror = dec_lo + 132;  // dec[31 - j]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(mirror + 32);
-  chunk::Segment* seg_shared = reinterpret_cast<chunk::Segment*>(bars + 10);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(dec_lo + 132);
+  chunk::Segment* seg_shared = reinterpret_cast<chunk::Segment*>(bars + 12);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seg_shared + 1);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* odd = reinterpret_cast<int*>(tmem_slot + 2);
@@ -214,13 +241,12 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       const double x = n ? exp(ld * n) : 1.0, rest = x - (double)(float)x;
       dec[n] = (float)x;
       dec_lo[n] = rest == rest ? (float)rest : 0.f;
-      if (n < 32) mirror[31 - n] = (float)x;
     }
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const int count = i == kFull ? (maps.used ? 1 : kLoaders)
-                                   : (i == kPDone || i == kKDone ? 128 : (i == kSReady || i == kXRead ? 256 : 1));
+      const int count = i == kFull || i == kVFull ? (maps.used ? 1 : kLoaders)
+                                   : (i >= kPDone ? 256 : 1);
       mbar_init(&bars[i], count);
     }
     *gave_up = 0;
@@ -265,13 +291,15 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
           const int token = (int)first_token(c);
           if (want_o) {
             if (c > 0 && !wait(&bars[kQS], (c - 1) & 1, gave_up)) break;
-            mbar_arrive_expect_tx(&bars[kFull], 3 * S::kTile);
+            mbar_arrive_expect_tx(&bars[kFull], 2 * S::kTile);
             for (int x = 0; x < D; x += 64) tma_load(base + S::kQ + x / 64 * kBlockBytes, mq, x, token, hq, b, &bars[kFull]);
           }
-          if (c > 0 && !wait(&bars[kKV], (c - 1) & 1, gave_up)) break;
-          if (!want_o) mbar_arrive_expect_tx(&bars[kFull], 2 * S::kTile);
+          if (c > 0 && !wait(&bars[kKFree], (c - 1) & 1, gave_up)) break;
+          if (!want_o) mbar_arrive_expect_tx(&bars[kFull], S::kTile);
           for (int x = 0; x < D; x += 64) tma_load(base + S::kK + x / 64 * kBlockBytes, mk, x, token, hk, b, &bars[kFull]);
-          for (int x = 0; x < D; x += 64) tma_load(base + S::kV + x / 64 * kBlockBytes, mv, x, token, hv, b, &bars[kFull]);
+          if (c > 0 && !wait(&bars[kKV], (c - 1) & 1, gave_up)) break;
+          mbar_arrive_expect_tx(&bars[kVFull], S::kTile);
+          for (int x = 0; x < D; x += 64) tma_load(base + S::kV + x / 64 * kBlockBytes, mv, x, token, hv, b, &bars[kVFull]);
           if (c + 1 < chunks) {
             const int next = (int)first_token(c + 1);
             for (int x = 0; x < D; x += 64) tma_prefetch(mk, x, next, hk, b);
@@ -302,13 +330,18 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
           if (c > 0 && !wait_warp(&bars[kQS], (c - 1) & 1, gave_up)) break;
           rows_in(S::kQ, R.q, R.qs, R.qdiv, R.wk, c);
         }
-        if (c > 0 && !wait_warp(&bars[kKV], (c - 1) & 1, gave_up)) break;
+        if (c > 0 && !wait_warp(&bars[kKFree], (c - 1) & 1, gave_up)) break;
         rows_in(S::kK, R.k, R.ks, R.kdiv, R.wk, c);
+        chunk::cp_commit();
+        if (c > 0 && !wait_warp(&bars[kKV], (c - 1) & 1, gave_up)) break;
         rows_in(S::kV, R.v, R.vs, R.vdiv, R.wv, c);
         chunk::cp_commit();
-        chunk::cp_wait<0>();
+        chunk::cp_wait<1>();
         fence_proxy_async();
         arrive(&bars[kFull]);
+        chunk::cp_wait<0>();
+        fence_proxy_async();
+        arrive(&bars[kVFull]);
       }
       chunk::cp_wait<0>();
     }
@@ -337,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
               mma_ss(tmem + S::kX, desc(base + S::kQ + k / 4 * kBlockBytes + k % 4 * 32, 16),
                      desc(base + (part ? S::kSLo : S::kSHi) + k * 2048, D * 128), kQSId, part + k > 0);
           commit(&bars[kQS]);
-          if (!wait(&bars[kPDone], ph, gave_up)) break;
+          if (!wait(&bars[kVFull], ph, gave_up) || !wait(&bars[kPDone], ph, gave_up)) break;
           fence_after();
 #pragma unroll
           for (int k = 0; k < kC / 16; ++k) {
@@ -348,15 +381,16 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
           commit(&bars[kPV]);
         }
         if (!wait(&bars[kKDone], ph, gave_up)) break;
-        if (!want_o && !wait(&bars[kSReady], ph, gave_up)) break;
+        if (!want_o && (!wait(&bars[kVFull], ph, gave_up) || !wait(&bars[kSReady], ph, gave_up))) break;
         if (want_o && S::kShared && !wait(&bars[kXRead], ph, gave_up)) break;
         fence_after();
 #pragma unroll
-        for (int k = 0; k < kC / 16; ++k) {
-          const uint64_t v = desc(base + S::kV + k * 2048, kBlockBytes);
-          mma_ss(tmem + S::kE, desc(base + S::kLo + k * 2048, kBlockBytes), v, kKVId, k > 0);
-          mma_ss(tmem + S::kE, desc(base + S::kMid + k * 2048, kBlockBytes), v, kKVId, 1);
-          mma_ss(tmem + S::kE, desc(base + S::kK + k * 2048, kBlockBytes), v, kKVId, 1);
+        for (int part = 0; part < 3; ++part) {
+#pragma unroll
+          for (int k = 0; k < kC / 16; ++k)
+            mma_ss(tmem + S::kE, desc(base + (part == 0 ? S::kK : (part == 1 ? S::kMid : S::kLo)) + k * 2048, kBlockBytes),
+                   desc(base + S::kV + k * 2048, kBlockBytes), kKVId, part + k > 0);
+          if (part == 0) commit(&bars[kKFree]);
         }
         commit(&bars[kKV]);
       }
@@ -381,9 +415,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = st[j + 2 * e], y = st[j + 2 * e + 1];
-            hi[e] = pack_bf16(x, y);
-            lo[e] = pack_bf16(x - low_f32(hi[e]), y - high_f32(hi[e]));
+            float x = st[j + 2 * e], y = st[j + 2 * e + 1];
+            hi[e] = take_bf16(x, y);
+            lo[e] = pack_bf16(x, y);
           }
           const uint32_t at = (c0 + j) / 64 * (D * 128) + row * 128 + ((((c0 + j) % 64) / 8) ^ (row & 7)) * 16;
           *reinterpret_cast<uint4*>(sm + S::kSHi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -400,37 +434,29 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       else arrive(&bars[kSReady]);
     }
     bool strange = false;
+    const float g = dec[1];
     for (int c = 0; c < chunks; ++c) {
       const uint32_t ph = c & 1;
       const int rows = min(kC, len - c * kC);
-      if (group == 0) {
-        if (want_o) {
-          if (!wait_warp(&bars[kQK], ph, gave_up)) break;
+      if (!wait_warp(want_o ? &bars[kQK] : &bars[kFull], ph, gave_up)) break;
+      if (want_o) {
           fence_after();
+          // the row's 4 pieces of 32 keys, every other one for each of the two warps that have the row
 #pragma unroll 1
-          for (int p = 0; p < 4; ++p) {
+          for (int p = group; p < 4; p += 2) {
             const uint32_t at = tmem + S::kP + p * 32 + lanes;
             uint32_t v[32], out[32];
-            if (p == warp) {  // the diagonal: g^d, d tokens from the key to the row
+            const bool diagonal = p == warp % 4;
+            if (diagonal || (p < warp % 4) != (back != 0)) {
               tmem_ld32(v, at);
+              const float w = diagonal ? 0.f : R.a * dec[back ? p * 32 - row : row - p * 32 - 31];
               tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int d = back ? j - lane : lane - j;
-                v[j] = d >= 0 ? __float_as_uint(__uint_as_float(v[j]) * (R.a * dec[d])) : 0;
-              }
-            } else if ((p < warp) != (back != 0)) {  // g^(from the piece's last key on) g^(to that key)
-              tmem_ld32(v, at);
-              const float f = R.a * dec[back ? p * 32 - row : row - p * 32 - 31];
-              const float4* tab = reinterpret_cast<const float4*>(back ? dec : mirror);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 w = tab[j / 4];
-                v[j] = __float_as_uint(__uint_as_float(v[j]) * f * w.x);
-                v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) * f * w.y);
-                v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) * f * w.z);
-                v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) * f * w.w);
+              if (diagonal) {
+                if (back) weigh<true, true>(v, w, R.a, g, lane);
+                else weigh<false, true>(v, w, R.a, g, lane);
+              } else {
+                if (back) weigh<true, false>(v, w, R.a, g, 0);
+                else weigh<false, false>(v, w, R.a, g, 0);
               }
             } else {  // keys behind all of this warp's rows
 #pragma unroll
@@ -438,21 +464,19 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const float x = __uint_as_float(v[2 * j]), y = __uint_as_float(v[2 * j + 1]);
-              out[j] = pack_bf16(x, y);
-              out[16 + j] = pack_bf16(x - low_f32(out[j]), y - high_f32(out[j]));
+              float x = __uint_as_float(v[2 * j]), y = __uint_as_float(v[2 * j + 1]);
+              out[j] = take_bf16(x, y);
+              out[16 + j] = pack_bf16(x, y);
             }
             tmem_st32(at, out);
           }
           tmem_st_wait();
           fence_before();
           arrive(&bars[kPDone]);
-        }
-      } else {
-        if (!wait_warp(want_o ? &bars[kQK] : &bars[kFull], ph, gave_up)) break;
-        const int t = threadIdx.x - 128;
+      }
+      {
 #pragma unroll 4
-        for (int i = t; i < S::kTile / 16; i += 128) {
+        for (int i = threadIdx.x; i < S::kTile / 16; i += 256) {
           const int j = i / 8 % kC;  // rows that belong to no token are zero
           const float w = R.c * dec[max(back ? rows - (kC - 1) + j : rows - 1 - j, 0)];
           uint4* at = reinterpret_cast<uint4*>(sm + S::kK) + i;
@@ -462,11 +486,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float x = low_f32(in[e]) * w, y = high_f32(in[e]) * w;
-            hi[e] = pack_bf16(x, y);
-            x -= low_f32(hi[e]);
-            y -= high_f32(hi[e]);
-            mid[e] = pack_bf16(x, y);
-            lo[e] = pack_bf16(x - low_f32(mid[e]), y - high_f32(mid[e]));
+            hi[e] = take_bf16(x, y);
+            mid[e] = take_bf16(x, y);
+            lo[e] = pack_bf16(x, y);
           }
           *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           reinterpret_cast<uint4*>(sm + S::kMid)[i] = make_uint4(mid[0], mid[1], mid[2], mid[3]);
@@ -477,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       }
       if (want_o) {
         // o: row `row` of the chunk, columns c0 .. c0 + D/2
-        constexpr int kW = 16;
+        constexpr int kW = D == 128 ? 32 : 16;
         float x_kept[S::kShared ? D / 2 : 1];
         if (!wait_warp(&bars[kQS], ph, gave_up)) break;
         fence_after();
@@ -506,8 +528,12 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
         for (int j = 0; j < D / 2; j += kW) {
           uint32_t o[kW], x[kW];
           __syncwarp();
-          tmem_ld16(o, tmem + S::kO + c0 + j + lanes);
-          if constexpr (!S::kShared) tmem_ld16(x, tmem + S::kX + c0 + j + lanes);
+          if constexpr (S::kShared) {
+            tmem_ld16(o, tmem + S::kO + c0 + j + lanes);
+          } else {
+            tmem_ld32(o, tmem + S::kO + c0 + j + lanes);
+            tmem_ld32(x, tmem + S::kX + c0 + j + lanes);
+          }
           tmem_ld_wait();
           float y[kW];
 #pragma unroll
