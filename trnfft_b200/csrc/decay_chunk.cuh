@@ -37,6 +37,8 @@ __device__ __forceinline__ uint32_t tf32(float x) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
   return r;
 }
+// The same in two integer instructions, for finite x: NaN may become 0.
+__device__ __forceinline__ uint32_t tf32_finite(float x) { return (__float_as_uint(x) + 0x1000u) & 0xffffe000u; }
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -65,9 +67,14 @@ __device__ __forceinline__ void mma_16<__half>(float (&d)[4], const uint32_t (&a
 template <int N, int PARTS>
 struct Frag {
   uint32_t p[PARTS][N];
+  // (the first of two parts is cut off, and keeps NaN; what is cut is rounded)
   __device__ __forceinline__ void set(int i, float x) {
-    p[0][i] = tf32(x);
-    if constexpr (PARTS > 1) p[1][i] = tf32(x - __uint_as_float(p[0][i]));
+    if constexpr (PARTS > 1) {
+      p[0][i] = __float_as_uint(x) & 0xffffe000u;
+      p[1][i] = tf32_finite(x - __uint_as_float(p[0][i]));
+    } else {
+      p[0][i] = tf32(x);
+    }
   }
   // a value that TF32 holds exactly
   __device__ __forceinline__ void exact(int i, float x) {
@@ -355,6 +362,11 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
   // rows of P and o: two of the warps that share a scheduler have 5 blocks of 16 keys together
   const int mi = warp < 4 ? warp : 7 - warp, oc = warp / 4 * (DV / 2);
   constexpr int PARTS = S::kSplit ? 2 : 1;
+  // Weights a g^d of this thread's places in a block of 8 keys, d tokens from the key to the row: in the
+  // row's own block, in the one before, and (as products with cf) in those before that.
+  const float own0 = R.a * dec[max(g - 2 * t, 0)], own1 = R.a * dec[max(g - 2 * t - 1, 0)];
+  const float next0 = R.a * dec[g + 8 - 2 * t], next1 = R.a * dec[g + 7 - 2 * t];
+  const float rf0 = R.a * dec[g + 1], rf1 = R.a * dec[g + 9], cf0 = dec[7 - 2 * t], cf1 = dec[6 - 2 * t], g8 = dec[8];
 
   for (int c = 0; c < chunks; ++c) {
     const int stage = STAGES == 2 ? c & 1 : 0, rows = min(kC, len - c * kC);
@@ -441,16 +453,35 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
         acc[j][2] *= f1;
         acc[j][3] *= f1;
       }
-      // + P v
+      // + P v, from the diagonal on to the first keys: there the weights shrink by g^8 a block
+      float near0 = rf0, near1 = rf1;
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
+      for (int n = 7; n >= 0; --n)
         if (n < 2 * mi + 2) {
+          float w[4];
+          if (n == 2 * mi + 1) {
+            w[0] = w[1] = 0.f;
+            w[2] = own0;
+            w[3] = own1;
+          } else if (n == 2 * mi) {
+            w[0] = own0;
+            w[1] = own1;
+            w[2] = next0;
+            w[3] = next1;
+          } else {
+            w[0] = near0 * cf0;
+            w[1] = near0 * cf1;
+            w[2] = near1 * cf0;
+            w[3] = near1 * cf1;
+            near0 *= g8;
+            near1 *= g8;
+          }
           Frag<4, PARTS> fp;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int d = mi * 16 + g + (e >> 1) * 8 - (n * 8 + 2 * t + (e & 1));
+            const bool behind = (n == 2 * mi + 1 && e < 2) || (n >= 2 * mi && (e >> 1) == n - 2 * mi && 2 * t + (e & 1) > g);
             // C layout (row, 2t + e&1) to A layout (row, slot t + 4 (e&1)): key 2t + s sits in slot t + 4 s
-            fp.set((e >> 1) + (e & 1) * 2, d >= 0 ? pr[n][e] * (R.a * dec[max(d, 0)]) : 0.f);
+            fp.set((e >> 1) + (e & 1) * 2, behind ? 0.f : pr[n][e] * w[e]);
           }
           mma_rows<T, S::kOTiles, PARTS, PV>(acc, fp, sv + n * 8 * PV + oc);
         }
