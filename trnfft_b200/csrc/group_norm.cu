@@ -118,13 +118,38 @@ __global__ void __launch_bounds__(kNormThreads, small_blocks(NV)) k_gn_small(con
 
 __device__ __forceinline__ float rstd_of(float var, float eps) { return __frsqrt_rn((var < 0.f ? 0.f : var) + eps); }
 
+// Joins the slots' sets of each group, by `glanes` threads: the distances of their means from the first of
+// them, as above.  Slots below `extra` have one row more than the others.
+__device__ __forceinline__ void join_slots(const GroupNormArgs& a, const GroupNormPlan& p, const float2* red,
+                                           const SplitPlace& at, float2* out) {
+  __syncthreads();
+  const int w = a.channels / a.groups, lanes = p.glanes, lane = threadIdx.x & (lanes - 1), full = at.rows / p.slots, extra = at.rows % p.slots;
+  const float inv = 1.f / ((float)at.rows * (float)w);
+  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x / lanes) {
+    const int g = g0 + threadIdx.x / lanes;
+    float t = 0.f, tt = 0.f, origin = 0.f;
+    if (g < a.groups) {
+      origin = red[g * w].x;
+      for (int j = 0, c = lane; j < p.slots; c += lanes) {
+        while (c >= w) c -= w, ++j;
+        if (j >= p.slots) break;
+        const float2 b = red[j * a.channels + g * w + c];
+        const float d = b.x - origin, nd = d * (float)(full + (j < extra));
+        t += nd;
+        tt += fmaf(nd, d, b.y);
+      }
+    }
+    lanes_sum(t, tt, lanes);
+    if (g < a.groups && lane == 0) out[g] = make_float2(fmaf(t, inv, origin), fmaf(-t * inv, t, tt));
+  }
+}
+
 // The sets of the block's rows of sample n, joined for each group: out[g], as (mean, M2).
 template <typename T, int V>
 __device__ __forceinline__ void split_stats(const GroupNormArgs& a, const GroupNormPlan& p, float2* red,
                                             const SplitPlace& at, SplitColumn<V>& col, long long n, float2* out) {
   constexpr int U = rows_ahead(V * sizeof(T));
   const T* x = static_cast<const T*>(a.x) + n * a.spots * a.channels + at.first;
-  const int w = a.channels / a.groups;
   for (int tile = 0; tile < p.tiles; ++tile) {
     if (p.tiles > 1) col.set(a, p, at, tile);
     if (!col.live) continue;
@@ -160,28 +185,50 @@ __device__ __forceinline__ void split_stats(const GroupNormArgs& a, const GroupN
       to[v] = make_float2(first.x[v] + d, fmaf(-s[v], d, ss[v]));
     }
   }
-  __syncthreads();
-  // Join the sets of a group, by `glanes` threads: the distances of their means from the first of
-  // them, as above.  Slots below `extra` have one row more than the others.
-  const int lanes = p.glanes, lane = threadIdx.x & (lanes - 1), full = at.rows / p.slots, extra = at.rows % p.slots;
-  const float inv = 1.f / ((float)at.rows * (float)w);
-  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x / lanes) {
-    const int g = g0 + threadIdx.x / lanes;
-    float t = 0.f, tt = 0.f, origin = 0.f;
-    if (g < a.groups) {
-      origin = red[g * w].x;
-      for (int j = 0, c = lane; j < p.slots; c += lanes) {
-        while (c >= w) c -= w, ++j;
-        if (j >= p.slots) break;
-        const float2 b = red[j * a.channels + g * w + c];
-        const float d = b.x - origin, nd = d * (float)(full + (j < extra));
-        t += nd;
-        tt += fmaf(nd, d, b.y);
+  join_slots(a, p, red, at, out);
+}
+
+// The same from the block's stream of rows.
+template <typename T, int V>
+__device__ __forceinline__ void stream_stats(const GroupNormArgs& a, const GroupNormPlan& p, unsigned char* raw, float2* red,
+                                             const SplitPlace& at, const SplitColumn<V>& col, long long n, int k,
+                                             float2* out) {
+  const void* const src[1] = {static_cast<const T*>(a.x) + (n * a.spots + (long long)k * p.part_rows) * a.channels};
+  RowStream<1> rows(raw, p, at.rows, (long long)a.channels * sizeof(T), src);
+  Pack<T, V> first;
+  float s[V], ss[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) first.x[v] = s[v] = ss[v] = 0.f;
+  for (int i = 0; i < rows.count; ++i) {
+    if (!rows.wait(i)) break;
+    if (col.live) {
+      const T* q = reinterpret_cast<const T*>(rows.buffer(i, 0)) + at.slot * a.channels + col.c;
+      const int mine = rows.rows_of(i);
+      if (i == 0 && at.slot < mine) first.load(q);
+#pragma unroll 4
+      for (int r = at.slot; r < mine; r += p.slots, q += at.step) {
+        Pack<T, V> b;
+        b.load(q);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float d = b.x[v] - first.x[v];
+          s[v] += d;
+          ss[v] = fmaf(d, d, ss[v]);
+        }
       }
     }
-    lanes_sum(t, tt, lanes);
-    if (g < a.groups && lane == 0) out[g] = make_float2(fmaf(t, inv, origin), fmaf(-t * inv, t, tt));
+    rows.release(i);
   }
+  if (col.live) {
+    const float inv = at.mine ? 1.f / (float)at.mine : 0.f;
+    float2* to = red + at.slot * a.channels + col.c;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float d = s[v] * inv;
+      to[v] = make_float2(first.x[v] + d, fmaf(-s[v], d, ss[v]));
+    }
+  }
+  join_slots(a, p, red, at, out);
 }
 
 // y of the block's rows of sample n, given (mean, rstd) of its groups.
@@ -246,12 +293,90 @@ __global__ void __launch_bounds__(kNormThreads, 3)
   }
 }
 
+// The same on samples streamed into shared memory, where both passes read them.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 3)
+    k_gn_whole_stream(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  extern __shared__ __align__(128) unsigned char raw[];
+  const long long size = a.spots * a.channels;
+  const void* const src[1] = {a.x};
+  SampleStream<1> samples(raw, p, a.batch, size * (long long)sizeof(T), src);
+  float2* red = reinterpret_cast<float2*>(raw + p.sample_buffers * size * sizeof(T) + 8 * kMaxSampleBuffers);
+  float2* group = red + p.slots * a.channels;
+  const SplitPlace at(a, p, 0);
+  SplitColumn<V> col;
+  col.set(a, p, at, 0);
+  const float inv = 1.f / ((float)a.spots * (float)(a.channels / a.groups)), inv_mine = at.mine ? 1.f / (float)at.mine : 0.f;
+  for (int i = 0; i < samples.count; ++i) {
+    const long long n = blockIdx.x + (long long)i * gridDim.x;
+    if (!samples.wait(i)) break;
+    const T* x = reinterpret_cast<const T*>(samples.buffer(i, 0)) + at.slot * a.channels + col.c;
+    if (col.live) {
+      Pack<T, V> first;
+      float s[V], ss[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) first.x[v] = s[v] = ss[v] = 0.f;
+      if (at.mine) first.load(x);
+      const T* q = x;
+#pragma unroll 4
+      for (int r = 0; r < at.mine; ++r, q += at.step) {
+        Pack<T, V> b;
+        b.load(q);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float d = b.x[v] - first.x[v];
+          s[v] += d;
+          ss[v] = fmaf(d, d, ss[v]);
+        }
+      }
+      float2* to = red + at.slot * a.channels + col.c;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float d = s[v] * inv_mine;
+        to[v] = make_float2(first.x[v] + d, fmaf(-s[v], d, ss[v]));
+      }
+    }
+    join_slots(a, p, red, at, group);
+    __syncthreads();
+    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
+      const float rstd = rstd_of(group[g].y * inv, a.eps);
+      group[g].y = rstd;
+      if (a.mean) {
+        a.mean[n * a.groups + g] = group[g].x;
+        a.rstd[n * a.groups + g] = rstd;
+      }
+    }
+    __syncthreads();
+    if (col.live) {
+      float mean[V], gain[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float2 s = group[col.group(v)];
+        mean[v] = s.x;
+        gain[v] = s.y * col.wt[v];
+      }
+      T* to = static_cast<T*>(a.y) + n * size + at.first + col.c;
+      const T* q = x;
+#pragma unroll 4
+      for (int r = 0; r < at.mine; ++r, q += at.step, to += at.step) {
+        Pack<T, V> b;
+        b.load(q);
+#pragma unroll
+        for (int v = 0; v < V; ++v) b.x[v] = activate<ACT>(fmaf(b.x[v] - mean[v], gain[v], col.bs[v]));
+        b.store(to);
+      }
+    }
+    samples.release(i);
+  }
+}
+
 // Block = part blockIdx.x % parts of sample blockIdx.x / parts: its groups' sets; the sample's last
 // block joins the parts' into (mean, rstd).
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads, 5)
+__global__ void __launch_bounds__(kNormThreads, 3)
     k_gn_stats(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
-  extern __shared__ __align__(16) float2 smem[];
+  extern __shared__ __align__(128) unsigned char raw[];
+  float2* smem = reinterpret_cast<float2*>(raw + (p.stage_rows ? kStreamBytes + 64 : 0));
   const long long n = blockIdx.x / p.parts;
   const int k = blockIdx.x % p.parts;
   float2* part = static_cast<float2*>(a.work) + n * p.parts * a.groups;
@@ -259,7 +384,10 @@ __global__ void __launch_bounds__(kNormThreads, 5)
     const SplitPlace at(a, p, k);
     SplitColumn<V> col;
     col.set(a, p, at, 0);
-    split_stats<T, V>(a, p, smem, at, col, n, part + (long long)k * a.groups);
+    if (p.stage_rows)
+      stream_stats<T, V>(a, p, raw, smem, at, col, n, k, part + (long long)k * a.groups);
+    else
+      split_stats<T, V>(a, p, smem, at, col, n, part + (long long)k * a.groups);
   }
   unsigned* count = reinterpret_cast<unsigned*>(static_cast<char*>(a.work) + p.off_sync);
   if (!last_of_sample(count + n, p.parts)) return;
@@ -293,15 +421,49 @@ __global__ void __launch_bounds__(kNormThreads, 5)
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormThreads, 4)
+__global__ void __launch_bounds__(kNormThreads, 3)
     k_gn_apply(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  extern __shared__ __align__(128) unsigned char raw[];
   const unsigned b = gridDim.x - 1 - blockIdx.x;
   const long long n = b / p.parts;
-  const SplitPlace at(a, p, b % p.parts);
+  const int k = b % p.parts;
+  const SplitPlace at(a, p, k);
   SplitColumn<V> col;
   col.set(a, p, at, 0);
-  const float2* result = reinterpret_cast<const float2*>(static_cast<const char*>(a.work) + p.off_result);
-  split_apply<T, V, ACT>(a, p, at, col, n, result + n * a.groups);
+  const float2* result = reinterpret_cast<const float2*>(static_cast<const char*>(a.work) + p.off_result) + n * a.groups;
+  if (!p.stage_rows) {
+    split_apply<T, V, ACT>(a, p, at, col, n, result);
+    return;
+  }
+  const long long base = (n * a.spots + (long long)k * p.part_rows) * a.channels;
+  const void* const src[1] = {static_cast<const T*>(a.x) + base};
+  RowStream<1> rows(raw, p, at.rows, (long long)a.channels * sizeof(T), src);
+  float mean[V], gain[V];
+  if (col.live) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float2 s = result[col.group(v)];
+      mean[v] = s.x;
+      gain[v] = s.y * col.wt[v];
+    }
+  }
+  T* to = static_cast<T*>(a.y) + base + (long long)at.slot * a.channels + col.c;
+  for (int i = 0; i < rows.count; ++i) {
+    if (!rows.wait(i)) break;
+    if (col.live) {
+      const T* q = reinterpret_cast<const T*>(rows.buffer(i, 0)) + at.slot * a.channels + col.c;
+      const int mine = rows.rows_of(i);
+#pragma unroll 4
+      for (int r = at.slot; r < mine; r += p.slots, q += at.step, to += at.step) {
+        Pack<T, V> x;
+        x.load(q);
+#pragma unroll
+        for (int v = 0; v < V; ++v) x.x[v] = activate<ACT>(fmaf(x.x[v] - mean[v], gain[v], col.bs[v]));
+        x.store(to);
+      }
+    }
+    rows.release(i);
+  }
 }
 
 // ---------------------------------------------------------------- kAny
@@ -360,16 +522,24 @@ static cudaError_t run_small(const GroupNormArgs& a, const GroupNormPlan& p, cud
 template <typename T, int V, int ACT>
 static cudaError_t run_split(const GroupNormArgs& a, const GroupNormPlan& p, cudaStream_t st) {
   cudaError_t e;
+  if (p.sample_buffers) {
+    const int smem = (int)(p.sample_buffers * a.spots * a.channels * sizeof(T)) + 8 * kMaxSampleBuffers + p.smem;
+    e = allow_smem(k_gn_whole_stream<T, V, ACT>, smem);
+    if (e == cudaSuccess) k_gn_whole_stream<T, V, ACT><<<p.grid, p.threads, smem, st>>>(a, p);
+    return e == cudaSuccess ? cudaGetLastError() : e;
+  }
   if (p.parts == 1) {
     e = allow_smem(k_gn_whole<T, V, ACT>, p.smem);
     if (e == cudaSuccess) k_gn_whole<T, V, ACT><<<p.grid, p.threads, p.smem, st>>>(a, p);
     return e == cudaSuccess ? cudaGetLastError() : e;
   }
-  e = allow_smem(k_gn_stats<T, V>, p.smem);
+  const int stream = p.stage_rows ? kStreamBytes + 64 : 0;
+  e = allow_smem(k_gn_stats<T, V>, p.smem + stream);
+  if (e == cudaSuccess) e = allow_smem(k_gn_apply<T, V, ACT>, stream);
   if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<char*>(a.work) + p.off_sync, 0, sizeof(unsigned) * a.batch, st);
   if (e != cudaSuccess) return e;
-  k_gn_stats<T, V><<<p.grid, p.threads, p.smem, st>>>(a, p);
-  k_gn_apply<T, V, ACT><<<p.grid, p.threads, 0, st>>>(a, p);
+  k_gn_stats<T, V><<<p.grid, p.threads, p.smem + stream, st>>>(a, p);
+  k_gn_apply<T, V, ACT><<<p.grid, p.threads, stream, st>>>(a, p);
   return cudaGetLastError();
 }
 
@@ -454,19 +624,31 @@ GroupNormPlan plan_group_norm(ElemType t, const GroupNormArgs& a, bool backward,
   p.threads = std::max(64, (p.slots * p.cols + 31) / 32 * 32);
   // a block's sets (backward: and its channels' sums, of one sample and of all), the groups' results
   p.smem = (int)sizeof(float2) * (p.slots * a.channels + (backward ? 2 * a.channels : 0) + a.groups);
-  const long long most = 8LL * kSms * kNormThreads / p.threads;  // blocks that fill the GPU, and then some
+  const long long most = 4LL * kSms * kNormThreads / p.threads;  // blocks that fill the GPU, and then some
   const long long bytes = a.spots * a.channels * size * (backward ? 2 : 1);
-  // parts of 32 KB at least, and as many as fill the GPU
+  // parts of 32 KB at least, as many as fill the GPU, and no more than one block joins in a few rounds
+  // of loads (1 x 16384 x 1024 in 32 groups: 592 parts 57 us, 296 parts 42 us)
   long long parts = 1;
   if (bytes > (48 << 10) && !(a.batch >= 2 * kSms && bytes <= (128 << 10)))
-    parts = std::max<long long>(1, std::min({(most + a.batch - 1) / a.batch, bytes / (32 << 10), (long long)a.spots}));
+    parts = std::max<long long>(1, std::min({(most + a.batch - 1) / a.batch, bytes / (32 << 10), (long long)a.spots,
+                                             std::max<long long>(kSms, 8192 / a.groups)}));
   // a block of one part only: cut large samples of a large batch as well, for the sake of L2
   if (parts == 1 && bytes > (128 << 10)) parts = std::min<long long>(a.spots, (bytes + (128 << 10) - 1) / (128 << 10));
   p.part_rows = (int)((a.spots + parts - 1) / parts);
   p.parts = (int)((a.spots + p.part_rows - 1) / p.part_rows);
+  // rows whose addresses and sizes are multiples of 16 bytes are streamed, whole rounds of slots at a time
+  const long long row_bytes = (long long)a.channels * size;
+  if (p.parts > 1 && p.tiles == 1 && row_bytes % 16 == 0 && align % 16 == 0)
+    p.stage_rows = (int)(kStreamBytes / kStages / (backward ? 2 : 1) / (row_bytes * p.slots)) * p.slots;
+  // samples of whole 16-byte pieces are streamed: some 64 KB of buffers per block, two blocks per SM or more
+  if (p.parts == 1 && p.tiles == 1 && a.spots * row_bytes % 16 == 0 && align % 16 == 0 && bytes <= (48 << 10)) {
+    p.sample_buffers = (int)std::min<long long>(gn::kMaxSampleBuffers, std::max<long long>(2, (64 << 10) / bytes));
+    if ((long long)p.sample_buffers * bytes + p.smem > (112 << 10)) p.sample_buffers = 0;
+  }
   p.glanes = lanes_for((long long)(backward ? 1 : p.slots) * w);
   p.planes = p.parts > 1 ? lanes_for(p.parts) : 1;
-  p.grid = (int)(p.parts == 1 ? std::min(a.batch, most) : a.batch * p.parts);
+  const long long per_sm = p.sample_buffers ? std::min<long long>(768 / p.threads, (220 << 10) / (p.sample_buffers * bytes + p.smem + 1024 + 64)) : 0;
+  p.grid = (int)(p.sample_buffers ? std::min(a.batch, kSms * per_sm) : p.parts == 1 ? std::min(a.batch, most) : a.batch * p.parts);
   const long long result = p.parts > 1 ? a.batch * a.groups * 8 : 0;
   p.off_result = (result * p.parts + 15) & ~15LL;
   p.off_channels = (p.off_result + result + 15) & ~15LL;

@@ -5,6 +5,7 @@
 
 #include "elem.cuh"
 #include "group_norm.h"
+#include "tma.cuh"
 
 namespace tfb {
 namespace gn {
@@ -195,6 +196,102 @@ struct SplitColumn {
     }
   }
 };
+
+// A block's rows of N tensors (contiguous in memory), streamed through kStages buffers in shared memory
+// by bulk copies that one thread issues ahead: bytes on their way take no registers, and the first
+// kStages buffers are asked for at once.
+template <int N>
+struct RowStream {
+  static constexpr int kBuffer = kStreamBytes / kStages / N;
+  unsigned char* buffers;
+  uint64_t* full;
+  const char* from[N];
+  long long row_bytes;
+  int rows, per, count;  // rows in all, of a buffer; buffers
+  __device__ __forceinline__ void issue(int i) {
+    const int first = i * per;
+    const uint32_t bytes = (uint32_t)(min(per, rows - first) * row_bytes);
+    uint64_t* bar = full + i % kStages;
+    mbar_arrive_expect_tx(bar, N * bytes);
+#pragma unroll
+    for (int j = 0; j < N; ++j) bulk_g2s(buffers + (i % kStages * N + j) * kBuffer, from[j] + first * row_bytes, bytes, bar);
+  }
+  __device__ __forceinline__ RowStream(unsigned char* smem, const GroupNormPlan& p, int row_count, long long bytes_per_row,
+                                       const void* const (&src)[N])
+      : buffers(smem), full(reinterpret_cast<uint64_t*>(smem + kStreamBytes)), row_bytes(bytes_per_row), rows(row_count),
+        per(p.stage_rows) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) from[j] = static_cast<const char*>(src[j]);
+    count = (rows + per - 1) / per;
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < kStages; ++i) mbar_init(full + i, 1);
+      mbar_init_fence();
+      for (int i = 0; i < min(kStages, count); ++i) issue(i);
+    }
+    __syncthreads();
+  }
+  // Waits for buffer i; true if it came.
+  __device__ __forceinline__ bool wait(int i) {
+    if (mbar_wait_bounded(full + i % kStages, i / kStages & 1)) return true;
+    if (threadIdx.x == 0) atomicExch(&g_dev_status, kStatusWaitTimeout);
+    return false;
+  }
+  __device__ __forceinline__ const unsigned char* buffer(int i, int tensor) const {
+    return buffers + (i % kStages * N + tensor) * kBuffer;
+  }
+  __device__ __forceinline__ int rows_of(int i) const { return min(per, rows - i * per); }
+  // All have read buffer i: it may be filled again.
+  __device__ __forceinline__ void release(int i) {
+    __syncthreads();
+    if (threadIdx.x == 0 && i + kStages < count) issue(i + kStages);
+  }
+};
+
+// A block's samples blockIdx.x, blockIdx.x + gridDim.x, ... of N tensors, streamed whole through
+// p.sample_buffers buffers.
+template <int N>
+struct SampleStream {
+  unsigned char* buffers;
+  uint64_t* full;
+  const char* from[N];
+  long long bytes;  // of a sample of one tensor
+  int count, ring;
+  __device__ __forceinline__ void issue(int i) {
+    uint64_t* bar = full + i % ring;
+    mbar_arrive_expect_tx(bar, (uint32_t)(N * bytes));
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      bulk_g2s(buffers + (i % ring * N + j) * bytes, from[j] + (blockIdx.x + (long long)i * gridDim.x) * bytes,
+               (uint32_t)bytes, bar);
+  }
+  __device__ __forceinline__ SampleStream(unsigned char* smem, const GroupNormPlan& p, long long samples,
+                                          long long sample_bytes, const void* const (&src)[N])
+      : buffers(smem), full(reinterpret_cast<uint64_t*>(smem + p.sample_buffers * N * sample_bytes)), bytes(sample_bytes),
+        ring(p.sample_buffers) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) from[j] = static_cast<const char*>(src[j]);
+    count = (int)((samples - blockIdx.x + gridDim.x - 1) / gridDim.x);
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < ring; ++i) mbar_init(full + i, 1);
+      mbar_init_fence();
+      for (int i = 0; i < min(ring, count); ++i) issue(i);
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ bool wait(int i) {
+    if (mbar_wait_bounded(full + i % ring, i / ring & 1)) return true;
+    if (threadIdx.x == 0) atomicExch(&g_dev_status, kStatusWaitTimeout);
+    return false;
+  }
+  __device__ __forceinline__ const unsigned char* buffer(int i, int tensor) const {
+    return buffers + (i % ring * N + tensor) * bytes;
+  }
+  __device__ __forceinline__ void release(int i) {
+    __syncthreads();
+    if (threadIdx.x == 0 && i + ring < count) issue(i + ring);
+  }
+};
+constexpr int kMaxSampleBuffers = 8;
 
 }  // namespace gn
 }  // namespace tfb

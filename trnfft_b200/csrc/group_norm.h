@@ -38,6 +38,8 @@ struct GroupNormPlan {
   int lanes, nv;
   // kSplit: `parts` blocks of `part_rows` rows per sample, `slots` rows of `cols` threads per block
   int parts, part_rows, slots, cols, tiles, threads, smem;
+  int stage_rows;      // parts > 1: rows of a buffer of a block's stream; 0: rows are loaded by their threads
+  int sample_buffers;  // parts == 1: buffers of a block's stream of samples; 0: rows are loaded by their threads
   int glanes, planes;  // threads that join a group's sets within a block, across the parts
   int grid;
   // work area, in bytes from its start (all 16-byte aligned); the parts' sets come first
@@ -47,6 +49,7 @@ struct GroupNormPlan {
 constexpr int kNormThreads = 256;
 constexpr int kMaxSplitChannels = 8192;  // three float2 each in shared memory
 constexpr int kSms = 148;
+constexpr int kStages = 4, kStreamBytes = 64 * 1024;  // buffers of a block's stream of rows
 // Rows of `bytes` that a thread of kSplit has on their way at a time.
 constexpr int rows_ahead(int bytes) { return 64 / bytes < 4 ? 64 / bytes : 4; }
 

@@ -121,12 +121,46 @@ struct SplitBwdSmem {
   float2* group;  // groups: (mean of u, mean of u h)
 };
 
+// The slots' sums joined: of each channel, added to the block's; of each group.
+__device__ __forceinline__ void join_slots_bwd(const GroupNormArgs& a, const GroupNormPlan& p, const SplitBwdSmem& sm,
+                                               float2* out) {
+  const int w = a.channels / a.groups;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.channels; i += blockDim.x) {
+    float2 s = make_float2(0.f, 0.f);
+    for (int j = 0; j < p.slots; ++j) {
+      const float2 b = sm.red[j * a.channels + i];
+      s.x += b.x;
+      s.y += b.y;
+    }
+    float2& acc = sm.acc[i];
+    acc.x += s.x;
+    acc.y += s.y;
+    const float wc = a.weight ? a.weight[i] : 1.f;
+    sm.chan[i] = make_float2(s.y * wc, s.x * wc);
+  }
+  __syncthreads();
+  if (!out) return;
+  const int lanes = p.glanes, lane = threadIdx.x & (lanes - 1);
+  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x / lanes) {
+    const int g = g0 + threadIdx.x / lanes;
+    float su = 0.f, suh = 0.f;
+    if (g < a.groups)
+      for (int c = lane; c < w; c += lanes) {
+        const float2 b = sm.chan[g * w + c];
+        su += b.x;
+        suh += b.y;
+      }
+    lanes_sum(su, suh, lanes);
+    if (g < a.groups && lane == 0) out[g] = make_float2(su, suh);
+  }
+}
+
 template <typename T, int V, int ACT>
 __device__ __forceinline__ void split_sums(const GroupNormArgs& a, const GroupNormPlan& p, const SplitBwdSmem& sm,
                                            const SplitPlace& at, SplitColumn<V>& col, long long n, float2* out) {
   constexpr int U = rows_ahead(2 * V * sizeof(T));
   const long long base = n * a.spots * a.channels + at.first;
-  const int w = a.channels / a.groups;
   for (int tile = 0; tile < p.tiles; ++tile) {
     if (p.tiles > 1) col.set(a, p, at, tile);
     if (!col.live) continue;
@@ -166,35 +200,52 @@ __device__ __forceinline__ void split_sums(const GroupNormArgs& a, const GroupNo
 #pragma unroll
     for (int v = 0; v < V; ++v) red[v] = make_float2(sw[v] * a.rstd[n * a.groups + col.group(v)], sb[v]);
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.channels; i += blockDim.x) {
-    float2 s = make_float2(0.f, 0.f);
-    for (int j = 0; j < p.slots; ++j) {
-      const float2 b = sm.red[j * a.channels + i];
-      s.x += b.x;
-      s.y += b.y;
-    }
-    float2& acc = sm.acc[i];
-    acc.x += s.x;
-    acc.y += s.y;
-    const float wc = a.weight ? a.weight[i] : 1.f;
-    sm.chan[i] = make_float2(s.y * wc, s.x * wc);
+  join_slots_bwd(a, p, sm, out);
+}
+
+// The same from the block's stream of rows.
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void stream_sums(const GroupNormArgs& a, const GroupNormPlan& p, unsigned char* raw,
+                                            const SplitBwdSmem& sm, const SplitPlace& at, const SplitColumn<V>& col,
+                                            long long n, int k, float2* out) {
+  const long long base = (n * a.spots + (long long)k * p.part_rows) * a.channels;
+  const void* const src[2] = {static_cast<const T*>(a.x) + base, static_cast<const T*>(a.dy) + base};
+  RowStream<2> rows(raw, p, at.rows, (long long)a.channels * sizeof(T), src);
+  float mean[V], gain[V], sw[V], sb[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const long long g = n * a.groups + (col.live ? col.group(v) : 0);
+    mean[v] = a.mean[g];
+    gain[v] = a.rstd[g] * col.wt[v];
+    sw[v] = sb[v] = 0.f;
   }
-  __syncthreads();
-  if (!out) return;
-  const int lanes = p.glanes, lane = threadIdx.x & (lanes - 1);
-  for (int g0 = 0; g0 < a.groups; g0 += blockDim.x / lanes) {
-    const int g = g0 + threadIdx.x / lanes;
-    float su = 0.f, suh = 0.f;
-    if (g < a.groups)
-      for (int c = lane; c < w; c += lanes) {
-        const float2 b = sm.chan[g * w + c];
-        su += b.x;
-        suh += b.y;
+  for (int i = 0; i < rows.count; ++i) {
+    if (!rows.wait(i)) break;
+    if (col.live) {
+      const T* px = reinterpret_cast<const T*>(rows.buffer(i, 0)) + at.slot * a.channels + col.c;
+      const T* pd = reinterpret_cast<const T*>(rows.buffer(i, 1)) + at.slot * a.channels + col.c;
+      const int mine = rows.rows_of(i);
+#pragma unroll 4
+      for (int r = at.slot; r < mine; r += p.slots, px += at.step, pd += at.step) {
+        Pack<T, V> q, d;
+        q.load(px);
+        d.load(pd);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float e = q.x[v] - mean[v], dz = d.x[v] * slope<ACT>(fmaf(e, gain[v], col.bs[v]));
+          sb[v] += dz;
+          sw[v] = fmaf(dz, e, sw[v]);
+        }
       }
-    lanes_sum(su, suh, lanes);
-    if (g < a.groups && lane == 0) out[g] = make_float2(su, suh);
+    }
+    rows.release(i);
   }
+  if (col.live) {
+    float2* red = sm.red + at.slot * a.channels + col.c;
+#pragma unroll
+    for (int v = 0; v < V; ++v) red[v] = make_float2(sw[v] * a.rstd[n * a.groups + col.group(v)], sb[v]);
+  }
+  join_slots_bwd(a, p, sm, out);
 }
 
 // dx of the block's rows of sample n, given the sums of (u, u h) over its groups times `inv`.
@@ -281,13 +332,90 @@ __global__ void __launch_bounds__(kNormThreads, 3)
   leave_channels(a, p, sm);
 }
 
+// The same on samples streamed into shared memory, where both passes read them.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 3)
+    k_gn_whole_stream_bwd(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  extern __shared__ __align__(128) unsigned char raw[];
+  const long long size = a.spots * a.channels;
+  const void* const src[2] = {a.x, a.dy};
+  SampleStream<2> samples(raw, p, a.batch, size * (long long)sizeof(T), src);
+  const SplitBwdSmem sm =
+      bwd_smem(a, p, reinterpret_cast<float2*>(raw + p.sample_buffers * 2 * size * sizeof(T) + 8 * kMaxSampleBuffers));
+  const SplitPlace at(a, p, 0);
+  SplitColumn<V> col;
+  col.set(a, p, at, 0);
+  const float inv = 1.f / ((float)a.spots * (float)(a.channels / a.groups));
+  for (int i = 0; i < samples.count; ++i) {
+    const long long n = blockIdx.x + (long long)i * gridDim.x;
+    if (!samples.wait(i)) break;
+    const T* x = reinterpret_cast<const T*>(samples.buffer(i, 0)) + at.slot * a.channels + col.c;
+    const T* dy = reinterpret_cast<const T*>(samples.buffer(i, 1)) + at.slot * a.channels + col.c;
+    float mean[V], rstd[V], gain[V];
+    if (col.live) {
+      float sw[V], sb[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const long long g = n * a.groups + col.group(v);
+        mean[v] = a.mean[g];
+        rstd[v] = a.rstd[g];
+        gain[v] = rstd[v] * col.wt[v];
+        sw[v] = sb[v] = 0.f;
+      }
+      const T *px = x, *pd = dy;
+#pragma unroll 2
+      for (int r = 0; r < at.mine; ++r, px += at.step, pd += at.step) {
+        Pack<T, V> q, d;
+        q.load(px);
+        d.load(pd);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float e = q.x[v] - mean[v], dz = d.x[v] * slope<ACT>(fmaf(e, gain[v], col.bs[v]));
+          sb[v] += dz;
+          sw[v] = fmaf(dz, e, sw[v]);
+        }
+      }
+      float2* red = sm.red + at.slot * a.channels + col.c;
+#pragma unroll
+      for (int v = 0; v < V; ++v) red[v] = make_float2(sw[v] * rstd[v], sb[v]);
+    }
+    join_slots_bwd(a, p, sm, sm.group);
+    __syncthreads();
+    if (a.y && col.live) {
+      float mu[V], muh[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float2 m = sm.group[col.group(v)];
+        mu[v] = rstd[v] * (m.x * inv);
+        muh[v] = rstd[v] * rstd[v] * (m.y * inv);
+      }
+      T* to = static_cast<T*>(a.y) + n * size + at.first + col.c;
+      const T *px = x, *pd = dy;
+#pragma unroll 2
+      for (int r = 0; r < at.mine; ++r, px += at.step, pd += at.step, to += at.step) {
+        Pack<T, V> q, d;
+        q.load(px);
+        d.load(pd);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float e = q.x[v] - mean[v], dz = d.x[v] * slope<ACT>(fmaf(e, gain[v], col.bs[v]));
+          q.x[v] = fmaf(-e, muh[v], fmaf(dz, gain[v], -mu[v]));
+        }
+        q.store(to);
+      }
+    }
+    samples.release(i);
+  }
+  leave_channels(a, p, sm);
+}
+
 // Block = part blockIdx.x % parts of sample blockIdx.x / parts: its channels' and groups' sums; the
 // sample's last block adds up the groups'.
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kNormThreads, 3)
     k_gn_sums(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
-  extern __shared__ __align__(16) float2 smem[];
-  const SplitBwdSmem sm = bwd_smem(a, p, smem);
+  extern __shared__ __align__(128) unsigned char raw[];
+  const SplitBwdSmem sm = bwd_smem(a, p, reinterpret_cast<float2*>(raw + (p.stage_rows ? kStreamBytes + 64 : 0)));
   const long long n = blockIdx.x / p.parts;
   const int k = blockIdx.x % p.parts;
   float2* part = static_cast<float2*>(a.work) + n * p.parts * a.groups;
@@ -295,7 +423,11 @@ __global__ void __launch_bounds__(kNormThreads, 3)
     const SplitPlace at(a, p, k);
     SplitColumn<V> col;
     col.set(a, p, at, 0);
-    split_sums<T, V, ACT>(a, p, sm, at, col, n, a.y ? part + (long long)k * a.groups : nullptr);
+    float2* out = a.y ? part + (long long)k * a.groups : nullptr;
+    if (p.stage_rows)
+      stream_sums<T, V, ACT>(a, p, raw, sm, at, col, n, k, out);
+    else
+      split_sums<T, V, ACT>(a, p, sm, at, col, n, out);
   }
   leave_channels(a, p, sm);
   if (!a.y) return;
@@ -323,14 +455,55 @@ __global__ void __launch_bounds__(kNormThreads, 3)
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kNormThreads, 3)
     k_gn_dx(const __grid_constant__ GroupNormArgs a, const __grid_constant__ GroupNormPlan p) {
+  extern __shared__ __align__(128) unsigned char raw[];
   const unsigned b = gridDim.x - 1 - blockIdx.x;
   const long long n = b / p.parts;
-  const SplitPlace at(a, p, b % p.parts);
+  const int k = b % p.parts;
+  const SplitPlace at(a, p, k);
   SplitColumn<V> col;
   col.set(a, p, at, 0);
-  const float2* result = reinterpret_cast<const float2*>(static_cast<const char*>(a.work) + p.off_result);
+  const float2* result = reinterpret_cast<const float2*>(static_cast<const char*>(a.work) + p.off_result) + n * a.groups;
   const float inv = 1.f / ((float)a.spots * (float)(a.channels / a.groups));
-  split_dx<T, V, ACT>(a, p, at, col, n, result + n * a.groups, inv);
+  if (!p.stage_rows) {
+    split_dx<T, V, ACT>(a, p, at, col, n, result, inv);
+    return;
+  }
+  const long long base = (n * a.spots + (long long)k * p.part_rows) * a.channels;
+  const void* const src[2] = {static_cast<const T*>(a.x) + base, static_cast<const T*>(a.dy) + base};
+  RowStream<2> rows(raw, p, at.rows, (long long)a.channels * sizeof(T), src);
+  float mean[V], gain[V], mu[V], muh[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int g = col.live ? col.group(v) : 0;
+    const float rstd = a.rstd[n * a.groups + g];
+    const float2 m = result[g];
+    mean[v] = a.mean[n * a.groups + g];
+    gain[v] = rstd * col.wt[v];
+    mu[v] = rstd * (m.x * inv);
+    muh[v] = rstd * rstd * (m.y * inv);
+  }
+  T* to = static_cast<T*>(a.y) + base + (long long)at.slot * a.channels + col.c;
+  for (int i = 0; i < rows.count; ++i) {
+    if (!rows.wait(i)) break;
+    if (col.live) {
+      const T* px = reinterpret_cast<const T*>(rows.buffer(i, 0)) + at.slot * a.channels + col.c;
+      const T* pd = reinterpret_cast<const T*>(rows.buffer(i, 1)) + at.slot * a.channels + col.c;
+      const int mine = rows.rows_of(i);
+#pragma unroll 4
+      for (int r = at.slot; r < mine; r += p.slots, px += at.step, pd += at.step, to += at.step) {
+        Pack<T, V> q, d;
+        q.load(px);
+        d.load(pd);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float e = q.x[v] - mean[v], dz = d.x[v] * slope<ACT>(fmaf(e, gain[v], col.bs[v]));
+          q.x[v] = fmaf(-e, muh[v], fmaf(dz, gain[v], -mu[v]));
+        }
+        q.store(to);
+      }
+    }
+    rows.release(i);
+  }
 }
 
 // dw, db = the sums of the blocks' rows of channel sums.
@@ -443,16 +616,24 @@ static cudaError_t run_small(const GroupNormArgs& a, const GroupNormPlan& p, cud
 template <typename T, int V, int ACT>
 static cudaError_t run_split(const GroupNormArgs& a, const GroupNormPlan& p, cudaStream_t st) {
   cudaError_t e;
+  if (p.sample_buffers) {
+    const int smem = (int)(p.sample_buffers * 2 * a.spots * a.channels * sizeof(T)) + 8 * kMaxSampleBuffers + p.smem;
+    e = allow_smem(k_gn_whole_stream_bwd<T, V, ACT>, smem);
+    if (e == cudaSuccess) k_gn_whole_stream_bwd<T, V, ACT><<<p.grid, p.threads, smem, st>>>(a, p);
+    return e == cudaSuccess ? cudaGetLastError() : e;
+  }
   if (p.parts == 1) {
     e = allow_smem(k_gn_whole_bwd<T, V, ACT>, p.smem);
     if (e == cudaSuccess) k_gn_whole_bwd<T, V, ACT><<<p.grid, p.threads, p.smem, st>>>(a, p);
     return e == cudaSuccess ? cudaGetLastError() : e;
   }
-  e = allow_smem(k_gn_sums<T, V, ACT>, p.smem);
+  const int stream = p.stage_rows ? kStreamBytes + 64 : 0;
+  e = allow_smem(k_gn_sums<T, V, ACT>, p.smem + stream);
+  if (e == cudaSuccess) e = allow_smem(k_gn_dx<T, V, ACT>, stream);
   if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<char*>(a.work) + p.off_sync, 0, sizeof(unsigned) * a.batch, st);
   if (e != cudaSuccess) return e;
-  k_gn_sums<T, V, ACT><<<p.grid, p.threads, p.smem, st>>>(a, p);
-  if (a.y) k_gn_dx<T, V, ACT><<<p.grid, p.threads, 0, st>>>(a, p);
+  k_gn_sums<T, V, ACT><<<p.grid, p.threads, p.smem + stream, st>>>(a, p);
+  if (a.y) k_gn_dx<T, V, ACT><<<p.grid, p.threads, stream, st>>>(a, p);
   return cudaGetLastError();
 }
 
