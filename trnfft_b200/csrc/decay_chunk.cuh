@@ -67,11 +67,13 @@ __device__ __forceinline__ void mma_16<__half>(float (&d)[4], const uint32_t (&a
 template <int N, int PARTS>
 struct Frag {
   uint32_t p[PARTS][N];
-  // (the first of two parts is cut off, and keeps NaN; what is cut is rounded)
+  // (Both parts are rounded: a first part that is merely cut off leaves a second one of the same sign
+  // always, and the products of second parts, which are left out, would add up to 1e-6.  Of NaN the
+  // first part may be 0, and the second is NaN.)
   __device__ __forceinline__ void set(int i, float x) {
     if constexpr (PARTS > 1) {
-      p[0][i] = __float_as_uint(x) & 0xffffe000u;
-      p[1][i] = tf32_finite(x - __uint_as_float(p[0][i]));
+      p[0][i] = tf32_finite(x);
+      p[1][i] = tf32(x - __uint_as_float(p[0][i]));
     } else {
       p[0][i] = tf32(x);
     }
@@ -86,6 +88,14 @@ template <int PA, int PB>
 __device__ __forceinline__ void mma_parts(float (&d)[4], const Frag<4, PA>& a, const Frag<2, PB>& b) {
   if constexpr (PB > 1) mma_tf32(d, a.p[0], b.p[1][0], b.p[1][1]);
   if constexpr (PA > 1) mma_tf32(d, a.p[1], b.p[0][0], b.p[0][1]);
+  mma_tf32(d, a.p[0], b.p[0][0], b.p[0][1]);
+}
+
+// The same with the products of a second part in a sum of their own, so that the first parts' sum is
+// truncated once, not three times, for each 8 terms (o of 64 x 64 heads: 1.2e-6 -> 4e-7 off).
+__device__ __forceinline__ void mma_apart(float (&d)[4], float (&rest)[4], const Frag<4, 2>& a, const Frag<2, 2>& b) {
+  mma_tf32(rest, a.p[0], b.p[1][0], b.p[1][1]);
+  mma_tf32(rest, a.p[1], b.p[0][0], b.p[0][1]);
   mma_tf32(d, a.p[0], b.p[0][0], b.p[0][1]);
 }
 
@@ -144,6 +154,20 @@ __device__ __forceinline__ void mma_rows(float (&d)[TILES][4], const Frag<4, PA>
         mma_parts(d[j + i], a, b);
       }
     }
+  }
+}
+
+template <int TILES, int PITCH>
+__device__ __forceinline__ void mma_rows_apart(float (&d)[TILES][4], float (&rest)[TILES][4], const Frag<4, 2>& a,
+                                               const float* rows) {
+  const int lane = threadIdx.x & 31;
+  const float* p = rows + lane % 4 * 2 * PITCH + lane / 4;
+#pragma unroll
+  for (int j = 0; j < TILES; ++j) {
+    Frag<2, 2> b;
+    b.set(0, p[j * 8]);
+    b.set(1, p[PITCH + j * 8]);
+    mma_apart(d[j], rest[j], a, b);
   }
 }
 
@@ -390,6 +414,16 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
       for (int n = 0; n < 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) pr[n][e] = 0.f;
+      constexpr int kRest = S::kSplit ? 8 : 1, kRestO = S::kSplit ? S::kOTiles : 1;
+      float pr_rest[kRest][4], acc_rest[kRestO][4];
+#pragma unroll
+      for (int n = 0; n < kRest; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pr_rest[n][e] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kRestO; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc_rest[j][e] = 0.f;
       // q k^T, for the 8-key blocks n that are not behind all rows, and q C, from the same parts of q
       if constexpr (S::kSplit) {
         const T* qrow = sq + (mi * 16 + g) * PK;
@@ -406,9 +440,9 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
               Frag<2, 2> fb;
               fb.set(0, to_f32(krow[n * 8 * PK]));
               fb.set(1, to_f32(krow[n * 8 * PK + 1]));
-              mma_parts(pr[n], fa, fb);
+              mma_apart(pr[n], pr_rest[n], fa, fb);
             }
-          mma_rows<float, S::kOTiles, 2, PS>(acc, fa, state + kk * 8 * PS + oc);
+          mma_rows_apart<S::kOTiles, PS>(acc, acc_rest, fa, state + kk * 8 * PS + oc);
         }
       } else {
         const T* qp = sq + (mi * 16 + lane % 16) * PK + lane / 16 * 8;
@@ -452,6 +486,12 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
         acc[j][1] *= f0;
         acc[j][2] *= f1;
         acc[j][3] *= f1;
+        if constexpr (S::kSplit) {
+          acc_rest[j][0] *= f0;
+          acc_rest[j][1] *= f0;
+          acc_rest[j][2] *= f1;
+          acc_rest[j][3] *= f1;
+        }
       }
       // + P v, from the diagonal on to the first keys: there the weights shrink by g^8 a block
       float near0 = rf0, near1 = rf1;
@@ -481,10 +521,21 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
           for (int e = 0; e < 4; ++e) {
             const bool behind = (n == 2 * mi + 1 && e < 2) || (n >= 2 * mi && (e >> 1) == n - 2 * mi && 2 * t + (e & 1) > g);
             // C layout (row, 2t + e&1) to A layout (row, slot t + 4 (e&1)): key 2t + s sits in slot t + 4 s
-            fp.set((e >> 1) + (e & 1) * 2, behind ? 0.f : pr[n][e] * w[e]);
+            float x = pr[n][e];
+            if constexpr (S::kSplit) x += pr_rest[n][e];
+            fp.set((e >> 1) + (e & 1) * 2, behind ? 0.f : x * w[e]);
           }
-          mma_rows<T, S::kOTiles, PARTS, PV>(acc, fp, sv + n * 8 * PV + oc);
+          if constexpr (S::kSplit)
+            mma_rows_apart<S::kOTiles, PV>(acc, acc_rest, fp, sv + n * 8 * PV + oc);
+          else
+            mma_rows<T, S::kOTiles, PARTS, PV>(acc, fp, sv + n * 8 * PV + oc);
         }
+      if constexpr (S::kSplit) {
+#pragma unroll
+        for (int j = 0; j < S::kOTiles; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] += acc_rest[j][e];
+      }
       // Keys behind a row have weight 0 in P, but 0 times an infinite or NaN value is NaN: where a
       // result is not finite, its rows are taken again from the keys before them alone.
       float bad = 0.f;
