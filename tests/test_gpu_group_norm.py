@@ -30,6 +30,11 @@ SHAPES = [  # shape, groups
     ((1, 200001, 8), 8),
     ((5, 3, 8192), 2),
     ((2, 12, 1001), 77),
+    ((2, 3, 9001), 1),       # more channels than a block's shared memory holds
+    ((3, 20000), 5),
+    ((2, 300, 8192), 8192),
+    ((300, 30, 40), 4),      # samples of a few KB
+    ((700, 9, 6), 1),
 ]
 
 

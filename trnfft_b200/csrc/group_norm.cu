@@ -608,13 +608,6 @@ GroupNormPlan plan_group_norm(ElemType t, const GroupNormArgs& a, bool backward,
     }
     return p;
   }
-  if (a.channels > kMaxSplitChannels) {
-    p.kind = GroupNormPlan::kAny;
-    p.vec = 1;
-    p.grid = (int)std::min<long long>(total, 16LL * kSms);
-    return p;
-  }
-  p.kind = GroupNormPlan::kSplit;
   // 4 elements per access: with 8 of a 16-bit type the channels' parameters would not fit the registers
   p.vec = a.channels % 4 == 0 && align % (4 * size) == 0 ? 4 : (size == 2 && a.channels % 2 == 0 && align % 4 == 0 ? 2 : 1);
   const int columns = (a.channels + p.vec - 1) / p.vec;
@@ -623,7 +616,16 @@ GroupNormPlan plan_group_norm(ElemType t, const GroupNormArgs& a, bool backward,
   p.slots = (int)std::min<long long>(kNormThreads / p.cols, a.spots);
   p.threads = std::max(64, (p.slots * p.cols + 31) / 32 * 32);
   // a block's sets (backward: and its channels' sums, of one sample and of all), the groups' results
-  p.smem = (int)sizeof(float2) * (p.slots * a.channels + (backward ? 2 * a.channels : 0) + a.groups);
+  const long long smem = 8LL * ((long long)p.slots * a.channels + (backward ? 2LL * a.channels : 0) + a.groups);
+  if (smem > kMaxSplitSmem) {
+    p = {};
+    p.kind = GroupNormPlan::kAny;
+    p.vec = 1;
+    p.grid = (int)std::min<long long>(total, 16LL * kSms);
+    return p;
+  }
+  p.smem = (int)smem;
+  p.kind = GroupNormPlan::kSplit;
   const long long most = 4LL * kSms * kNormThreads / p.threads;  // blocks that fill the GPU, and then some
   const long long bytes = a.spots * a.channels * size * (backward ? 2 : 1);
   // parts of 32 KB at least, as many as fill the GPU, and no more than one block joins in a few rounds

@@ -47,7 +47,7 @@ struct GroupNormPlan {
 };
 
 constexpr int kNormThreads = 256;
-constexpr int kMaxSplitChannels = 8192;  // three float2 each in shared memory
+constexpr int kMaxSplitSmem = 200 * 1024;
 constexpr int kSms = 148;
 constexpr int kStages = 4, kStreamBytes = 64 * 1024;  // buffers of a block's stream of rows
 // Rows of `bytes` that a thread of kSplit has on their way at a time.
