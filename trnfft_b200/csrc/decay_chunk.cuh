@@ -426,14 +426,19 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
         for (int e = 0; e < 4; ++e) acc_rest[j][e] = 0.f;
       // q k^T, for the 8-key blocks n that are not behind all rows, and q C, from the same parts of q
       if constexpr (S::kSplit) {
+        // (one after the other: the sums of both at once do not fit the registers of two blocks per SM)
         const T* qrow = sq + (mi * 16 + g) * PK;
-#pragma unroll 2
-        for (int kk = 0; kk < DK / 8; ++kk) {
+        auto q_parts = [&](int kk) {
           Frag<4, 2> fa;
           const int at = kk * 8 + 2 * t;
 #pragma unroll
           for (int e = 0; e < 4; ++e) fa.set(e, to_f32(qrow[at + (e & 1) * 8 * PK + (e >> 1)]));
-          const T* krow = sk + g * PK + at;
+          return fa;
+        };
+#pragma unroll 1
+        for (int kk = 0; kk < DK / 8; ++kk) {
+          const Frag<4, 2> fa = q_parts(kk);
+          const T* krow = sk + g * PK + kk * 8 + 2 * t;
 #pragma unroll
           for (int n = 0; n < 8; ++n)
             if (n < 2 * mi + 2) {
@@ -442,8 +447,14 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
               fb.set(1, to_f32(krow[n * 8 * PK + 1]));
               mma_apart(pr[n], pr_rest[n], fa, fb);
             }
-          mma_rows_apart<S::kOTiles, PS>(acc, acc_rest, fa, state + kk * 8 * PS + oc);
         }
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pr[n][e] += pr_rest[n][e];
+#pragma unroll 1
+        for (int kk = 0; kk < DK / 8; ++kk)
+          mma_rows_apart<S::kOTiles, PS>(acc, acc_rest, q_parts(kk), state + kk * 8 * PS + oc);
       } else {
         const T* qp = sq + (mi * 16 + lane % 16) * PK + lane / 16 * 8;
         const T* kp = sk + (lane / 16 * 8 + lane % 8) * PK + lane / 8 % 2 * 8;
@@ -521,9 +532,7 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
           for (int e = 0; e < 4; ++e) {
             const bool behind = (n == 2 * mi + 1 && e < 2) || (n >= 2 * mi && (e >> 1) == n - 2 * mi && 2 * t + (e & 1) > g);
             // C layout (row, 2t + e&1) to A layout (row, slot t + 4 (e&1)): key 2t + s sits in slot t + 4 s
-            float x = pr[n][e];
-            if constexpr (S::kSplit) x += pr_rest[n][e];
-            fp.set((e >> 1) + (e & 1) * 2, behind ? 0.f : x * w[e]);
+            fp.set((e >> 1) + (e & 1) * 2, behind ? 0.f : pr[n][e] * w[e]);
           }
           if constexpr (S::kSplit)
             mma_rows_apart<S::kOTiles, PV>(acc, acc_rest, fp, sv + n * 8 * PV + oc);
