@@ -126,8 +126,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     q is (batch, time, heads, width), k and v are (batch, time, kv_heads, width) and
     (batch, time, kv_heads, value width), all float32, bfloat16 or float16, any strides;
     query head h reads key/value head h // (heads // kv_heads).  Widths go up to 128.
-    log_decay (heads) holds the logarithm of each head's factor (0: no decay, -inf: the
-    token alone); it is a constant, not differentiated.  scale defaults to width ** -0.5.
+    log_decay (heads) holds the logarithm of each head's factor, at most 0 (0: no decay, -inf:
+    the token alone); it is a constant, not differentiated.  scale defaults to width ** -0.5.
 
     initial_state (sequences, heads, width, value width), float32, is the state before the
     first token (zero by default).  With return_state the result is (o, state): the state
@@ -180,9 +180,14 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     state), o (batch, heads, value width).  No gradient: train with ``decay_attention``.
     """
     fn = "decay_attention_step"
-    _check_heads(fn, q, k, v, log_decay, 3)
-    b, h, dk = q.shape
-    dv = v.shape[2]
+    qs, ks, vs = q.shape, k.shape, v.shape
+    # (the checks of _check_heads in one expression: a single token's call takes no longer than its kernel)
+    if not (len(qs) == len(ks) == len(vs) == 3 and q.dtype in DTYPES and k.dtype == q.dtype and v.dtype == q.dtype
+            and ks[:2] == vs[:2] and qs[0] == ks[0] and qs[2] == ks[2] and ks[1] > 0 and qs[1] > 0 and qs[1] % ks[1] == 0
+            and qs[2] > 0 and vs[2] > 0 and log_decay.shape == qs[1:2] and log_decay.dtype == torch.float32):
+        _check_heads(fn, q, k, v, log_decay, 3)
+    b, h, dk = qs
+    dv = vs[2]
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, log_decay, state)):
         raise ValueError(f"{fn}: has no gradient; use decay_attention, or torch.no_grad()")
     one = h * dk * dv
@@ -198,7 +203,10 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
         o, got = decay_attention_step(q, k, v, log_decay, dev_state, scale=scale)
         new_state.copy_(got)
         return restore(o), new_state
-    (q, k, v, log_decay, _), restore = place_layer(fn, q, k, v, log_decay, state)
+    device = state.get_device()
+    restore = None
+    if not (q.get_device() == k.get_device() == v.get_device() == log_decay.get_device() == device):
+        (q, k, v, log_decay, _), restore = place_layer(fn, q, k, v, log_decay, state)
     q, k, v = _unit_inner(q), _unit_inner(k), _unit_inner(v)
     if log_decay.dtype != torch.float32 or not log_decay.is_contiguous():
         log_decay = log_decay.float().contiguous()
@@ -206,8 +214,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     shape = _lib.DECAY_STEP_SHAPE.pack(b, h, k.shape[1], dk, dv, *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
                                        state.stride(0) if b > 1 else one, new_state.stride(0) if b > 1 else one,
                                        DTYPES[q.dtype], dk ** -0.5 if scale is None else scale)
-    device = q.get_device()
     _lib.call("trnfft_decay_attention_step", shape, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
               state.data_ptr(), new_state.data_ptr(), o.data_ptr(), device, _lib.raw_stream(device))
     torch.autograd.graph.increment_version(new_state)
-    return restore(o), new_state
+    return (o if restore is None else restore(o)), new_state

@@ -78,16 +78,12 @@ class _GroupNormFn(torch.autograd.Function):
         return dx, dw, db, None, None, None
 
 
-def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
-               eps: float = 1e-5, activation: str | None = None) -> torch.Tensor:
-    """act(group_norm(x)) over channels-last features, in one operator.
+def _fits(p, c):
+    return p is None or (p.dim() == 1 and p.shape[0] == c and p.dtype in DTYPES)
 
-    x is (batch, ..., channels), float32, bfloat16 or float16.  The channels fall into
-    num_groups groups; each group of each sample is normalised by its mean and variance
-    over all positions (statistics in float32), then scaled by weight and shifted by bias
-    (channels each, optional) and put through the activation: None, "relu", "silu" or
-    "gelu" (the exact one, with erf).  Differentiable once in x, weight and bias.
-    """
+
+def _refuse(x, num_groups, weight, bias, eps, activation):
+    """Says what is wrong with the arguments; the number of groups as an int if nothing is."""
     if x.dim() < 2:
         raise ValueError(f"group_norm: x must be (batch, ..., channels), got {tuple(x.shape)}")
     if x.dtype not in DTYPES:
@@ -103,11 +99,34 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
         if p is not None and (p.shape != (c,) or p.dtype not in DTYPES):
             raise ValueError(f"group_norm: {name} must hold {c} values in float32, bfloat16 or float16, got {p.dtype} "
                              f"{tuple(p.shape)}")
-    (x, weight, bias), restore = place_layer("group_norm", x, weight, bias)
+    return num_groups
+
+
+def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, activation: str | None = None) -> torch.Tensor:
+    """act(group_norm(x)) over channels-last features, in one operator.
+
+    x is (batch, ..., channels), float32, bfloat16 or float16.  The channels fall into
+    num_groups groups; each group of each sample is normalised by its mean and variance
+    over all positions (statistics in float32), then scaled by weight and shifted by bias
+    (channels each, optional) and put through the activation: None, "relu", "silu" or
+    "gelu" (z times the normal distribution function, to 1e-7).  Differentiable once in x, weight and bias.
+    """
+    c = x.shape[-1] if x.dim() else 0
+    if not (x.dim() >= 2 and x.dtype in DTYPES and c > 0 and type(num_groups) is int and num_groups > 0 and c % num_groups == 0
+            and activation in ACTIVATIONS and eps >= 0 and _fits(weight, c) and _fits(bias, c)):
+        num_groups = _refuse(x, num_groups, weight, bias, eps, activation)
+    restore = None
+    device = x.get_device()
+    if device < 0 or (weight is not None and weight.get_device() != device) or (bias is not None and
+                                                                               bias.get_device() != device):
+        (x, weight, bias), restore = place_layer("group_norm", x, weight, bias)
     x = x.contiguous()
-    weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and any(p is not None and p.requires_grad for p in (x, weight, bias)):
-        return restore(_GroupNormFn.apply(x, weight, bias, num_groups, eps, act))
-    w, b = _float(weight), _float(bias)
-    return restore(_forward(x, num_groups, w, b, eps, act, False)[0])
+        y = _GroupNormFn.apply(x, weight, bias, num_groups, eps, act)
+    else:
+        y = _forward(x, num_groups, _float(weight), _float(bias), eps, act, False)[0]
+    return y if restore is None else restore(y)

@@ -5,7 +5,21 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace tfb {
+
+// Allows kernel K `bytes` of dynamic shared memory on the current device; asked of the driver once per device.
+template <auto K>
+cudaError_t allow_shared(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ULL << dev, std::memory_order_relaxed);
+  return e;
+}
 
 enum ElemType { kF32 = 0, kBF16 = 1, kF16 = 2 };
 

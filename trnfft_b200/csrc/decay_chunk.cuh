@@ -748,7 +748,7 @@ static __global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant
 template <typename T, int D0, int D1>
 static cudaError_t run_widths(const DecayArgs& a, Pass pass, cudaStream_t st) {
   constexpr int smem = Shape<T, D0, D1>::kSmem > Shape<T, D1, D0>::kSmem ? Shape<T, D0, D1>::kSmem : Shape<T, D1, D0>::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(k_decay_chunk<T, D0, D1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = allow_shared<k_decay_chunk<T, D0, D1>>(smem);
   if (e != cudaSuccess) return e;
   const unsigned units = (unsigned)a.units + (a.cu && pass != kLocal ? 1 : 0);
   k_decay_chunk<T, D0, D1><<<dim3(units * a.heads, 1, a.roles), kThreads, smem, st>>>(a, pass);

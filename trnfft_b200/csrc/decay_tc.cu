@@ -653,7 +653,7 @@ static bool operand_map(CUtensorMap* m, const void* p, const long long* stride, 
 template <int D>
 static cudaError_t run_tc(const DecayArgs& a, const Maps& maps, chunk::Pass pass, cudaStream_t st) {
   using S = Shape<D>;
-  cudaError_t e = cudaFuncSetAttribute(k_decay_tc<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  const cudaError_t e = allow_shared<k_decay_tc<D>>(S::kSmem);
   if (e != cudaSuccess) return e;
   const unsigned units = (unsigned)a.units + (a.cu && pass != chunk::kLocal ? 1 : 0);
   k_decay_tc<D><<<dim3(units * a.heads, 1, a.roles), kThreads, S::kSmem, st>>>(a, maps, pass);

@@ -149,10 +149,10 @@ __device__ __forceinline__ bool last_of_sample(unsigned* counter, int parts) {
   return before == parts - 1;
 }
 
-template <typename K>
-static cudaError_t allow_smem(K kernel, int bytes) {
-  if (bytes <= 48 * 1024) return cudaSuccess;
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+constexpr int kMostShared = 220 * 1024;  // more than any launch here asks for
+template <auto K>
+cudaError_t allow_smem(int bytes) {
+  return bytes <= 48 * 1024 ? cudaSuccess : allow_shared<K>(kMostShared);
 }
 
 // c / w for 0 <= c < 2^14, w >= 1, where inv = 1.f / w: (c + 1/2) / w is at least 1 / (2 w) from a whole

@@ -618,18 +618,18 @@ static cudaError_t run_split(const GroupNormArgs& a, const GroupNormPlan& p, cud
   cudaError_t e;
   if (p.sample_buffers) {
     const int smem = (int)(p.sample_buffers * 2 * a.spots * a.channels * sizeof(T)) + 8 * kMaxSampleBuffers + p.smem;
-    e = allow_smem(k_gn_whole_stream_bwd<T, V, ACT>, smem);
+    e = allow_smem<k_gn_whole_stream_bwd<T, V, ACT>>(smem);
     if (e == cudaSuccess) k_gn_whole_stream_bwd<T, V, ACT><<<p.grid, p.threads, smem, st>>>(a, p);
     return e == cudaSuccess ? cudaGetLastError() : e;
   }
   if (p.parts == 1) {
-    e = allow_smem(k_gn_whole_bwd<T, V, ACT>, p.smem);
+    e = allow_smem<k_gn_whole_bwd<T, V, ACT>>(p.smem);
     if (e == cudaSuccess) k_gn_whole_bwd<T, V, ACT><<<p.grid, p.threads, p.smem, st>>>(a, p);
     return e == cudaSuccess ? cudaGetLastError() : e;
   }
   const int stream = p.stage_rows ? kStreamBytes + 64 : 0;
-  e = allow_smem(k_gn_sums<T, V, ACT>, p.smem + stream);
-  if (e == cudaSuccess) e = allow_smem(k_gn_dx<T, V, ACT>, stream);
+  e = allow_smem<k_gn_sums<T, V, ACT>>(p.smem + stream);
+  if (e == cudaSuccess) e = allow_smem<k_gn_dx<T, V, ACT>>(stream);
   if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<char*>(a.work) + p.off_sync, 0, sizeof(unsigned) * a.batch, st);
   if (e != cudaSuccess) return e;
   k_gn_sums<T, V, ACT><<<p.grid, p.threads, p.smem + stream, st>>>(a, p);
