@@ -193,6 +193,7 @@ LENGTHS = [
     ([128, 128, 1], 4, 0),
     ([700, 1, 90], 7, 9),
     ([0, 0, 0], 3, 2),
+    ([0, 0], 0, 0),          # no rows at all
 ]
 
 
@@ -229,6 +230,52 @@ def test_packed(lengths, before, behind, dtype):
         check(got[3][i:i + 1], wg[3], tg[3], dtype, terms, f"dinitial of {i}", fp32_out=True)
     for z in (o.detach(), *got[:3]):
         assert float(z[:, outside].abs().sum()) == 0, "rows of no sequence are zero"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_graph_follows_the_lengths(dtype):
+    """A captured call reads the lengths where they are: a buffer of many rows, few of them used, others each time."""
+    rows, h, d = 1500, 2, 64
+    q, k, v, _ = inputs(1, rows, h, h, d, d, dtype, seed=12)
+    g = rates(h)
+    cu = torch.tensor([0, 700, 701, 1400], device="cuda", dtype=torch.int32)
+    first = torch.randn(3, h, d, d, device="cuda")
+
+    def call(c):
+        with torch.no_grad():
+            return trnfft.decay_attention(q, k, v, g, initial_state=first, cu_seqlens=c, return_state=True)
+
+    call(cu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, s = call(cu)
+    for ends in ([0, 700, 701, 1400], [0, 3, 3, 10], [0, 0, 1500, 1500], [5, 64, 128, 1000]):
+        cu.copy_(torch.tensor(ends, dtype=torch.int32))
+        graph.replay()
+        wo, ws = call(torch.tensor(ends, device="cuda"))
+        assert torch.equal(o, wo) and torch.equal(s, ws), ends
+
+
+def test_two_streams_and_inference_mode():
+    """Calls that run at once, each with workspaces of its own; states made in inference mode."""
+    g = rates(4)
+    sets = [inputs(1, 6000, 4, 4, 64, 64, t, seed=13)[:3] for t in DTYPES]
+    want = [trnfft.decay_attention(*x, g, return_state=True) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[] for _ in sets]
+    for _ in range(5):
+        for s, x, keep in zip(streams, sets, got):
+            with torch.cuda.stream(s):
+                keep.append(trnfft.decay_attention(*x, g, return_state=True))
+    torch.cuda.synchronize()
+    for keep, w in zip(got, want):
+        assert all(torch.equal(o, w[0]) and torch.equal(s, w[1]) for o, s in keep)
+    with torch.inference_mode():
+        q, k, v = (x[:, -1] for x in sets[0])
+        state = torch.zeros(1, 4, 64, 64, device="cuda")
+        o, new = trnfft.decay_attention_step(q, k, v, g, state)
+    assert new is state and bool(torch.isfinite(o).all()) and float(state.abs().max()) > 0
 
 
 def test_packed_of_no_sequence():
