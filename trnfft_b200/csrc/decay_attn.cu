@@ -59,7 +59,8 @@ int64_t plan_decay_attention(ElemType t, DecayArgs& a) {
   const long long total = (a.tokens + chunk - 1) / chunk;  // chunks, of one dense or of all packed sequences
   int wide = 0;
   for (int i = 0; i < a.roles; ++i) wide = max(wide, max(a.role[i].wk, a.role[i].wv));
-  const long long slots = (long long)kSms * (wide <= 64 ? 2 : 1), walks = (long long)a.heads * max(a.roles, 1);
+  const long long slots = (long long)kSms * (wide <= 64 && t != kBF16 ? 2 : 1),  // blocks at a time
+                  walks = (long long)a.heads * max(a.roles, 1);
   // packed: how the rows fall on the sequences is on the device; take the longest for four times the mean
   const long long longest = a.cu ? (a.nseq ? std::min(total, 4 * total / a.nseq + 1) : 0) : total;
   auto units = [&](long long s) { return a.cu ? total / s + a.nseq : a.nseq * ((total + s - 1) / s); };

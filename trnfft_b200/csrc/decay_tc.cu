@@ -57,8 +57,9 @@ struct Shape {
   static constexpr int kQ = 0, kK = kTile, kV = 2 * kTile, kMid = 3 * kTile, kLo = 4 * kTile;
   static constexpr int kSHi = 5 * kTile, kSLo = kSHi + kState, kTable = kSLo + kState;
   static constexpr int kSmem = kTable + (int)sizeof(float) * 2 * 132 + 12 * 8 + 64;
-  // TMEM columns: P (also in two bfloat16 parts), O, X, E.  With D = 64, E shares X's, so that two
-  // blocks fit on an SM; X is then read before E is issued.
+  // TMEM columns: P (also in two bfloat16 parts), O, X, E.  With D = 64, E shares X's (256 columns
+  // in all); X is then read before E is issued.  (80 registers a thread, for two blocks on an SM, spill:
+  // 8 x 4096 tokens of 16 heads of 64 take 177 us with two blocks, 153 us with one.)
   static constexpr int kP = 0, kO = 128, kX = 128 + D, kE = D == 64 ? kX : kX + D;
   static constexpr int kColumns = D == 64 ? 256 : 512;
   static constexpr bool kShared = D == 64;
@@ -202,7 +203,7 @@ __device__ __forceinline__ void tma_prefetch(const CUtensorMap* map, int x, int 
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, 1)
     k_decay_tc(const __grid_constant__ DecayArgs a, const __grid_constant__ Maps maps, int pass) {
   using S = Shape<D>;
   using chunk::kCarried;
