@@ -517,3 +517,26 @@ def test_offsets_past_32_bits():
     assert torch.equal(trnfft.decay_attention(y, k, v, rates(1)), want)
     y.copy_(v)
     assert torch.equal(trnfft.decay_attention(q, k, y, rates(1)), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [(1, 1500, 2, 1, 64, 64), (2, 300, 2, 2, 128, 128), (2, 257, 4, 2, 40, 72), (1, 4096, 1, 1, 33, 30)])
+def test_sixteen_bit_results_lose_their_own_rounding_alone(size, dtype):
+    """o and the gradients are as far from 64 bits as those rounded to the type are.
+
+    P and C enter the products in two parts (2^-16 of them at worst) and sums are of 32 bits, so an error
+    of some 2^-16 of the result joins the rounding's, which is at least 2^-13 of it in the mean: less than
+    1 % more in the root of the sum of squares.  P and C in the type's own 11 bits would give 41 % more."""
+    b, t, h, hk, dk, dv = size
+    q, k, v, do = inputs(*size, dtype, seed=20)
+    g = rates(h)
+    first = torch.randn(b, h, dk, dv, device="cuda")
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    o = trnfft.decay_attention(q, k, v, g, initial_state=first)
+    got = (o, *torch.autograd.grad(o, leaves, do))
+    xs = [x.detach().double().requires_grad_() for x in leaves]
+    wo, _ = decay_ref(*xs, g, dk ** -0.5, first)
+    for name, x, w in zip(("o", "dq", "dk", "dv"), got, (wo, *torch.autograd.grad(wo, xs, do.double()))):
+        w = w.detach()
+        rounding = float((w.to(dtype).double() - w).norm())
+        assert float((x.detach().double() - w).norm()) < 1.02 * rounding, name

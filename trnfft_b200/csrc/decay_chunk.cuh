@@ -12,16 +12,16 @@
 //
 // Precision.  float32 operands are split in two TF32 parts each and multiplied
 // as hi hi + hi lo + lo hi (2^-22).  16-bit operands are exact in TF32 (and
-// q . k runs on their own type); P and C are rounded to TF32 where they are
-// multiplied (2^-12, a sixteenth of a float16 step or less), and the scaled k,
-// which the state accumulates, is split in two parts.  The tensor core
+// q . k runs on their own type); P, C and the scaled k are multiplied in two
+// parts (P and C: the parts cut off, 2^-20; one part, rounded, would lose
+// 2^-11, as much as the rounding of a float16 o).  The tensor core
 // truncates as it accumulates, so C never is an accumulator over chunks: a
 // chunk's sum starts from 0 and is added to the scaled C in round-to-nearest,
 // with g^n as the sum of two float32.
 //
-// Bound by instruction issue (59 % of the slots; tensor pipe 36 %): 112501
-// tokens of 8 heads of 64 x 64 in float16 take 488 us in segments, a packed
-// float32 call of 2517 rows 73 us.
+// Bound by instruction issue: 112501 tokens of 8 heads of 64 x 64 in float16
+// take 543 us in segments (501 us with one part of P and C), a packed float32
+// call of 2517 rows 71 us.
 #pragma once
 
 #include <type_traits>
@@ -81,6 +81,13 @@ struct Frag {
     } else {
       p[0][i] = tf32(x);
     }
+  }
+  // Both parts cut off, in three instructions: for products with a factor that is exact, where no
+  // product of two second parts is left out.
+  __device__ __forceinline__ void cut(int i, float x) {
+    static_assert(PARTS == 2, "two parts");
+    p[0][i] = __float_as_uint(x) & 0xffffe000u;
+    p[1][i] = __float_as_uint(x - __uint_as_float(p[0][i])) & 0xffffe000u;
   }
   // a value that TF32 holds exactly
   __device__ __forceinline__ void exact(int i, float x) {
@@ -380,16 +387,14 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
     for (int j = 0; j < S::kSTiles; ++j)
 #pragma unroll
       for (int e = 0; e < 4; e += 2) {
-        float2 x = make_float2(st[j][e], st[j][e + 1]);
-        if (!S::kSplit) x = make_float2(__uint_as_float(tf32(x.x)), __uint_as_float(tf32(x.y)));
-        *reinterpret_cast<float2*>(state + (sr + g + (e >> 1) * 8) * PS + sc + j * 8 + 2 * t) = x;
+        *reinterpret_cast<float2*>(state + (sr + g + (e >> 1) * 8) * PS + sc + j * 8 + 2 * t) =
+            make_float2(st[j][e], st[j][e + 1]);
       }
   };
   if (want_o) put_state();
 
   // rows of P and o: two of the warps that share a scheduler have 5 blocks of 16 keys together
   const int mi = warp < 4 ? warp : 7 - warp, oc = warp / 4 * (DV / 2);
-  constexpr int PARTS = S::kSplit ? 2 : 1;
   // Weights a g^d of this thread's places in a block of 8 keys, d tokens from the key to the row: in the
   // row's own block, in the one before, and (as products with cf) in those before that.
   const float own0 = R.a * dec[max(g - 2 * t, 0)], own1 = R.a * dec[max(g - 2 * t - 1, 0)];
@@ -485,9 +490,9 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
             const float* sp = state + (kb * 16 + half * 8 + 2 * t) * PS + oc + g;
 #pragma unroll
             for (int j = 0; j < S::kOTiles; ++j) {
-              Frag<2, 1> fb;
-              fb.exact(0, sp[j * 8]);
-              fb.exact(1, sp[PS + j * 8]);
+              Frag<2, 2> fb;
+              fb.cut(0, sp[j * 8]);
+              fb.cut(1, sp[PS + j * 8]);
               mma_parts(acc[j], fa, fb);
             }
           }
@@ -531,17 +536,19 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
             near0 *= g8;
             near1 *= g8;
           }
-          Frag<4, PARTS> fp;
+          Frag<4, 2> fp;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const bool behind = (n == 2 * mi + 1 && e < 2) || (n >= 2 * mi && (e >> 1) == n - 2 * mi && 2 * t + (e & 1) > g);
             // C layout (row, 2t + e&1) to A layout (row, slot t + 4 (e&1)): key 2t + s sits in slot t + 4 s
-            fp.set((e >> 1) + (e & 1) * 2, behind ? 0.f : pr[n][e] * w[e]);
+            const float x = behind ? 0.f : pr[n][e] * w[e];
+            if constexpr (S::kSplit) fp.set((e >> 1) + (e & 1) * 2, x);
+            else fp.cut((e >> 1) + (e & 1) * 2, x);
           }
           if constexpr (S::kSplit)
             mma_rows_apart<S::kOTiles, PV>(acc, acc_rest, fp, sv + n * 8 * PV + oc);
           else
-            mma_rows<T, S::kOTiles, PARTS, PV>(acc, fp, sv + n * 8 * PV + oc);
+            mma_rows<T, S::kOTiles, 2, PV>(acc, fp, sv + n * 8 * PV + oc);
         }
       if constexpr (S::kSplit) {
 #pragma unroll
