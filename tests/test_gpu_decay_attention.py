@@ -540,3 +540,46 @@ def test_sixteen_bit_results_lose_their_own_rounding_alone(size, dtype):
         w = w.detach()
         rounding = float((w.to(dtype).double() - w).norm())
         assert float((x.detach().double() - w).norm()) < 1.02 * rounding, name
+
+
+def same_infinities(got, want, rel, what):
+    """Infinite where the 64-bit form is, with its sign; near it elsewhere; nowhere NaN."""
+    got, inf = got.detach().double(), want.isinf()
+    assert not bool(want.isnan().any()), "the case has no NaN"
+    assert torch.equal(got.isinf(), inf) and not bool(got.isnan().any()), what
+    assert torch.equal(got[inf], want[inf]), what
+    assert float((got[~inf] - want[~inf]).norm()) <= rel * float(want[~inf].norm()), what
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [33, 40, 64, 128])
+@pytest.mark.parametrize("t", [1, 200, 3000])
+def test_infinite_states_stay_infinite(dtype, d, t):
+    """An infinite element of a state, or one that an infinite key makes, stays infinite however it decays."""
+    q, k, v, do = inputs(1, t, 3, 3, d, d, dtype, seed=25)
+    g = torch.tensor([-0.1, 0.0, -60.0]).cuda()
+    rel = {torch.float32: 1e-5, torch.bfloat16: 5e-3, torch.float16: 1e-3}[dtype]
+    first = torch.randn(1, 3, d, d, device="cuda")
+    first[0, :, 1, 2] = math.inf
+    first[0, :, 4, 0] = -math.inf
+    o, s = trnfft.decay_attention(q, k, v, g, initial_state=first, return_state=True)
+    want, ws = decay_ref(q, k, v, g, d ** -0.5, first)
+    same_infinities(s, ws, 1e-5, "state of an infinite state")
+    same_infinities(o, want, rel, "o of an infinite state")
+    state = first.clone()
+    o1, _ = trnfft.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state)
+    w1, ws1 = decay_ref(q[:, :1], k[:, :1], v[:, :1], g, d ** -0.5, first)
+    same_infinities(state, ws1, 1e-5, "state of a step")
+    same_infinities(o1, w1[:, 0], rel, "o of a step")
+    k2 = k.clone()
+    k2[0, t // 2, 0, 3], k2[0, t // 2, 1:, 5] = math.inf, -math.inf
+    o, s = trnfft.decay_attention(q, k2, v, g, return_state=True)
+    want, ws = decay_ref(q, k2, v, g, d ** -0.5)
+    same_infinities(s, ws, 1e-5, "state of an infinite key")
+    same_infinities(o, want, rel, "o of an infinite key")
+    one = torch.zeros(1, 3, d, d, device="cuda", requires_grad=True)
+    dlast = torch.randn_like(one)
+    dlast[0, :, 2, 3] = math.inf
+    _, s = trnfft.decay_attention(q, k, v, g, initial_state=one, return_state=True)
+    (di,) = torch.autograd.grad(s, one, dlast)
+    same_infinities(di, dlast.double() * torch.exp(g.double() * t).clamp_min(1e-300)[:, None, None], 1e-5, "gradient of the state")

@@ -138,6 +138,9 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     Rows of no sequence get zeros.  The values stay on the device and are not checked: of
     values that are not ascending or not in range, no output is defined.
 
+    A NaN or an infinite value in an operand reaches the results that its sums lead to and no
+    others; an infinite state stays infinite however it decays (but NaN under log_decay -inf).
+
     Differentiable once in q, k, v and initial_state, from o and from the state.
     """
     _check_heads("decay_attention", q, k, v, log_decay, 4)

@@ -69,7 +69,7 @@ struct DecayArgs {
   int segs;
   int units;
   int split;
-  int* flags;  // (role, unit, head): blocks that the tensor-core kernel leaves to the other one, or null
+  int* flags;  // (role, unit, head): blocks that the tensor-core kernel leaves to the other one's walk with care, or null
 };
 
 constexpr int padded_width(int w) { return w <= 32 ? 32 : (w <= 64 ? 64 : 128); }

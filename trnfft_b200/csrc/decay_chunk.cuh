@@ -17,7 +17,7 @@
 // 2^-11, as much as the rounding of a float16 o).  The tensor core
 // truncates as it accumulates, so C never is an accumulator over chunks: a
 // chunk's sum starts from 0 and is added to the scaled C in round-to-nearest,
-// with g^n as the sum of two float32.
+// with g^n as the sum of two float32 (decay_state.cuh).
 //
 // Bound by instruction issue: 112501 tokens of 8 heads of 64 x 64 in float16
 // take 543 us in segments (501 us with one part of P and C), a packed float32
@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "decay_attn.h"
+#include "decay_state.cuh"
 #include "elem.cuh"
 #include "tma.cuh"
 
@@ -200,11 +201,12 @@ struct Shape {
   static constexpr int kPK = pitch<T>(DK), kPV = pitch<T>(DV), kPS = DV + 4;
   static constexpr int kTile = kC * (2 * kPK + kPV) * sizeof(T);  // q, k, v of one chunk
   static constexpr int kState = DK * kPS * 4;
-  static constexpr int kTable = 2 * (kC + 1) * 4 + 24;
+  static constexpr int kTable = 3 * (kC + 1) * 4 + 24;
   static constexpr int kStages = 2 * kTile + kState + kTable <= 113 * 1024 || sizeof(T) == 2 ? 2 : 1;
   static constexpr int kSmem = kStages * kTile + kState + kTable;
   static constexpr int kBlocks = kSmem <= 113 * 1024 && DK * DV <= 64 * 64 ? 2 : 1;  // per SM
   static_assert(kSmem <= 227 * 1024, "shared memory");
+  static_assert(2 * DK * DV * 4 <= kStages * kTile + kState, "walk_with_care keeps two states");
   // state: warps tile DK in blocks of 16 rows, the rest of them the columns
   static constexpr int kSRows = DK / 16 < 8 ? DK / 16 : 8, kSCols = 8 / kSRows;
   static constexpr int kSTiles = DV / 8 / kSCols;          // 8-column tiles of a warp
@@ -298,13 +300,96 @@ __device__ __forceinline__ Segment find_segment(const DecayArgs& a, int unit) {
 // outputs from the states carried into them.
 enum Pass { kWhole, kLocal, kCarried };
 
+// The start of a pass over a segment: its (sequence, head)'s place in the tensors.
+struct Place {
+  long long row0;   // row i of the segment is token row0 + i, or row0 - i from the sequence's end
+  long long batch, sbase;
+  float* seg_state;
+  __device__ __forceinline__ Place(const DecayArgs& a, const DecayRole& R, const Segment& seg, int unit, int h) {
+    row0 = seg.start + (R.back ? seg.total - 1 - seg.first : seg.first);
+    batch = a.cu ? 0 : seg.seq;
+    sbase = ((long long)seg.seq * a.heads + h) * R.wk * R.wv;
+    seg_state = R.seg ? R.seg + ((long long)unit * a.heads + h) * R.wk * R.wv : nullptr;
+  }
+};
+
+// The same segment token by token, one product at a time, where the walk's states do not end finite.  In
+// the walk an infinite factor in two parts makes NaN of sums that are infinite, and keys behind a row
+// have weight 0 in P, but 0 times an infinite or NaN value is NaN.  Here, with A_t = sum_{s<=t} g^{t-s}
+// k_s v_s^T from 0 and B_t = g^{t+1-back} C, o_t = a q_t A_t + r q_t B_t and C' = g^n C + c g^back A.
+template <typename T>
+__device__ __forceinline__ void walk_with_care(const DecayArgs& a, const DecayRole& R, int pass, const Segment& seg, const DecayFactor& factor,
+                                            float* sm) {
+  const int h = blockIdx.x % a.heads, unit = blockIdx.x / a.heads, tid = threadIdx.x;
+  const Place at(a, R, seg, unit, h);
+  const T* q = static_cast<const T*>(R.q) + at.batch * R.qs[0] + (long long)(h / R.qdiv) * R.qs[2];
+  const T* k = static_cast<const T*>(R.k) + at.batch * R.ks[0] + (long long)(h / R.kdiv) * R.ks[2];
+  const T* v = static_cast<const T*>(R.v) + at.batch * R.vs[0] + (long long)(h / R.vdiv) * R.vs[2];
+  const bool want_o = R.o && pass != kLocal;
+  const int size = R.wk * R.wv;
+  float *A = sm, *B = A + size;
+  __shared__ float red[kThreads];
+  const DecayFactor f = factor;
+  // a thread has one column and every `step`-th row
+  int columns = 1;
+  while (columns < R.wv) columns *= 2;
+  const int col = tid % columns, step = kThreads / columns;
+  const bool mine = col < R.wv;
+  __syncthreads();
+#pragma unroll 1
+  for (int d = tid / columns; mine && d < R.wk; d += step) {
+    A[d * R.wv + col] = 0.f;
+    float x = 0.f;
+    if (pass == kCarried) x = at.seg_state[d * R.wv + col];
+    if (pass == kWhole && R.first) x = R.first[at.sbase + d * R.first_sk + col * R.first_sv];
+    B[d * R.wv + col] = x;
+  }
+#pragma unroll 1
+  for (long long i = 0; i < seg.len; ++i) {
+    const long long token = R.back ? at.row0 - i : at.row0 + i;
+    float x = 0.f, y = 0.f;
+    const float vc = mine ? to_f32(v[token * R.vs[1] + col]) : 0.f;
+#pragma unroll 1
+    for (int d = tid / columns; mine && d < R.wk; d += step) {
+      float &Ad = A[d * R.wv + col], &Bd = B[d * R.wv + col];
+      const float b = Bd, next = f.step(b, 0.f);
+      Ad = f.step(Ad, to_f32(k[token * R.ks[1] + d]) * vc);
+      Bd = next;
+      if (want_o) {
+        const float qd = to_f32(q[token * R.qs[1] + d]);
+        x = fmaf(qd, Ad, x);
+        y = fmaf(qd, R.back ? b : next, y);
+      }
+    }
+    if (!want_o) continue;
+    red[tid] = R.a * x + R.r * y;
+    __syncthreads();
+    if (tid < R.wv) {
+      float o = 0.f;
+#pragma unroll 1
+      for (int j = 0; j < step; ++j) o += red[j * columns + tid];
+      const long long to = at.batch * R.os[0] + (long long)h * R.os[2] + token * R.os[1] + tid;
+      if (R.o_f32) static_cast<float*>(R.o)[to] = o;
+      else static_cast<T*>(R.o)[to] = from_f32<T>(o);
+    }
+    __syncthreads();
+  }
+  float* to = pass == kLocal ? at.seg_state : (pass == kWhole && R.last ? R.last + at.sbase : nullptr);
+  if (!to) return;
+#pragma unroll 1
+  for (int d = tid / columns; mine && d < R.wk; d += step) {
+    const float s = A[d * R.wv + col];
+    to[d * R.wv + col] = fmaf(R.c, R.back ? f.step(s, 0.f) : s, B[d * R.wv + col]);
+  }
+}
+
 template <typename T, int DK, int DV>
 __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int pass, unsigned char* sm) {
   using S = Shape<T, DK, DV>;
   constexpr int PK = S::kPK, PV = S::kPV, PS = S::kPS, STAGES = S::kStages;
   float* state = reinterpret_cast<float*>(sm + STAGES * S::kTile);
-  float* dec = state + DK * PS;      // g^n, n <= 64, and what float32 loses of it
-  float* dec_lo = dec + kC + 1;
+  float* dec = state + DK * PS;  // g^n, n <= 64, and the same as factors of a state
+  DecayFactor* factor = reinterpret_cast<DecayFactor*>(dec + kC + 1);
   __shared__ Segment seg_shared;
 
   const int h = blockIdx.x % a.heads, unit = blockIdx.x / a.heads;
@@ -331,11 +416,11 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
     if (lane == 0) seg_shared = s;
   }
   {
-    const double ld = a.log_decay[h];
+    const float ld = a.log_decay[h];
     for (int n = threadIdx.x; n <= kC; n += kThreads) {
-      const double x = n ? exp(ld * n) : 1.0;
+      const double x = n ? exp((double)ld * n) : 1.0;
       dec[n] = (float)x;
-      dec_lo[n] = x - (double)(float)x == x - (double)(float)x ? (float)(x - (double)(float)x) : 0.f;
+      factor[n] = DecayFactor(x, ld);
     }
   }
   __syncthreads();
@@ -343,15 +428,13 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
   if (seg.seq < 0) return;
   const int back = R.back, len = (int)seg.len;
   const bool want_o = R.o && pass != kLocal;
-  // row i of the segment is token row0 + i, or row0 - i from the sequence's end
-  const long long row0 = seg.start + (back ? seg.total - 1 - seg.first : seg.first);
-  const long long batch = a.cu ? 0 : seg.seq;
+  const Place place(a, R, seg, unit, h);
+  const long long row0 = place.row0, batch = place.batch, sbase = place.sbase;
   const T* q = static_cast<const T*>(R.q) + batch * R.qs[0] + (long long)(h / R.qdiv) * R.qs[2] + row0 * R.qs[1];
   const T* k = static_cast<const T*>(R.k) + batch * R.ks[0] + (long long)(h / R.kdiv) * R.ks[2] + row0 * R.ks[1];
   const T* v = static_cast<const T*>(R.v) + batch * R.vs[0] + (long long)(h / R.vdiv) * R.vs[2] + row0 * R.vs[1];
   const long long obase = batch * R.os[0] + (long long)h * R.os[2] + row0 * R.os[1];
-  const long long sbase = ((long long)seg.seq * a.heads + h) * R.wk * R.wv;
-  float* seg_state = R.seg ? R.seg + ((long long)unit * a.heads + h) * R.wk * R.wv : nullptr;
+  float* seg_state = place.seg_state;
   // a kLocal pass of a sequence's last segment serves its final state alone
   if (pass == kLocal && !R.last && seg.first + seg.len >= seg.total) return;
 
@@ -364,12 +447,12 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
     load_rows<T, DV, PV>(dst + 2 * kC * PK, v + skip * R.vs[1], R.vs[1], rows, R.wv, back, R.wide & 4);
     cp_commit();
   };
-  const int chunks = (len + kC - 1) / kC;
-  if (chunks > 0) load(0, 0);
+  const int chunks = a.flags ? 0 : (len + kC - 1) / kC;  // (what is left to this kernel is walked with care)
 
   // the state: rows sr + g (+ 8), columns sc + 8 j + 2 t (+ 1)
   const int sr = warp % S::kSRows * 16, sc = warp / S::kSRows * (S::kSTiles * 8);
   float st[S::kSTiles][4];
+  if (chunks > 0) load(0, 0);
   {
     const float* from = pass == kCarried ? seg_state : (pass == kWhole ? R.first : nullptr);
     const long long sk = pass == kCarried ? R.wv : R.first_sk, sv = pass == kCarried ? 1 : R.first_sv;
@@ -556,38 +639,6 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[j][e] += acc_rest[j][e];
       }
-      // Keys behind a row have weight 0 in P, but 0 times an infinite or NaN value is NaN: where a
-      // result is not finite, its rows are taken again from the keys before them alone.
-      float bad = 0.f;
-#pragma unroll
-      for (int j = 0; j < S::kOTiles; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bad = fmaf(acc[j][e], 0.f, bad);
-      if (__any_sync(~0u, bad != 0.f)) {
-        for (int r = 0; r < 16 && mi * 16 + r < rows; ++r) {
-          const int i = mi * 16 + r;
-          const T* qr = sq + i * PK;
-          for (int c0 = oc; c0 < min(oc + DV / 2, R.wv); c0 += 32) {
-            const int col = c0 + lane;
-            const bool in = col < min(oc + DV / 2, R.wv);
-            float x = 0.f;
-            for (int d = 0; d < R.wk; ++d) x = fmaf(to_f32(qr[d]), in ? state[d * PS + col] : 0.f, x);
-            x *= R.r * dec[i + 1 - back];
-            for (int j = 0; j <= i; ++j) {
-              float w = 0.f;
-              for (int d = lane; d < R.wk; d += 32) w = fmaf(to_f32(qr[d]), to_f32(sk[j * PK + d]), w);
-#pragma unroll
-              for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(~0u, w, o);
-              x = fmaf(w * (R.a * dec[i - j]), in ? to_f32(sv[j * PV + col]) : 0.f, x);
-            }
-            const long long at = obase + (long long)(back ? -(c * kC + i) : c * kC + i) * R.os[1] + col;
-            if (in) {
-              if (R.o_f32) static_cast<float*>(R.o)[at] = x;
-              else static_cast<T*>(R.o)[at] = from_f32<T>(x);
-            }
-          }
-        }
-      } else
 #pragma unroll
       for (int e = 0; e < 4; e += 2) {
         const int i = i0 + (e >> 1) * 8;
@@ -653,11 +704,11 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
           mma_rows<T, S::kSTiles, 2, PV>(d, fa, sv + (kb * 16 + half * 8) * PV + sc);
         }
       }
-      const float hi = dec[rows], lo = dec_lo[rows];
+      const DecayFactor f = factor[rows];
 #pragma unroll
       for (int j = 0; j < S::kSTiles; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) st[j][e] = fmaf(st[j][e], hi, fmaf(st[j][e], lo, d[j][e]));
+        for (int e = 0; e < 4; ++e) st[j][e] = f.step(st[j][e], d[j][e]);
     }
     if (c + 1 < chunks) {
       __syncthreads();  // all have read the stage and the state
@@ -665,6 +716,12 @@ __device__ __forceinline__ void walk(const DecayArgs& a, const DecayRole& R, int
       if (STAGES == 1) load(c + 1, 0);
     }
   }
+  float bad = 0.f;
+#pragma unroll
+  for (int j = 0; j < S::kSTiles; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bad = fmaf(st[j][e], 0.f, bad);
+  if (__syncthreads_or(bad != 0.f || a.flags)) return walk_with_care<T>(a, R, pass, seg_shared, factor[1], reinterpret_cast<float*>(sm));
   float* to = pass == kLocal ? seg_state : (pass == kWhole && R.last ? R.last + sbase : nullptr);
   if (to) {
 #pragma unroll
@@ -723,8 +780,7 @@ static __global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant
   // (units: what the work area holds; only lengths that are not ascending lead past it)
   if (e >= size || first_unit + segs > a.units) return;
   const double ld = a.log_decay[h];
-  const double gd = exp(ld * a.seg_len);
-  const float hi = (float)gd, lo = (float)(gd - (double)hi);
+  const DecayFactor f(exp(ld * a.seg_len), a.log_decay[h]);
   float s = 0.f;
   const long long sbase = ((long long)seq * a.heads + h) * size;
   if (R.first) s = R.first[sbase + e / R.wv * R.first_sk + e % R.wv * R.first_sv];
@@ -738,7 +794,7 @@ static __global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       p[u * step] = s;
-      s = fmaf(s, hi, fmaf(s, lo, x[u]));
+      s = f.step(s, x[u]);
     }
   }
   for (; i < segs; ++i, p += step) {
@@ -746,12 +802,10 @@ static __global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant
     const float x = end && !R.last ? 0.f : *p;
     *p = s;
     if (!end) {
-      s = fmaf(s, hi, fmaf(s, lo, x));
+      s = f.step(s, x);
     } else if (R.last) {
       const long long n = total - (long long)i * a.seg_len;
-      const double gn = n ? exp(ld * n) : 1.0;
-      const float h2 = (float)gn, l2 = (float)(gn - (double)h2);
-      R.last[sbase + e] = fmaf(s, h2, fmaf(s, l2, x));
+      R.last[sbase + e] = DecayFactor(n ? exp(ld * n) : 1.0, a.log_decay[h]).step(s, x);
     }
   }
 }

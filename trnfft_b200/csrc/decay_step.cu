@@ -6,8 +6,10 @@
 // neighbouring columns (1 where rows are not 16-byte aligned) and every
 // 256/lanes-th row, four rows in flight, so that a warp reads whole row runs;
 // the partial sums of o meet in shared memory.  The factor g is kept as the
-// sum of two float32, so that thousands of steps do not drift by its rounding.
+// sum of two float32, so that thousands of steps do not drift by its rounding
+// (decay_state.cuh).
 #include "decay_attn.h"
+#include "decay_state.cuh"
 #include "elem.cuh"
 
 namespace tfb {
@@ -66,8 +68,7 @@ __global__ void __launch_bounds__(kStepThreads) k_decay_step(const __grid_consta
     vj[i] = mine ? to_f32(v[col + i]) : 0.f;
     acc[i] = 0.f;
   }
-  const double gd = exp((double)a.log_decay[h]);
-  const float ghi = (float)gd, glo = (float)(gd - (double)ghi);
+  const DecayFactor decay(exp((double)a.log_decay[h]), a.log_decay[h]);
   __syncthreads();
   if (mine) {
     for (int c0 = row; c0 < a.dk; c0 += U * rows) {
@@ -79,7 +80,7 @@ __global__ void __launch_bounds__(kStepThreads) k_decay_step(const __grid_consta
         Vec<V> y;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          y.x[i] = fmaf(x[u].x[i], ghi, fmaf(x[u].x[i], glo, kc * vj[i]));
+          y.x[i] = decay.step(x[u].x[i], kc * vj[i]);
           acc[i] = fmaf(qc, y.x[i], acc[i]);
         }
         y.store(n + c * a.dv);

@@ -35,9 +35,10 @@
 // buffer (227 KB are full), so their load is not hidden.  Measured: 8500 cycles
 // a chunk; 8 x 4096 tokens, 16 heads (4 for k and v): 202 us, 1.7 TB/s.
 //
-// A masked P is 0, and 0 times an infinite or NaN value is NaN: blocks whose o
-// is not finite somewhere say so, and the walk of decay_chunk.cuh, which looks
-// at such rows one by one, takes them again.
+// A masked P is 0, and 0 times an infinite or NaN value is NaN; so is an infinite
+// value in parts.  Blocks whose o or last state is not finite somewhere say so,
+// and decay_chunk.cuh takes them again one product at a time; a segment's own
+// state is summed again in place.
 #include <cuda.h>
 
 #include "decay_attn.h"
@@ -56,7 +57,7 @@ struct Shape {
   static constexpr int kTile = kC * D * 2, kState = D * D * 2;
   static constexpr int kQ = 0, kK = kTile, kV = 2 * kTile, kMid = 3 * kTile, kLo = 4 * kTile;
   static constexpr int kSHi = 5 * kTile, kSLo = kSHi + kState, kTable = kSLo + kState;
-  static constexpr int kSmem = kTable + (int)sizeof(float) * 2 * 132 + 12 * 8 + 64;
+  static constexpr int kSmem = kTable + (int)sizeof(float) * 3 * 132 + 12 * 8 + 64;
   // TMEM columns: P (also in two bfloat16 parts), O, X, E.  With D = 64, E shares X's (256 columns
   // in all); X is then read before E is issued.  (80 registers a thread, for two blocks on an SM, spill:
   // 8 x 4096 tokens of 16 heads of 64 take 177 us with two blocks, 153 us with one.)
@@ -211,8 +212,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   using chunk::kWhole;
   extern __shared__ __align__(1024) unsigned char sm[];
   float* dec = reinterpret_cast<float*>(sm + S::kTable);
-  float* dec_lo = dec + 132;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(dec_lo + 132);
+  DecayFactor* factor = reinterpret_cast<DecayFactor*>(dec + 132);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(factor + 132);
   chunk::Segment* seg_shared = reinterpret_cast<chunk::Segment*>(bars + 12);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seg_shared + 1);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -239,11 +240,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) *seg_shared = s;
   }
   {
-    const double ld = a.log_decay[h];
+    const float ld = a.log_decay[h];
     for (int n = threadIdx.x; n <= kC; n += kThreads) {
-      const double x = n ? exp(ld * n) : 1.0, rest = x - (double)(float)x;
+      const double x = n ? exp((double)ld * n) : 1.0;
       dec[n] = (float)x;
-      dec_lo[n] = rest == rest ? (float)rest : 0.f;
+      factor[n] = DecayFactor(x, ld);
     }
   }
   if (threadIdx.x == 0) {
@@ -576,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!wait_warp(&bars[kKV], ph, gave_up)) break;
       fence_after();
-      const float hi = dec[rows], lo = dec_lo[rows];
+      const DecayFactor f = factor[rows];
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < D / 2; j += 32) {
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld32(v, tmem + S::kE + c0 + j + lanes);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) st[j + e] = fmaf(st[j + e], hi, fmaf(st[j + e], lo, __uint_as_float(v[e])));
+        for (int e = 0; e < 32; ++e) st[j + e] = f.step(st[j + e], __uint_as_float(v[e]));
       }
       if (c + 1 < chunks) {
         if (want_o) {
@@ -596,13 +597,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (strange) *odd = 1;
     float* to = pass == kLocal ? seg_state : (pass == kWhole && R.last ? R.last + sbase : nullptr);
     if (to && row < R.wk) {
+      float bad = 0.f;
 #pragma unroll
       for (int j = 0; j < D / 2; ++j)
-        if (c0 + j < R.wv) to[row * R.wv + c0 + j] = st[j];
+        if (c0 + j < R.wv) {
+          to[row * R.wv + c0 + j] = st[j];
+          bad = fmaf(st[j], 0.f, bad);
+        }
+      if (bad != 0.f) {
+        strange = true;
+        if (pass == kLocal) {  // here, from the operands themselves, one product at a time
+          const __nv_bfloat16* kh = static_cast<const __nv_bfloat16*>(R.k) + batch * R.ks[0] + (long long)(h / R.kdiv) * R.ks[2];
+          const __nv_bfloat16* vh = static_cast<const __nv_bfloat16*>(R.v) + batch * R.vs[0] + (long long)(h / R.vdiv) * R.vs[2];
+#pragma unroll 1
+          for (int j = 0; j < D / 2 && c0 + j < R.wv; j += 8) {  // (widths are multiples of 8)
+            float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int c = 0; c < chunks; ++c) {
+              const int rows = min(kC, len - c * kC);
+              const long long token = first_token(c) + (back ? kC - rows : 0);
+              float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+              for (int i = 0; i < rows; ++i) {
+                const float w = dec[back ? i + 1 : rows - 1 - i], x = to_f32(kh[(token + i) * R.ks[1] + row]);
+                const uint4 raw = *reinterpret_cast<const uint4*>(vh + (token + i) * R.vs[1] + c0 + j);
+                const uint32_t two[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const float y = e % 2 ? high_f32(two[e / 2]) : low_f32(two[e / 2]);
+                  sum[e] = fmaf(R.c * (finite(x) && finite(y) ? w : above_zero(w, a.log_decay[h])) * x, y, sum[e]);
+                }
+              }
+#pragma unroll
+              for (int e = 0; e < 8; ++e) s[e] = factor[rows].step(s[e], sum[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) to[row * R.wv + c0 + j + e] = s[e];
+          }
+        }
+      }
     }
+    if (strange) *odd = 1;
   }
   fence_before();
   __syncthreads();
