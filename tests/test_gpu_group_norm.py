@@ -212,3 +212,43 @@ def test_offsets_past_32_bits():
     y = trnfft.group_norm(x, 2)
     near(y[-1:], norm_ref(x[-1:].double(), 2, None, None, 1e-5, None), torch.bfloat16, "last row")
     assert float(y[:-1].abs().max()) == 0
+
+
+@pytest.mark.parametrize("shape,groups", [
+    ((64, 128), 1), ((64, 256), 1), ((64, 512), 1), ((40, 4096), 8), ((3, 20, 12), 1),  # in registers
+    ((300, 30, 40), 2), ((200, 10, 1024), 1), ((5, 3, 8192), 2),                        # whole samples
+    ((2, 300, 1024), 1), ((1, 5000, 1024), 4), ((2, 20000, 36), 3),                     # samples in parts
+])
+@pytest.mark.parametrize("what", ["value", "channel", "row"])
+def test_statistics_with_one_far_start(shape, groups, what):
+    """The first value, channel or row of a group far from the others: the sums of squares that start there
+    lose no more than a few roundings of the variance, which is made of nothing else.
+
+    Its relative error of e moves the result by e / 2.  Estimates of the mean up to 4 deviations off lose
+    17 roundings of 2^-24 at most, and a thread's own rows their number of them, but these only of the part
+    of the variance that is theirs: 2e-6, as for values without a far start."""
+    x = data(shape, torch.float32, seed=4)[0].clone()
+    rows = x.view(shape[0], -1, groups, shape[-1] // groups)
+    {"value": rows[:, 0, :, 0], "channel": rows[..., 0], "row": rows[:, 0]}[what].add_(1000.0)
+    want = norm_ref(x.double(), groups, None, None, 1e-5, None)
+    off = trnfft.group_norm(x, groups).double() - want
+    assert float(off.norm() / want.norm()) < 2e-6
+    x.requires_grad_()
+    dy = data(shape, torch.float32, seed=5)[3]
+    xd = x.detach().double().requires_grad_()
+    (dx,) = torch.autograd.grad(trnfft.group_norm(x, groups), x, dy)
+    (wd,) = torch.autograd.grad(norm_ref(xd, groups, None, None, 1e-5, None), xd, dy.double())
+    assert float((dx.double() - wd).norm() / wd.norm()) < 4e-6
+
+
+def test_far_starts_leave_other_groups_as_they_are():
+    """A group's result depends on its own values alone, to the last bit."""
+    for shape, groups in (((64, 128), 8), ((300, 30, 40), 2), ((2, 5000, 64), 8)):
+        x = data(shape, torch.float32, seed=6)[0]
+        want = trnfft.group_norm(x, groups)
+        y = x.clone().view(shape[0], -1, groups, shape[-1] // groups)
+        y[0, 0, 1, 0] += 1e4
+        got = trnfft.group_norm(y.view(shape), groups).view(y.shape)
+        rest = torch.ones_like(y, dtype=torch.bool)
+        rest[0, :, 1] = False
+        assert torch.equal(got[rest], want.view(y.shape)[rest])
