@@ -252,3 +252,27 @@ def test_far_starts_leave_other_groups_as_they_are():
         rest = torch.ones_like(y, dtype=torch.bool)
         rest[0, :, 1] = False
         assert torch.equal(got[rest], want.view(y.shape)[rest])
+
+
+WIDE = [((2, 3, 30000), 1), ((1, 300, 26000), 26000), ((2, 7, 25700), 5), ((1, 1, 40000), 16), ((3, 40, 25800), 2)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,groups", WIDE)
+@pytest.mark.parametrize("act", ACTS)
+def test_more_channels_than_shared_memory_holds(shape, groups, dtype, act):
+    """The general form, forward and backward: a block's sets of the channels and groups would take more
+    than 200 KB in the forward pass too."""
+    assert 8 * (shape[-1] + groups) > 200 * 1024
+    test_forward_and_gradients(shape, groups, dtype, act)
+
+
+@pytest.mark.parametrize("shape,groups", [((2, 3, 30000), 1), ((1, 5000, 13000), 13000)])
+def test_general_form_with_many_terms_and_a_far_mean(shape, groups):
+    """Sums of thousands of terms by one thread, and a mean twenty times the spread, as exact as the other
+    forms': the mean is kept in more than 32 bits, so what remains is the rounding of a few operations."""
+    assert 8 * (shape[-1] + groups) > 200 * 1024
+    x = data(shape, torch.float32, shift=30.0)[0]
+    want = norm_ref(x.double(), groups, None, None, 1e-5, None)
+    off = trnfft.group_norm(x, groups).double() - want
+    assert float(off.norm() / want.norm()) < 3e-7

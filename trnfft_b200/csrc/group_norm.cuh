@@ -115,12 +115,6 @@ struct Pack {
   }
 };
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
-}
-
 // Two sums over aligned groups of `lanes` threads (a power of two).
 __device__ __forceinline__ void lanes_sum(float& u, float& v, int lanes) {
 #pragma unroll
@@ -134,6 +128,29 @@ __device__ __forceinline__ void lanes_sum(float& u, float& v, int lanes) {
 // Blocks of 256 threads an SM holds with a thread's NV accesses and their parameters in registers.
 constexpr int small_blocks(int nv) { return nv == 1 ? 4 : (nv == 2 ? 3 : 2); }
 constexpr int small_blocks_bwd(int nv) { return nv == 1 ? 3 : (nv == 2 ? 2 : 1); }
+
+// kAny: a thread's elements of a group of w channels, every kNormThreads-th of the rows one after the other.
+struct AnyPlace {
+  long long row;
+  int c, w;
+  __device__ __forceinline__ explicit AnyPlace(int width) : row(threadIdx.x / width), c(threadIdx.x % width), w(width) {}
+  __device__ __forceinline__ void next() {
+    row += kNormThreads / w;
+    c += kNormThreads % w;
+    if (c >= w) c -= w, ++row;
+  }
+};
+
+__device__ __forceinline__ double block_sum(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int i = 0; i < kNormThreads / 32; ++i) v += red[i];
+  return v;
+}
 
 // True in the block that is the last of its sample's `parts` to come here; it sees what all of
 // them wrote before.

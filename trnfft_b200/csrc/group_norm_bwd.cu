@@ -537,67 +537,57 @@ __global__ void __launch_bounds__(kSumCols * kSumRows) k_gn_sum_rows(const float
   }
 }
 
-// Any number of channels: one block per group for dx, one per channel for dw and db.
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  v = warp_sum(v);
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int i = 0; i < kNormThreads / 32; ++i) v += red[i];
-  return v;
-}
-
+// Any number of channels: one block per group for dx, one per channel for dw and db, sums in 64 bits.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kNormThreads) k_gn_any_dx(const __grid_constant__ GroupNormArgs a) {
-  __shared__ float red[kNormThreads / 32];
+  __shared__ double red[kNormThreads / 32];
   const int w = a.channels / a.groups;
-  const float inv = 1.f / (float)(a.spots * w);
+  const double inv = 1.0 / ((double)a.spots * w);
   for (long long id = blockIdx.x; id < a.batch * a.groups; id += gridDim.x) {
     const int g = (int)(id % a.groups);
     const long long base = id / a.groups * a.spots * a.channels + (long long)g * w;
     const float mean = a.mean[id], rstd = a.rstd[id];
-    float su = 0.f, suh = 0.f;
+    double sum = 0.0, sum_h = 0.0;
+    float mu = 0.f, muh = 0.f;
     for (int pass = 0; pass < 2; ++pass) {
       if (pass) {
-        su = block_sum(su, red) * inv;
-        suh = block_sum(suh, red) * inv;
+        mu = (float)(block_sum(sum, red) * inv);
+        muh = (float)(block_sum(sum_h, red) * inv);
       }
-      for (long long r = 0; r < a.spots; ++r)
-        for (int i = threadIdx.x; i < w; i += kNormThreads) {
-          const long long at = base + r * a.channels + i;
-          const int c = g * w + i;
-          const float wc = a.weight ? a.weight[c] : 1.f, h = (to_f32(static_cast<const T*>(a.x)[at]) - mean) * rstd;
-          const float u = to_f32(static_cast<const T*>(a.dy)[at]) * slope<ACT>(fmaf(h, wc, a.bias ? a.bias[c] : 0.f)) * wc;
-          if (pass) {
-            static_cast<T*>(a.y)[at] = from_f32<T>(rstd * (u - su - h * suh));
-          } else {
-            su += u;
-            suh = fmaf(u, h, suh);
-          }
+      for (AnyPlace at(w); at.row < a.spots; at.next()) {
+        const long long i = base + at.row * a.channels + at.c;
+        const int c = g * w + at.c;
+        const float wc = a.weight ? a.weight[c] : 1.f, h = (to_f32(static_cast<const T*>(a.x)[i]) - mean) * rstd;
+        const float u = to_f32(static_cast<const T*>(a.dy)[i]) * slope<ACT>(fmaf(h, wc, a.bias ? a.bias[c] : 0.f)) * wc;
+        if (pass) {
+          static_cast<T*>(a.y)[i] = from_f32<T>(rstd * (u - mu - h * muh));
+        } else {
+          sum += u;
+          sum_h += (double)u * h;
         }
+      }
     }
   }
 }
 
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kNormThreads) k_gn_any_dw(const __grid_constant__ GroupNormArgs a) {
-  __shared__ float red[kNormThreads / 32];
+  __shared__ double red[kNormThreads / 32];
   const int c = blockIdx.x, g = c / (a.channels / a.groups);
   const float wc = a.weight ? a.weight[c] : 1.f, bc = a.bias ? a.bias[c] : 0.f;
-  float sw = 0.f, sb = 0.f;
+  double sw = 0.0, sb = 0.0;
   for (long long i = threadIdx.x; i < a.batch * a.spots; i += kNormThreads) {
     const long long n = i / a.spots * a.groups + g;
     const float h = (to_f32(static_cast<const T*>(a.x)[i * a.channels + c]) - a.mean[n]) * a.rstd[n];
     const float dz = to_f32(static_cast<const T*>(a.dy)[i * a.channels + c]) * slope<ACT>(fmaf(h, wc, bc));
     sb += dz;
-    sw = fmaf(dz, h, sw);
+    sw += (double)dz * h;
   }
   sw = block_sum(sw, red);
   sb = block_sum(sb, red);
   if (threadIdx.x == 0) {
-    if (a.dw) a.dw[c] = sw;
-    if (a.db) a.db[c] = sb;
+    if (a.dw) a.dw[c] = (float)sw;
+    if (a.db) a.db[c] = (float)sb;
   }
 }
 
