@@ -1,6 +1,8 @@
 """Argument checks of the sequence and normalisation operators, without a GPU."""
 
 import ctypes
+import pathlib
+import re
 
 import pytest
 import torch
@@ -168,3 +170,19 @@ def test_layers_have_their_parameters():
     m = ComplexDecayAttention(6, 3, 4)
     assert m.log_decay.shape == (3,) and (m.log_decay < 0).all() and (m.log_decay.diff() > 0).all()
     assert m.initial_state(5).shape == (5, 3, 8, 8)
+
+
+# -- waits that give up ------------------------------------------------------------------------
+
+
+def source(name):
+    return (pathlib.Path(_lib.__file__).parent / "csrc" / name).read_text()
+
+
+def test_roles_of_a_block_meet_at_bounded_waits_alone():
+    """A warp whose wait ran out leaves its loop.  A barrier of a given number of threads inside the loops
+    would wait for it without a limit: the roles of the tensor-core walk meet at bounded waits alone."""
+    text = source("decay_tc.cu")
+    assert not re.search(r"\b(bar|barrier)(\.cta)?\.(sync|red|arrive)\b", text)
+    roles = text[text.index("if (warp > kMmaWarp)"):text.index("tcgen05.dealloc")]
+    assert "__syncthreads" not in roles[:roles.rindex("fence_before();")], "no barrier of the block inside a role"

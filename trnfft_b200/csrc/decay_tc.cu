@@ -33,7 +33,8 @@
 // tensor pipe, its bytes 5700 at 1/148 of the measured bandwidth, the operands,
 // parts and staging in shared memory 6250 at 128 bytes a cycle; k and v have one
 // buffer (227 KB are full), so their load is not hidden.  Measured: 8500 cycles
-// a chunk; 8 x 4096 tokens, 16 heads (4 for k and v): 202 us, 1.7 TB/s.
+// a chunk; 8 x 4096 tokens, 16 heads (4 for k and v): 206-211 us, 1.6 TB/s (2 %
+// of it for a bounded wait, not a barrier, before the state goes where o was).
 //
 // A masked P is 0, and 0 times an infinite or NaN value is NaN; so is an infinite
 // value in parts.  Blocks whose o or last state is not finite somewhere say so,
@@ -57,7 +58,7 @@ struct Shape {
   static constexpr int kTile = kC * D * 2, kState = D * D * 2;
   static constexpr int kQ = 0, kK = kTile, kV = 2 * kTile, kMid = 3 * kTile, kLo = 4 * kTile;
   static constexpr int kSHi = 5 * kTile, kSLo = kSHi + kState, kTable = kSLo + kState;
-  static constexpr int kSmem = kTable + (int)sizeof(float) * 3 * 132 + 12 * 8 + 64;
+  static constexpr int kSmem = kTable + (int)sizeof(float) * 3 * 132 + 14 * 8 + 64;
   // TMEM columns: P (also in two bfloat16 parts), O, X, E.  With D = 64, E shares X's (256 columns
   // in all); X is then read before E is issued.  (80 registers a thread, for two blocks on an SM, spill:
   // 8 x 4096 tokens of 16 heads of 64 take 177 us with two blocks, 153 us with one.)
@@ -74,7 +75,7 @@ struct Maps {
   int used;
 };
 
-enum Bar { kFull, kVFull, kQK, kQS, kPV, kKFree, kKV, kPDone, kKDone, kSReady, kXRead, kBars };
+enum Bar { kFull, kVFull, kQK, kQS, kPV, kKFree, kKV, kDrained, kPDone, kKDone, kSReady, kXRead, kOTaken, kBars };
 
 __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
   uint64_t d = (uint64_t)((addr >> 4) & 0x3FFF);
@@ -110,7 +111,8 @@ __device__ __forceinline__ void arrive(uint64_t* bar) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// A bounded wait; false once any wait of the block has given up.
+// A bounded wait; false once any wait of the block has given up.  Between the roles of a block there is
+// no other kind of barrier, so that all of them come to the end of the kernel.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
   bool ok = false;
   for (int i = 0; i < (1 << 22) && !*gave_up; ++i)
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* dec = reinterpret_cast<float*>(sm + S::kTable);
   DecayFactor* factor = reinterpret_cast<DecayFactor*>(dec + 132);
   uint64_t* bars = reinterpret_cast<uint64_t*>(factor + 132);
-  chunk::Segment* seg_shared = reinterpret_cast<chunk::Segment*>(bars + 12);
+  chunk::Segment* seg_shared = reinterpret_cast<chunk::Segment*>(bars + 14);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(seg_shared + 1);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* odd = reinterpret_cast<int*>(tmem_slot + 2);
@@ -222,6 +224,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const DecayRole& R = a.role[blockIdx.z];
   const int h = blockIdx.x % a.heads, unit = blockIdx.x / a.heads;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const bool want_o = R.o && pass != kLocal;
+  static_assert(kBars <= 14, "barriers");
 
   if (a.cu && unit == a.units) {  // the rows of no sequence
     if (!R.o || pass == kLocal) return;
@@ -249,8 +253,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBars; ++i) {
-      const int count = i == kFull || i == kVFull ? (maps.used ? 1 : kLoaders)
-                                   : (i >= kPDone ? 256 : 1);
+      int count = i == kOTaken ? 8 : (i >= kPDone ? 256 : 1);
+      if (i == kFull || i == kVFull) count = !maps.used ? kLoaders : (i == kFull && want_o ? 2 : 1);
       mbar_init(&bars[i], count);
     }
     *gave_up = 0;
@@ -277,7 +281,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot, base = smem_u32(sm);
-  const bool want_o = R.o && pass != kLocal;
   const long long batch = a.cu ? 0 : seg.seq;
   const int chunks = (len + kC - 1) / kC;
   // token of row 0 of chunk c (backwards it may lie before the sequence), and the rows that belong to it
@@ -291,17 +294,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (warp == kLoadWarp && lane == 0) {
         const CUtensorMap *mq = &maps.m[blockIdx.z][0], *mk = &maps.m[blockIdx.z][1], *mv = &maps.m[blockIdx.z][2];
         const int hq = h / R.qdiv, hk = h / R.kdiv, hv = h / R.vdiv, b = (int)batch;
+        int last = -1, last_v = -1;  // chunks whose loads have been issued
         for (int c = 0; c < chunks; ++c) {
           const int token = (int)first_token(c);
           if (want_o) {
             if (c > 0 && !wait(&bars[kQS], (c - 1) & 1, gave_up)) break;
-            mbar_arrive_expect_tx(&bars[kFull], 2 * S::kTile);
+            mbar_arrive_expect_tx(&bars[kFull], S::kTile);
             for (int x = 0; x < D; x += 64) tma_load(base + S::kQ + x / 64 * kBlockBytes, mq, x, token, hq, b, &bars[kFull]);
           }
-          if (c > 0 && !wait(&bars[kKFree], (c - 1) & 1, gave_up)) break;
-          if (!want_o) mbar_arrive_expect_tx(&bars[kFull], S::kTile);
+          last = c;
+          if (c > 0 && !wait(&bars[kKFree], (c - 1) & 1, gave_up)) {
+            if (want_o) arrive(&bars[kFull]);  // in k's place: q is on its way
+            else --last;
+            break;
+          }
+          mbar_arrive_expect_tx(&bars[kFull], S::kTile);
           for (int x = 0; x < D; x += 64) tma_load(base + S::kK + x / 64 * kBlockBytes, mk, x, token, hk, b, &bars[kFull]);
           if (c > 0 && !wait(&bars[kKV], (c - 1) & 1, gave_up)) break;
+          last_v = c;
           mbar_arrive_expect_tx(&bars[kVFull], S::kTile);
           for (int x = 0; x < D; x += 64) tma_load(base + S::kV + x / 64 * kBlockBytes, mv, x, token, hv, b, &bars[kVFull]);
           if (c + 1 < chunks) {
@@ -310,6 +320,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int x = 0; x < D; x += 64) tma_prefetch(mv, x, next, hv, b);
           }
         }
+        // nothing is on its way to shared memory when the block ends, however the loop did
+        if (last >= 0 && !mbar_wait_bounded(&bars[kFull], last & 1)) *gave_up = 1;
+        if (last_v >= 0 && !mbar_wait_bounded(&bars[kVFull], last_v & 1)) *gave_up = 1;
       }
     } else {
       const int t = threadIdx.x - 32 * kLoadWarp;
@@ -398,6 +411,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         commit(&bars[kKV]);
       }
+      commit(&bars[kDrained]);  // no product reads shared memory or writes TMEM when the block ends
+      if (!mbar_wait_bounded(&bars[kDrained], 0)) *gave_up = 1;
     }
   } else {
     // ---------------- P, k', o and the state
@@ -589,7 +604,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (c + 1 < chunks) {
         if (want_o) {
-          asm volatile("bar.sync 1, 256;" ::: "memory");  // all warps have taken their o from there
+          __syncwarp();
+          if (lane == 0) arrive(&bars[kOTaken]);
+          if (!wait_warp(&bars[kOTaken], ph, gave_up)) break;  // all warps have taken their o from there
           put_state();
         } else {
           fence_before();
