@@ -186,3 +186,12 @@ def test_roles_of_a_block_meet_at_bounded_waits_alone():
     assert not re.search(r"\b(bar|barrier)(\.cta)?\.(sync|red|arrive)\b", text)
     roles = text[text.index("if (warp > kMmaWarp)"):text.index("tcgen05.dealloc")]
     assert "__syncthreads" not in roles[:roles.rindex("fence_before();")], "no barrier of the block inside a role"
+
+
+def test_streams_of_buffers_give_up_with_the_whole_block():
+    """A thread whose wait for a buffer ran out goes through the same barriers as the others, to the end."""
+    for name in ("group_norm.cu", "group_norm_bwd.cu"):
+        text = source(name)
+        waits = re.findall(r"[^\n]*\b(?:rows|samples)\.wait\([^\n]*", text)
+        assert waits and all(w.strip() in ("rows.wait(i);", "samples.wait(i);") for w in waits), "no thread leaves by itself"
+        assert len(re.findall(r"\b(?:rows|samples)\.finish\(\);", text)) == len(waits)

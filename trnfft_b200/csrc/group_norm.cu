@@ -247,7 +247,7 @@ __device__ __forceinline__ void stream_stats(const GroupNormArgs& a, const Group
 #pragma unroll
   for (int v = 0; v < V; ++v) first.x[v] = s[v] = ss[v] = 0.f;
   for (int i = 0; i < rows.count; ++i) {
-    if (!rows.wait(i)) break;
+    rows.wait(i);
     if (col.live) {
       const T* q = reinterpret_cast<const T*>(rows.buffer(i, 0)) + at.slot * a.channels + col.c;
       const int mine = rows.rows_of(i);
@@ -266,6 +266,7 @@ __device__ __forceinline__ void stream_stats(const GroupNormArgs& a, const Group
     }
     rows.release(i);
   }
+  rows.finish();
   if (col.live) {
     const float inv = at.mine ? 1.f / (float)at.mine : 0.f;
     float2* to = red + at.slot * a.channels + col.c;
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
   const float inv = 1.f / ((float)a.spots * (float)(a.channels / a.groups)), inv_mine = at.mine ? 1.f / (float)at.mine : 0.f;
   for (int i = 0; i < samples.count; ++i) {
     const long long n = blockIdx.x + (long long)i * gridDim.x;
-    if (!samples.wait(i)) break;
+    samples.wait(i);
     const T* x = reinterpret_cast<const T*>(samples.buffer(i, 0)) + at.slot * a.channels + col.c;
     if (col.live) {
       Pack<T, V> first;
@@ -415,6 +416,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
     }
     samples.release(i);
   }
+  samples.finish();
 }
 
 // Block = part blockIdx.x % parts of sample blockIdx.x / parts: its groups' sets; the sample's last
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
   }
   T* to = static_cast<T*>(a.y) + base + (long long)at.slot * a.channels + col.c;
   for (int i = 0; i < rows.count; ++i) {
-    if (!rows.wait(i)) break;
+    rows.wait(i);
     if (col.live) {
       const T* q = reinterpret_cast<const T*>(rows.buffer(i, 0)) + at.slot * a.channels + col.c;
       const int mine = rows.rows_of(i);
@@ -509,6 +511,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
     }
     rows.release(i);
   }
+  rows.finish();
 }
 
 // ---------------------------------------------------------------- kAny

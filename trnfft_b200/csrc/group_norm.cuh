@@ -225,6 +225,7 @@ struct RowStream {
   const char* from[N];
   long long row_bytes;
   int rows, per, count;  // rows in all, of a buffer; buffers
+  int gave_up = -1;      // the buffer at which this thread's wait ran out
   __device__ __forceinline__ void issue(int i) {
     const int first = i * per;
     const uint32_t bytes = (uint32_t)(min(per, rows - first) * row_bytes);
@@ -247,11 +248,10 @@ struct RowStream {
     }
     __syncthreads();
   }
-  // Waits for buffer i; true if it came.
-  __device__ __forceinline__ bool wait(int i) {
-    if (mbar_wait_bounded(full + i % kStages, i / kStages & 1)) return true;
-    if (threadIdx.x == 0) atomicExch(&g_dev_status, kStatusWaitTimeout);
-    return false;
+  // Waits for buffer i.  A thread whose wait gives up goes on with whatever the buffer holds, through the
+  // same barriers as the others, and waits no more; finish() says so in the status word.
+  __device__ __forceinline__ void wait(int i) {
+    if (gave_up < 0 && !mbar_wait_bounded(full + i % kStages, i / kStages & 1)) gave_up = i;
   }
   __device__ __forceinline__ const unsigned char* buffer(int i, int tensor) const {
     return buffers + (i % kStages * N + tensor) * kBuffer;
@@ -260,7 +260,14 @@ struct RowStream {
   // All have read buffer i: it may be filled again.
   __device__ __forceinline__ void release(int i) {
     __syncthreads();
-    if (threadIdx.x == 0 && i + kStages < count) issue(i + kStages);
+    if (threadIdx.x == 0 && gave_up < 0 && i + kStages < count) issue(i + kStages);
+  }
+  // After the last buffer: nothing is on its way to shared memory when the block ends.
+  __device__ __forceinline__ void finish() {
+    if (gave_up < 0) return;
+    atomicExch(&g_dev_status, kStatusWaitTimeout);
+    if (threadIdx.x == 0)
+      for (int i = gave_up; i < min(gave_up + kStages, count); ++i) (void)mbar_wait_bounded(full + i % kStages, i / kStages & 1);
   }
 };
 
@@ -273,6 +280,7 @@ struct SampleStream {
   const char* from[N];
   long long bytes;  // of a sample of one tensor
   int count, ring;
+  int gave_up = -1;
   __device__ __forceinline__ void issue(int i) {
     uint64_t* bar = full + i % ring;
     mbar_arrive_expect_tx(bar, (uint32_t)(N * bytes));
@@ -295,17 +303,21 @@ struct SampleStream {
     }
     __syncthreads();
   }
-  __device__ __forceinline__ bool wait(int i) {
-    if (mbar_wait_bounded(full + i % ring, i / ring & 1)) return true;
-    if (threadIdx.x == 0) atomicExch(&g_dev_status, kStatusWaitTimeout);
-    return false;
+  __device__ __forceinline__ void wait(int i) {  // this, release() and finish() as above
+    if (gave_up < 0 && !mbar_wait_bounded(full + i % ring, i / ring & 1)) gave_up = i;
   }
   __device__ __forceinline__ const unsigned char* buffer(int i, int tensor) const {
     return buffers + (i % ring * N + tensor) * bytes;
   }
   __device__ __forceinline__ void release(int i) {
     __syncthreads();
-    if (threadIdx.x == 0 && i + ring < count) issue(i + ring);
+    if (threadIdx.x == 0 && gave_up < 0 && i + ring < count) issue(i + ring);
+  }
+  __device__ __forceinline__ void finish() {
+    if (gave_up < 0) return;
+    atomicExch(&g_dev_status, kStatusWaitTimeout);
+    if (threadIdx.x == 0)
+      for (int i = gave_up; i < min(gave_up + ring, count); ++i) (void)mbar_wait_bounded(full + i % ring, i / ring & 1);
   }
 };
 constexpr int kMaxSampleBuffers = 8;

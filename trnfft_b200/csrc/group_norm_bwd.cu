@@ -220,7 +220,7 @@ __device__ __forceinline__ void stream_sums(const GroupNormArgs& a, const GroupN
     sw[v] = sb[v] = 0.f;
   }
   for (int i = 0; i < rows.count; ++i) {
-    if (!rows.wait(i)) break;
+    rows.wait(i);
     if (col.live) {
       const T* px = reinterpret_cast<const T*>(rows.buffer(i, 0)) + at.slot * a.channels + col.c;
       const T* pd = reinterpret_cast<const T*>(rows.buffer(i, 1)) + at.slot * a.channels + col.c;
@@ -240,6 +240,7 @@ __device__ __forceinline__ void stream_sums(const GroupNormArgs& a, const GroupN
     }
     rows.release(i);
   }
+  rows.finish();
   if (col.live) {
     float2* red = sm.red + at.slot * a.channels + col.c;
 #pragma unroll
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
   const float inv = 1.f / ((float)a.spots * (float)(a.channels / a.groups));
   for (int i = 0; i < samples.count; ++i) {
     const long long n = blockIdx.x + (long long)i * gridDim.x;
-    if (!samples.wait(i)) break;
+    samples.wait(i);
     const T* x = reinterpret_cast<const T*>(samples.buffer(i, 0)) + at.slot * a.channels + col.c;
     const T* dy = reinterpret_cast<const T*>(samples.buffer(i, 1)) + at.slot * a.channels + col.c;
     float mean[V], rstd[V], gain[V];
@@ -406,6 +407,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
     }
     samples.release(i);
   }
+  samples.finish();
   leave_channels(a, p, sm);
 }
 
@@ -484,7 +486,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
   }
   T* to = static_cast<T*>(a.y) + base + (long long)at.slot * a.channels + col.c;
   for (int i = 0; i < rows.count; ++i) {
-    if (!rows.wait(i)) break;
+    rows.wait(i);
     if (col.live) {
       const T* px = reinterpret_cast<const T*>(rows.buffer(i, 0)) + at.slot * a.channels + col.c;
       const T* pd = reinterpret_cast<const T*>(rows.buffer(i, 1)) + at.slot * a.channels + col.c;
@@ -504,6 +506,7 @@ __global__ void __launch_bounds__(kNormThreads, 3)
     }
     rows.release(i);
   }
+  rows.finish();
 }
 
 // dw, db = the sums of the blocks' rows of channel sums.
