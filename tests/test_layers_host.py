@@ -71,6 +71,29 @@ def test_group_norm_refuses():
             trnfft.group_norm(*args, **kw)
 
 
+def test_forward_mode_is_refused():
+    """A tangent would be lost: no kernel carries it.  Without one, an open level of forward mode changes nothing."""
+    fwd = torch.autograd.forward_ad
+    q, k, v, g = qkv()
+    s = torch.zeros(2, 4, 8, 6)
+    x, w = torch.zeros(2, 5, 12), torch.ones(12)
+    calls = [(trnfft.decay_attention, [q, k, v, g], (0, 1, 2, 3)),
+             (lambda q, k, v, g, s: trnfft.decay_attention(q, k, v, g, initial_state=s), [q, k, v, g, s], (4,)),
+             (trnfft.decay_attention_step, [q[:, 0], k[:, 0], v[:, 0], g, s], (0, 1, 2, 3, 4)),
+             (lambda x, w, b: trnfft.group_norm(x, 3, w, b), [x, w, w], (0, 1, 2))]
+    for call, args, places in calls:
+        for i in places:
+            with fwd.dual_level():
+                dual = fwd.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(*args[:i], dual, *args[i + 1:])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(lambda y: call(y, *args[1:]), (args[0],), (torch.ones_like(args[0]),))
+    with fwd.dual_level():
+        with pytest.raises(ValueError, match="fall into"):
+            trnfft.group_norm(x, 5)
+
+
 def test_no_cpu_fallback():
     if torch.cuda.is_available():
         pytest.skip("a CUDA device is visible")

@@ -13,9 +13,10 @@ bfloat16 or float16; states are float32.
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as fwd
 
 from . import _lib
-from ._device import place_layer
+from ._device import place_layer, refuse_tangents
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -141,7 +142,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     A NaN or an infinite value in an operand reaches the results that its sums lead to and no
     others; an infinite state stays infinite however it decays (but NaN under log_decay -inf).
 
-    Differentiable once in q, k, v and initial_state, from o and from the state.
+    Differentiable once in q, k, v and initial_state, from o and from the state; forward-mode tangents are
+    refused.
     """
     _check_heads("decay_attention", q, k, v, log_decay, 4)
     b, t, h, dk = q.shape
@@ -158,6 +160,8 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
     if initial_state is not None and (initial_state.shape != (nseq, h, dk, dv) or initial_state.dtype != torch.float32):
         raise ValueError(f"decay_attention: initial_state must be float32 {(nseq, h, dk, dv)}, got {initial_state.dtype} "
                          f"{tuple(initial_state.shape)}")
+    if fwd._current_level >= 0:
+        refuse_tangents("decay_attention", q, k, v, log_decay, initial_state)
     (q, k, v, log_decay, initial, cu), restore = place_layer("decay_attention", q, k, v, log_decay, initial_state, cu_seqlens)
     q, k, v = _unit_inner(q), _unit_inner(k), _unit_inner(v)
     log_decay = log_decay.detach().float().contiguous()
@@ -193,6 +197,8 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     dv = vs[2]
     if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, log_decay, state)):
         raise ValueError(f"{fn}: has no gradient; use decay_attention, or torch.no_grad()")
+    if fwd._current_level >= 0:
+        refuse_tangents(fn, q, k, v, log_decay, state, new_state)
     one = h * dk * dv
     for s in (state,) if new_state is None else (state, new_state):
         if s.shape != (b, h, dk, dv) or s.dtype != torch.float32 or s.device != state.device:

@@ -11,6 +11,7 @@ device every transform raises (there is no CPU fallback).
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as fwd
 
 from . import _lib
 
@@ -64,6 +65,14 @@ def place_layer(fn: str, *ts: torch.Tensor | None):
         dev = torch.device("cuda", torch.cuda.current_device())
     out = [None if t is None else t.to(device=dev) for t in ts]
     return out, (_same if ts[0].is_cuda else _to_host)
+
+
+def refuse_tangents(fn: str, *ts: torch.Tensor | None):
+    """Raise for operands that carry a forward-mode tangent: a kernel would drop it without a word.
+    To be called where a level of forward-mode differentiation is open (``fwd._current_level >= 0``)."""
+    for t in ts:
+        if t is not None and fwd.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{fn}: has no forward-mode derivative; use torch.autograd.grad or backward")
 
 
 def _same(t: torch.Tensor) -> torch.Tensor:

@@ -5,10 +5,11 @@ from __future__ import annotations
 import functools
 
 import torch
+import torch.autograd.forward_ad as fwd
 
 from . import _lib
 from ._attention import DTYPES, _addr, once
-from ._device import place_layer
+from ._device import place_layer, refuse_tangents
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
@@ -110,12 +111,15 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
     num_groups groups; each group of each sample is normalised by its mean and variance
     over all positions (statistics in float32), then scaled by weight and shifted by bias
     (channels each, optional) and put through the activation: None, "relu", "silu" or
-    "gelu" (z times the normal distribution function, to 1e-7).  Differentiable once in x, weight and bias.
+    "gelu" (z times the normal distribution function, to 1e-7).  Differentiable once in x, weight and bias;
+    forward-mode tangents are refused.
     """
     c = x.shape[-1] if x.dim() else 0
     if not (x.dim() >= 2 and x.dtype in DTYPES and c > 0 and type(num_groups) is int and num_groups > 0 and c % num_groups == 0
             and activation in ACTIVATIONS and eps >= 0 and _fits(weight, c) and _fits(bias, c)):
         num_groups = _refuse(x, num_groups, weight, bias, eps, activation)
+    if fwd._current_level >= 0:
+        refuse_tangents("group_norm", x, weight, bias)
     restore = None
     device = x.get_device()
     if device < 0 or (weight is not None and weight.get_device() != device) or (bias is not None and
