@@ -195,6 +195,17 @@ def test_layers_have_their_parameters():
     assert m.initial_state(5).shape == (5, 3, 8, 8)
 
 
+@pytest.mark.parametrize("heads,width", [(2, 65), (2, 128), (2, 0), (0, 8), (-1, 8)])
+def test_layer_refuses_heads_that_it_cannot_run(heads, width):
+    """When it is made, not at its first call."""
+    with pytest.raises(ValueError, match="width"):
+        ComplexDecayAttention(12, heads, width)
+
+
+def test_widest_layer():
+    assert ComplexDecayAttention(12, 2, 64).initial_state(1).shape == (1, 2, 128, 128)
+
+
 # -- waits that give up ------------------------------------------------------------------------
 
 

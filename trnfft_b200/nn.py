@@ -151,13 +151,16 @@ class ComplexDecayAttention(nn.Module):
     """Mixing along time for complex features (batch, frames, features): decayed linear attention
     between ``ComplexLinear`` projections, each head's output normalised for itself.
 
-    A head of complex width w is a real head of width 2w over [re, im], so scores are
+    A head of complex width w (up to 64) is a real head of width 2w over [re, im], so scores are
     Re(q conj(k)).  ``forward`` runs whole sequences; ``step`` one frame (batch, features) of each
     stream on the state that ``forward(..., return_state=True)`` or ``initial_state`` gives, in
     place.  Head h forgets over 2^(3 + 6h/(heads-1)) frames."""
 
     def __init__(self, features: int, heads: int, head_width: int):
         super().__init__()
+        if heads < 1 or not 1 <= head_width <= 64:
+            raise ValueError("ComplexDecayAttention: needs a head or more, of a complex width from 1 to 64 (real heads are "
+                             f"twice as wide, up to 128), got {heads} of width {head_width}")
         self.heads, self.head_width = heads, head_width
         self.q = ComplexLinear(features, heads * head_width, bias=False)
         self.k = ComplexLinear(features, heads * head_width, bias=False)
