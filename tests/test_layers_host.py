@@ -206,6 +206,17 @@ def test_widest_layer():
     assert ComplexDecayAttention(12, 2, 64).initial_state(1).shape == (1, 2, 128, 128)
 
 
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
+def test_states_are_float32_whatever_the_default_type(default):
+    m = ComplexDecayAttention(6, 3, 4)
+    kept = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        assert m.initial_state(5).dtype == torch.float32
+    finally:
+        torch.set_default_dtype(kept)
+
+
 # -- waits that give up ------------------------------------------------------------------------
 
 

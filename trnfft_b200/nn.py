@@ -181,7 +181,8 @@ class ComplexDecayAttention(nn.Module):
 
     def initial_state(self, batch: int, device=None) -> torch.Tensor:
         w = 2 * self.head_width
-        return torch.zeros(batch, self.heads, w, w, device=self.log_decay.device if device is None else device)
+        return torch.zeros(batch, self.heads, w, w, dtype=torch.float32,
+                           device=self.log_decay.device if device is None else device)
 
     def forward(self, x: ComplexTensor, state: torch.Tensor | None = None, return_state: bool = False):
         q, k, v = (self._heads(p(x)) for p in (self.q, self.k, self.v))
