@@ -186,6 +186,15 @@ def test_norm_entry_refuses():
                   None)
 
 
+@pytest.mark.parametrize("work", [4097, 4100, 4104])
+def test_norm_entry_refuses_a_misaligned_work_area(work):
+    """Its sums are stored 8 and 16 bytes at a time."""
+    with pytest.raises(ValueError, match="misaligned work"):
+        _lib.call("trnfft_group_norm", 64, None, None, 64, None, None, 2, 300, 12, 3, 1e-5, 0, 0, work, 0, None)
+    with pytest.raises(ValueError, match="misaligned work"):
+        _lib.call("trnfft_group_norm_backward", 64, 64, None, None, 64, 64, 64, None, None, 2, 300, 12, 3, 0, 0, work, 0, None)
+
+
 def test_layers_have_their_parameters():
     assert set(GroupNorm(2, 8).state_dict()) == {"weight", "bias"}
     assert not GroupNorm(2, 8, affine=False).state_dict()

@@ -341,6 +341,7 @@ int trnfft_group_norm(const void* x, const float* weight, const float* bias, voi
     return bad(TRNFFT_INVALID_VALUE, "%s: misaligned pointer", fn);
   if (!work && group_norm_work_bytes((ElemType)dtype, a, false))
     return bad(TRNFFT_INVALID_VALUE, "%s: null work area", fn);
+  if (misaligned(work, 16)) return bad(TRNFFT_INVALID_VALUE, "%s: misaligned work area", fn);
   a.x = x;
   a.y = y;
   a.weight = weight;
@@ -363,6 +364,7 @@ int trnfft_group_norm_backward(const void* x, const void* dy, const float* weigh
   GroupNormArgs a;
   int rc = norm_args(fn, a, batch, spots, channels, groups, activation, dtype);
   if (rc) return rc;
+  if (misaligned(work, 16)) return bad(TRNFFT_INVALID_VALUE, "%s: misaligned work area", fn);
   OnDevice d(device);
   if (!d.ok) return bad(TRNFFT_CUDA_ERROR, "%s: cannot select device %d", fn, device);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
