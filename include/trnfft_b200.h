@@ -371,7 +371,8 @@ TRNFFT_API int trnfft_decay_attention_backward(const trnfft_decay_shape* shape, 
 /* One new token of each of `batch` streams: q (batch, heads, key_width),
  * k and v (batch, kv_heads, width) with strides of batch and head; states
  * (batch, heads, key_width, value_width), each stream's contiguous; o
- * (batch, heads, value_width) contiguous.  new_state may be state itself. */
+ * (batch, heads, value_width) contiguous.  new_state is state itself or
+ * overlaps it nowhere (the states of two buffers may interleave at one stride). */
 typedef struct {
   int64_t batch, heads, kv_heads, key_width, value_width;
   int64_t q_stride[2], k_stride[2], v_stride[2];

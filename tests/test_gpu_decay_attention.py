@@ -583,3 +583,26 @@ def test_infinite_states_stay_infinite(dtype, d, t):
     _, s = trnfft.decay_attention(q, k, v, g, initial_state=one, return_state=True)
     (di,) = torch.autograd.grad(s, one, dlast)
     same_infinities(di, dlast.double() * torch.exp(g.double() * t).clamp_min(1e-300)[:, None, None], 1e-5, "gradient of the state")
+
+
+def test_step_between_two_buffers_of_one_pool():
+    """Old and new states of the streams side by side, each stream's in turn: they interleave, and do not overlap."""
+    b, h, dk, dv = 5, 2, 8, 12
+    q, k, v, _ = (x[:, 0] for x in inputs(b, 1, h, h, dk, dv, torch.float32, seed=26))
+    g = rates(h)
+    pool = torch.randn(b, 3, h, dk, dv, device="cuda")
+    kept = pool.clone()
+    want, ws = trnfft.decay_attention_step(q, k, v, g, pool[:, 0].contiguous())
+    for old, new in ((0, 1), (0, 2), (1, 0), (2, 1)):
+        pool.copy_(kept)
+        pool[:, old] = kept[:, 0]
+        o, got = trnfft.decay_attention_step(q, k, v, g, pool[:, old], new_state=pool[:, new])
+        assert torch.equal(o, want) and torch.equal(got, ws) and torch.equal(pool[:, old], kept[:, 0])
+        third = 3 - old - new
+        assert torch.equal(pool[:, third], kept[:, third])
+    one = h * dk * dv
+    flat = pool.view(-1)
+    for off in (1, one - 1, 2 * one + 1, 3 * one - 1, 3 * one):
+        shifted = torch.as_strided(flat, (b - 1, h, dk, dv), (3 * one, dk * dv, dv, 1), off)
+        with pytest.raises(ValueError, match="overlaps"):
+            trnfft.decay_attention_step(q[:-1], k[:-1], v[:-1], g, pool[:-1, 0], new_state=shifted)

@@ -271,7 +271,12 @@ int trnfft_decay_attention_step(const trnfft_decay_step_shape* s, const void* q,
   const char* a0 = reinterpret_cast<const char*>(state);
   const char* b0 = reinterpret_cast<const char*>(new_state);
   const int64_t an = 4 * ((s->batch - 1) * s->state_stride + one), bn = 4 * ((s->batch - 1) * s->new_state_stride + one);
-  if (a0 == b0 ? s->state_stride != s->new_state_stride : (a0 < b0 + bn && b0 < a0 + an))
+  bool apart = a0 >= b0 + bn || b0 >= a0 + an;
+  if (s->state_stride == s->new_state_stride) {  // each new state between two old ones, or in the place of one's own
+    const int64_t step = 4 * s->state_stride, off = ((b0 - a0) % step + step) % step;
+    apart = apart || a0 == b0 || (off >= 4 * one && off <= step - 4 * one);
+  }
+  if (!apart)
     return bad(TRNFFT_INVALID_VALUE, "%s: the new state overlaps the old one without being it", fn);
   DecayStepArgs a;
   std::memset(&a, 0, sizeof a);
