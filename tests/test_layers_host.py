@@ -61,6 +61,13 @@ def test_step_refuses():
         trnfft.decay_attention_step(q.requires_grad_(), k, v, g, s)
 
 
+def test_step_refuses_to_write_into_a_leaf_of_a_graph():
+    q, k, v, g = qkv()
+    s = torch.zeros(2, 4, 8, 6)
+    with pytest.raises(ValueError, match="no gradient"):
+        trnfft.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, s, new_state=s.clone().requires_grad_())
+
+
 def test_group_norm_refuses():
     x = torch.zeros(2, 5, 12)
     for args, kw, match in [((x[0, 0], 3), {}, "batch"), ((x.double(), 3), {}, "float32"), ((x, 5), {}, "fall into"),

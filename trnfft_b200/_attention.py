@@ -195,7 +195,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
         _check_heads(fn, q, k, v, log_decay, 3)
     b, h, dk = qs
     dv = vs[2]
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, v, log_decay, state)):
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, log_decay, state, new_state)):
         raise ValueError(f"{fn}: has no gradient; use decay_attention, or torch.no_grad()")
     if fwd._current_level >= 0:
         refuse_tangents(fn, q, k, v, log_decay, state, new_state)
