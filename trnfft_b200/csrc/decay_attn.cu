@@ -10,6 +10,7 @@
 // of them with time reversed (DecayRole); the state of dv's role ends as the
 // gradient of the initial state.
 #include "decay_attn.h"
+#include "decay_chunk.cuh"
 #include "elem.cuh"
 #include "kernels.h"
 
@@ -103,6 +104,76 @@ cudaError_t launch_decay_attention(ElemType t, DecayArgs a, void* work, cudaStre
       return launch_decay_tc(a, st);
     default: return launch_decay_chunks_f16(a, st);
   }
+}
+
+// The states carried into the segments of one (sequence, head, role), in place of the segments' own
+// final states, and the sequence's final state.
+__global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant__ DecayArgs a) {
+  const DecayRole& R = a.role[blockIdx.z];
+  const int h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
+  __shared__ int first_unit;
+  __shared__ long long shared_total;
+  if (threadIdx.x < 32) {
+    long long n = a.tokens;
+    int before = seq * a.segs;
+    if (a.cu) {
+      before = 0;
+      for (int i = threadIdx.x; i < seq; i += 32) {
+        const long long m = chunk::cu_value(a, i + 1) - chunk::cu_value(a, i);
+        before += max(1, (int)(((m < 0 ? 0 : m) + a.seg_len - 1) / a.seg_len));
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
+      n = chunk::cu_value(a, seq + 1) - chunk::cu_value(a, seq);
+      if (n < 0) n = 0;
+    }
+    if (threadIdx.x == 0) {
+      first_unit = before;
+      shared_total = n;
+    }
+  }
+  __syncthreads();
+  const long long total = shared_total, size = (long long)R.wk * R.wv;
+  const int e = blockIdx.y * 256 + threadIdx.x;
+  const int segs = max(1, (int)((total + a.seg_len - 1) / a.seg_len));
+  // (units: what the work area holds; only lengths that are not ascending lead past it)
+  if (e >= size || first_unit + segs > a.units) return;
+  const double ld = a.log_decay[h];
+  const DecayFactor f(exp(ld * a.seg_len), a.log_decay[h]);
+  float s = 0.f;
+  const long long sbase = ((long long)seq * a.heads + h) * size;
+  if (R.first) s = R.first[sbase + e / R.wv * R.first_sk + e % R.wv * R.first_sv];
+  float* p = R.seg + ((long long)first_unit * a.heads + h) * size + e;
+  const long long step = a.heads * size;
+  int i = 0;
+  for (; i + 4 < segs; i += 4, p += 4 * step) {
+    float x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = p[u * step];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      p[u * step] = s;
+      s = f.step(s, x[u]);
+    }
+  }
+  for (; i < segs; ++i, p += step) {
+    const bool end = i == segs - 1;
+    const float x = end && !R.last ? 0.f : *p;
+    *p = s;
+    if (!end) {
+      s = f.step(s, x);
+    } else if (R.last) {
+      const long long n = total - (long long)i * a.seg_len;
+      R.last[sbase + e] = DecayFactor(n ? exp(ld * n) : 1.0, a.log_decay[h]).step(s, x);
+    }
+  }
+}
+
+cudaError_t launch_decay_scan(const DecayArgs& a, cudaStream_t st) {
+  int size = 0;
+  for (int i = 0; i < a.roles; ++i) size = max(size, a.role[i].wk * a.role[i].wv);
+  k_decay_scan<<<dim3((unsigned)a.nseq * a.heads, (size + 255) / 256, a.roles), 256, 0, st>>>(a);
+  return cudaGetLastError();
 }
 
 template <typename T>

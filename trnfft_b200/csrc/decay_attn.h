@@ -83,6 +83,10 @@ cudaError_t launch_decay_chunks_f32(const DecayArgs& a, cudaStream_t st);
 cudaError_t launch_decay_chunks_bf16(const DecayArgs& a, cudaStream_t st);
 cudaError_t launch_decay_chunks_f16(const DecayArgs& a, cudaStream_t st);
 cudaError_t launch_decay_tc(const DecayArgs& a, cudaStream_t st);
+// The blocks of a pass (chunk::Pass) that the tensor-core kernel has flagged, walked with care.
+cudaError_t launch_decay_flagged_bf16(const DecayArgs& a, int pass, cudaStream_t st);
+// The states carried into the segments, from the segments' own.
+cudaError_t launch_decay_scan(const DecayArgs& a, cudaStream_t st);
 
 // out[row][hk][w] = sum over g < group of in[row][hk*group + g][w], float32 in, element type out.
 cudaError_t launch_sum_heads(ElemType t, const float* in, void* out, long long rows, int kv_heads, int group, int width,

@@ -104,7 +104,8 @@ __device__ __forceinline__ void mma_parts(float (&d)[4], const Frag<4, PA>& a, c
 }
 
 // The same with the products of a second part in a sum of their own, so that the first parts' sum is
-// truncated once, not three times, for each 8 terms (o of 64 x 64 heads: 1.2e-6 -> 4e-7 off).
+// truncated once, not three times, for each 8 terms (o of 64 x 64 heads: 1.3e-6 -> 6e-7 off; the packed
+// call above: 66 -> 71 us).
 __device__ __forceinline__ void mma_apart(float (&d)[4], float (&rest)[4], const Frag<4, 2>& a, const Frag<2, 2>& b) {
   mma_tf32(rest, a.p[0], b.p[1][0], b.p[1][1]);
   mma_tf32(rest, a.p[1], b.p[0][0], b.p[0][1]);
@@ -747,69 +748,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<T, D0, D1>::kBlocks))
     walk<T, D1, D0>(a, R, pass, sm);
 }
 
-// The states carried into the segments of one (sequence, head, role), in place of the segments' own
-// final states, and the sequence's final state.
-static __global__ void __launch_bounds__(256) k_decay_scan(const __grid_constant__ DecayArgs a) {
-  const DecayRole& R = a.role[blockIdx.z];
-  const int h = blockIdx.x % a.heads, seq = blockIdx.x / a.heads;
-  __shared__ int first_unit;
-  __shared__ long long shared_total;
-  if (threadIdx.x < 32) {
-    long long n = a.tokens;
-    int before = seq * a.segs;
-    if (a.cu) {
-      before = 0;
-      for (int i = threadIdx.x; i < seq; i += 32) {
-        const long long m = cu_value(a, i + 1) - cu_value(a, i);
-        before += max(1, (int)(((m < 0 ? 0 : m) + a.seg_len - 1) / a.seg_len));
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
-      n = cu_value(a, seq + 1) - cu_value(a, seq);
-      if (n < 0) n = 0;
-    }
-    if (threadIdx.x == 0) {
-      first_unit = before;
-      shared_total = n;
-    }
-  }
-  __syncthreads();
-  const long long total = shared_total, size = (long long)R.wk * R.wv;
-  const int e = blockIdx.y * 256 + threadIdx.x;
-  const int segs = max(1, (int)((total + a.seg_len - 1) / a.seg_len));
-  // (units: what the work area holds; only lengths that are not ascending lead past it)
-  if (e >= size || first_unit + segs > a.units) return;
-  const double ld = a.log_decay[h];
-  const DecayFactor f(exp(ld * a.seg_len), a.log_decay[h]);
-  float s = 0.f;
-  const long long sbase = ((long long)seq * a.heads + h) * size;
-  if (R.first) s = R.first[sbase + e / R.wv * R.first_sk + e % R.wv * R.first_sv];
-  float* p = R.seg + ((long long)first_unit * a.heads + h) * size + e;
-  const long long step = a.heads * size;
-  int i = 0;
-  for (; i + 4 < segs; i += 4, p += 4 * step) {
-    float x[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = p[u * step];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      p[u * step] = s;
-      s = f.step(s, x[u]);
-    }
-  }
-  for (; i < segs; ++i, p += step) {
-    const bool end = i == segs - 1;
-    const float x = end && !R.last ? 0.f : *p;
-    *p = s;
-    if (!end) {
-      s = f.step(s, x);
-    } else if (R.last) {
-      const long long n = total - (long long)i * a.seg_len;
-      R.last[sbase + e] = DecayFactor(n ? exp(ld * n) : 1.0, a.log_decay[h]).step(s, x);
-    }
-  }
-}
-
 template <typename T, int D0, int D1>
 static cudaError_t run_widths(const DecayArgs& a, Pass pass, cudaStream_t st) {
   constexpr int smem = Shape<T, D0, D1>::kSmem > Shape<T, D1, D0>::kSmem ? Shape<T, D0, D1>::kSmem : Shape<T, D1, D0>::kSmem;
@@ -829,18 +767,11 @@ cudaError_t run_chunks(const DecayArgs& a, Pass pass, cudaStream_t st) {
   return lo == 64 ? run_widths<T, 64, 128>(a, pass, st) : run_widths<T, 128, 128>(a, pass, st);
 }
 
-inline cudaError_t run_scan(const DecayArgs& a, cudaStream_t st) {
-  int size = 0;
-  for (int i = 0; i < a.roles; ++i) size = max(size, a.role[i].wk * a.role[i].wv);
-  k_decay_scan<<<dim3((unsigned)a.nseq * a.heads, (size + 255) / 256, a.roles), 256, 0, st>>>(a);
-  return cudaGetLastError();
-}
-
 template <typename T>
 cudaError_t run_all(const DecayArgs& a, cudaStream_t st) {
   if (!a.split) return run_chunks<T>(a, kWhole, st);
   cudaError_t e = run_chunks<T>(a, kLocal, st);
-  if (e == cudaSuccess) e = run_scan(a, st);
+  if (e == cudaSuccess) e = launch_decay_scan(a, st);
   return e == cudaSuccess ? run_chunks<T>(a, kCarried, st) : e;
 }
 

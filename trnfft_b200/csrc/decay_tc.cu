@@ -12,9 +12,10 @@
 // serve as K-major and, with rows as K, as MN-major operand.
 //
 // Precision: q k^T is exact up to float32 sums.  P and C are multiplied in two
-// bfloat16 parts each (2^-17), k' in three (2^-25): with one part each, rounding
+// bfloat16 parts each (2^-16: the first is cut off, which leaves up to 2^-7, and
+// the rest rounded to 8 bits), k' in three (2^-24): with one part each, rounding
 // P and C alone would double the error that the rounding of o makes, and the
-// state, a float32 result, would be off by 2^-9.  C itself stays in float32
+// state, a float32 result, would be off by 2^-8.  C itself stays in float32
 // registers and is scaled by g^n as a sum of two float32.
 //
 // One block per (segment, head, role), 12 warps:
@@ -60,8 +61,9 @@ struct Shape {
   static constexpr int kSHi = 5 * kTile, kSLo = kSHi + kState, kTable = kSLo + kState;
   static constexpr int kSmem = kTable + (int)sizeof(float) * 3 * 132 + 14 * 8 + 64;
   // TMEM columns: P (also in two bfloat16 parts), O, X, E.  With D = 64, E shares X's (256 columns
-  // in all); X is then read before E is issued.  (80 registers a thread, for two blocks on an SM, spill:
-  // 8 x 4096 tokens of 16 heads of 64 take 177 us with two blocks, 153 us with one.)
+  // in all); X is then read before E is issued.  That and the shared memory would let two blocks share
+  // an SM, but at 80 registers a thread they spill: 8 x 4096 tokens of 16 heads of 64 take 177 us with
+  // two blocks, 153 us with one, which leaves the other half of both unused.
   static constexpr int kP = 0, kO = 128, kX = 128 + D, kE = D == 64 ? kX : kX + D;
   static constexpr int kColumns = D == 64 ? 256 : 512;
   static constexpr bool kShared = D == 64;
@@ -734,12 +736,12 @@ cudaError_t launch_decay_tc(const DecayArgs& a, cudaStream_t st) {
     DecayArgs b = a;
     b.flags = nullptr;
     e = wide <= 64 ? tc::run_tc<64>(b, maps, chunk::kLocal, st) : tc::run_tc<128>(b, maps, chunk::kLocal, st);
-    if (e == cudaSuccess) e = chunk::run_scan(a, st);
+    if (e == cudaSuccess) e = launch_decay_scan(a, st);
     if (e != cudaSuccess) return e;
   }
   e = wide <= 64 ? tc::run_tc<64>(a, maps, last, st) : tc::run_tc<128>(a, maps, last, st);
   if (e != cudaSuccess) return e;
-  return chunk::run_chunks<__nv_bfloat16>(a, last, st);  // the blocks that said so, and no others
+  return launch_decay_flagged_bf16(a, last, st);  // the blocks that said so, and no others
 }
 
 }  // namespace tfb

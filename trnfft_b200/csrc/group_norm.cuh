@@ -172,8 +172,9 @@ cudaError_t allow_smem(int bytes) {
   return bytes <= 48 * 1024 ? cudaSuccess : allow_shared<K>(kMostShared);
 }
 
-// c / w for 0 <= c < 2^14, w >= 1, where inv = 1.f / w: (c + 1/2) / w is at least 1 / (2 w) from a whole
-// number, and the rounding is below 2^14 / w * 2^-22.
+// c / w for 0 <= c < 2^20, w >= 1, where inv = 1.f / w: (c + 1/2) / w is at least 1 / (2 w) from a whole
+// number, c + 1/2 is exact, and inv and the product are off by 2^-24 of themselves each: by less than
+// c / w * 2^-22 < 1 / (2 w) together.  (kSplit has at most 25600 channels: their sets fill kMaxSplitSmem.)
 __device__ __forceinline__ int quotient(int c, float inv) { return (int)(((float)c + 0.5f) * inv); }
 
 // A block's rows of a sample, part k, and a thread's place among them: its column of a tile of
