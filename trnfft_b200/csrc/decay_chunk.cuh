@@ -19,9 +19,10 @@
 // chunk's sum starts from 0 and is added to the scaled C in round-to-nearest,
 // with g^n as the sum of two float32 (decay_state.cuh).
 //
-// Bound by instruction issue: 112501 tokens of 8 heads of 64 x 64 in float16
-// take 543 us in segments (501 us with one part of P and C), a packed float32
-// call of 2517 rows 71 us.
+// Bound by instruction issue and the tensor pipe together (55 and 46 % of
+// their cycles with two blocks of 8 warps per SM, 64 x 64 float16): 112501
+// tokens of 8 such heads take 531 us in segments (501 us with one part of P and
+// C), a packed float32 call of 2517 rows 72-77 us.
 #pragma once
 
 #include <type_traits>
