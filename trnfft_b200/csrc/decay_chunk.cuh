@@ -208,7 +208,7 @@ struct Shape {
   static constexpr int kSmem = kStages * kTile + kState + kTable;
   static constexpr int kBlocks = kSmem <= 113 * 1024 && DK * DV <= 64 * 64 ? 2 : 1;  // per SM
   static_assert(kSmem <= 227 * 1024, "shared memory");
-  static_assert(2 * DK * DV * 4 <= kStages * kTile + kState, "walk_with_care keeps two states");
+  static_assert(4 * (DK * DV + 8 * (2 * DK + DV + kThreads)) <= kStages * kTile + kState, "walk_with_care");
   // state: warps tile DK in blocks of 16 rows, the rest of them the columns
   static constexpr int kSRows = DK / 16 < 8 ? DK / 16 : 8, kSCols = 8 / kSRows;
   static constexpr int kSTiles = DV / 8 / kSCols;          // 8-column tiles of a warp
@@ -317,20 +317,19 @@ struct Place {
 
 // The same segment token by token, one product at a time, where the walk's states do not end finite.  In
 // the walk an infinite factor in two parts makes NaN of sums that are infinite, and keys behind a row
-// have weight 0 in P, but 0 times an infinite or NaN value is NaN.  Here, with A_t = sum_{s<=t} g^{t-s}
-// k_s v_s^T from 0 and B_t = g^{t+1-back} C, o_t = a q_t A_t + r q_t B_t and C' = g^n C + c g^back A.
+// have weight 0 in P, but 0 times an infinite or NaN value is NaN.  All roles have a = r c, so here
+//   forwards   S = g S + c k v^T,  o = r q S        backwards   S = S + c k v^T,  o = r q S,  S = g S
+// from S = C, and C' = S.  kCare tokens at a time: their rows in shared memory as float32, and a thread
+// takes each of its elements of S through all of them (8 x 4096 tokens of 16 heads of 128,
+// every head with a NaN: 9 ms).
+constexpr int kCare = 8;
 template <typename T>
-__device__ __forceinline__ void walk_with_care(const DecayArgs& a, const DecayRole& R, int pass, const Segment& seg, const DecayFactor& factor,
-                                            float* sm) {
+__device__ __forceinline__ void walk_with_care(const DecayArgs& a, const DecayRole& R, int pass, const Segment& seg,
+                                               const DecayFactor& factor, float* sm) {
   const int h = blockIdx.x % a.heads, unit = blockIdx.x / a.heads, tid = threadIdx.x;
   const Place at(a, R, seg, unit, h);
-  const T* q = static_cast<const T*>(R.q) + at.batch * R.qs[0] + (long long)(h / R.qdiv) * R.qs[2];
-  const T* k = static_cast<const T*>(R.k) + at.batch * R.ks[0] + (long long)(h / R.kdiv) * R.ks[2];
-  const T* v = static_cast<const T*>(R.v) + at.batch * R.vs[0] + (long long)(h / R.vdiv) * R.vs[2];
-  const bool want_o = R.o && pass != kLocal;
-  const int size = R.wk * R.wv;
-  float *A = sm, *B = A + size;
-  __shared__ float red[kThreads];
+  const bool want_o = R.o && pass != kLocal, back = R.back;
+  float *S = sm, *sk = S + (R.wk * R.wv + 3) / 4 * 4, *sq = sk + kCare * R.wk, *sv = sq + kCare * R.wk, *red = sv + kCare * R.wv;
   const DecayFactor f = factor;
   // a thread has one column and every `step`-th row
   int columns = 1;
@@ -340,49 +339,81 @@ __device__ __forceinline__ void walk_with_care(const DecayArgs& a, const DecayRo
   __syncthreads();
 #pragma unroll 1
   for (int d = tid / columns; mine && d < R.wk; d += step) {
-    A[d * R.wv + col] = 0.f;
     float x = 0.f;
     if (pass == kCarried) x = at.seg_state[d * R.wv + col];
     if (pass == kWhole && R.first) x = R.first[at.sbase + d * R.first_sk + col * R.first_sv];
-    B[d * R.wv + col] = x;
+    S[d * R.wv + col] = x;
   }
 #pragma unroll 1
-  for (long long i = 0; i < seg.len; ++i) {
-    const long long token = R.back ? at.row0 - i : at.row0 + i;
-    float x = 0.f, y = 0.f;
-    const float vc = mine ? to_f32(v[token * R.vs[1] + col]) : 0.f;
+  for (long long i = 0; i < seg.len; i += kCare) {
+    const int rows = (int)min((long long)kCare, seg.len - i);
+    const long long token = R.back ? at.row0 - i : at.row0 + i;  // of row 0; the others follow in time
+    auto stage = [&](float* to, const void* from, const long long* stride, int div, int width) {
+      const T* p = static_cast<const T*>(from) + at.batch * stride[0] + (long long)(h / div) * stride[2];
+#pragma unroll 1
+      for (int e = tid; e < rows * width; e += kThreads) {
+        const int r = e / width, x = e % width;
+        to[x * kCare + r] = to_f32(p[(token + (R.back ? -r : r)) * stride[1] + x]);
+      }
+    };
+    stage(sk, R.k, R.ks, R.kdiv, R.wk);
+    stage(sv, R.v, R.vs, R.vdiv, R.wv);
+    if (want_o) stage(sq, R.q, R.qs, R.qdiv, R.wk);
+    __syncthreads();
+    float v[kCare], o[kCare];
+#pragma unroll
+    for (int r = 0; r < kCare; ++r) {
+      v[r] = mine && r < rows ? R.c * sv[col * kCare + r] : 0.f;
+      o[r] = 0.f;
+    }
 #pragma unroll 1
     for (int d = tid / columns; mine && d < R.wk; d += step) {
-      float &Ad = A[d * R.wv + col], &Bd = B[d * R.wv + col];
-      const float b = Bd, next = f.step(b, 0.f);
-      Ad = f.step(Ad, to_f32(k[token * R.ks[1] + d]) * vc);
-      Bd = next;
-      if (want_o) {
-        const float qd = to_f32(q[token * R.qs[1] + d]);
-        x = fmaf(qd, Ad, x);
-        y = fmaf(qd, R.back ? b : next, y);
+      float x = S[d * R.wv + col], k[kCare], q[kCare];
+#pragma unroll
+      for (int r = 0; r < kCare; r += 4) {
+        const float4 k4 = *reinterpret_cast<const float4*>(sk + d * kCare + r), q4 = *reinterpret_cast<const float4*>(sq + d * kCare + r);
+        k[r] = k4.x, k[r + 1] = k4.y, k[r + 2] = k4.z, k[r + 3] = k4.w;
+        q[r] = q4.x, q[r + 1] = q4.y, q[r + 2] = q4.z, q[r + 3] = q4.w;
       }
+      if (back) {
+#pragma unroll
+        for (int r = 0; r < kCare; ++r)
+          if (r < rows) {
+            x += k[r] * v[r];
+            o[r] = fmaf(q[r], x, o[r]);
+            x = f.step(x, 0.f);
+          }
+      } else {
+#pragma unroll
+        for (int r = 0; r < kCare; ++r)
+          if (r < rows) {
+            x = f.step(x, k[r] * v[r]);
+            o[r] = fmaf(q[r], x, o[r]);
+          }
+      }
+      S[d * R.wv + col] = x;
     }
+    if (want_o) {
+#pragma unroll
+      for (int r = 0; r < kCare; ++r) red[r * kThreads + tid] = o[r];
+    }
+    __syncthreads();
     if (!want_o) continue;
-    red[tid] = R.a * x + R.r * y;
-    __syncthreads();
-    if (tid < R.wv) {
-      float o = 0.f;
 #pragma unroll 1
-      for (int j = 0; j < step; ++j) o += red[j * columns + tid];
-      const long long to = at.batch * R.os[0] + (long long)h * R.os[2] + token * R.os[1] + tid;
-      if (R.o_f32) static_cast<float*>(R.o)[to] = o;
-      else static_cast<T*>(R.o)[to] = from_f32<T>(o);
+    for (int e = tid; e < rows * R.wv; e += kThreads) {
+      const int r = e / R.wv, x = e % R.wv;
+      float sum = 0.f;
+#pragma unroll 1
+      for (int j = 0; j < step; ++j) sum += red[r * kThreads + j * columns + x];
+      const long long to = at.batch * R.os[0] + (long long)h * R.os[2] + (token + (R.back ? -r : r)) * R.os[1] + x;
+      if (R.o_f32) static_cast<float*>(R.o)[to] = R.r * sum;
+      else static_cast<T*>(R.o)[to] = from_f32<T>(R.r * sum);
     }
-    __syncthreads();
   }
   float* to = pass == kLocal ? at.seg_state : (pass == kWhole && R.last ? R.last + at.sbase : nullptr);
   if (!to) return;
 #pragma unroll 1
-  for (int d = tid / columns; mine && d < R.wk; d += step) {
-    const float s = A[d * R.wv + col];
-    to[d * R.wv + col] = fmaf(R.c, R.back ? f.step(s, 0.f) : s, B[d * R.wv + col]);
-  }
+  for (int d = tid / columns; mine && d < R.wk; d += step) to[d * R.wv + col] = S[d * R.wv + col];
 }
 
 template <typename T, int DK, int DV>
