@@ -606,3 +606,20 @@ def test_step_between_two_buffers_of_one_pool():
         shifted = torch.as_strided(flat, (b - 1, h, dk, dv), (3 * one, dk * dv, dv, 1), off)
         with pytest.raises(ValueError, match="overlaps"):
             trnfft.decay_attention_step(q[:-1], k[:-1], v[:-1], g, pool[:-1, 0], new_state=shifted)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_nan_decay_is_not_hidden(dtype):
+    """A head whose log_decay is NaN has no number in its state or, from a carried state, in its outputs."""
+    q, k, v, _ = inputs(1, 70, 3, 3, 64, 64, dtype, seed=27)
+    g = rates(3)
+    first = torch.randn(1, 3, 64, 64, device="cuda")
+    want, ws = trnfft.decay_attention(q, k, v, g, initial_state=first, return_state=True)
+    g[1] = math.nan
+    o, s = trnfft.decay_attention(q, k, v, g, initial_state=first, return_state=True)
+    assert bool(s[:, 1].isnan().all()) and bool(o[:, :, 1].isnan().all())
+    assert torch.equal(o[:, :, ::2], want[:, :, ::2]) and torch.equal(s[:, ::2], ws[:, ::2])
+    state = first.clone()
+    o, _ = trnfft.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state)
+    assert bool(state[:, 1].isnan().all()) and bool(o[:, 1].isnan().all())
+    assert bool(torch.isfinite(state[:, ::2]).all()) and bool(torch.isfinite(o[:, ::2]).all())

@@ -21,9 +21,10 @@ struct DecayFactor {
   __device__ __forceinline__ DecayFactor(double g, float log_decay) {
     hi = __double2float_rz(g);
     const float rest = (float)(g - (double)hi);
-    const float least = log_decay > -INFINITY ? __uint_as_float(1u) : 0.f;
-    hi = fmaxf(hi, least);
-    lo = fmaxf(rest, least);  // (of an infinite g the rest is NaN, and lo the least)
+    const float least = __uint_as_float(1u);
+    const bool above = log_decay > -INFINITY;  // (not of NaN, which both parts keep)
+    hi = above ? fmaxf(hi, least) : hi;
+    lo = above ? fmaxf(rest, least) : rest;  // (of an infinite g the rest is NaN, and lo the least)
   }
   __device__ __forceinline__ float step(float s, float x) const { return fmaf(s, hi, fmaf(s, lo, x)); }
 };
